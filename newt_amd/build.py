@@ -8,10 +8,14 @@
     is compiled offline with hipcc for gfx950, instantiating every template the
     code generator emits, so a broken header fails the build instead of the
     first kernel launch.
+  * libnewt_ops.so - the hand-written operators (include/newt_ops.h, csrc/ops),
+    compiled by hipcc for gfx950, a file at a time side by side.
 
 Run: python -m newt_amd.build
 """
 
+import concurrent.futures
+import glob
 import os
 import subprocess
 import sys
@@ -108,6 +112,26 @@ def check_device_header():
     return out
 
 
+def build_operators():
+    """The hand-written operators: every csrc/ops/*.hip into one library."""
+    wdir = os.path.join(CSRC, "_build")
+    os.makedirs(wdir, exist_ok=True)
+    hipcc = os.path.join(ROCM, "bin", "hipcc")
+    flags = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wno-pass-failed", *HIP_FLAGS]
+
+    def compile_one(src):
+        obj = os.path.join(wdir, os.path.basename(src) + ".o")
+        _run([hipcc, *flags, f"-I{os.path.join(CSRC, 'device')}", "-c", src, "-o", obj])
+        return obj
+
+    out = os.path.join(CSRC, "libnewt_ops.so")
+    with concurrent.futures.ThreadPoolExecutor(4) as pool:
+        objects = list(pool.map(compile_one, sorted(glob.glob(os.path.join(CSRC, "ops", "*.hip")))))
+    _run([hipcc, "--offload-arch=gfx950", "-shared", "-fPIC", *objects, "-o", out + ".tmp"])
+    os.replace(out + ".tmp", out)
+    return out
+
+
 def build(verbose=True):
     lib = build_library()
     if verbose:
@@ -115,6 +139,9 @@ def build(verbose=True):
     launcher = build_launcher()
     if verbose:
         print("built", launcher)
+    operators = build_operators()
+    if verbose:
+        print("built", operators)
     co = check_device_header()
     if verbose:
         print("device header compiled for gfx950:", co)

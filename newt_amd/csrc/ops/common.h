@@ -1,0 +1,49 @@
+// What the operators of libnewt_ops.so share: error reporting at the C entries,
+// element conversions and reductions over a workgroup. Device templates
+// (vector accesses, wave64 butterflies, MFMA wrappers, LDS tiles) come from
+// newt_gfx950.h, the header of the compiled kernels.
+#pragma once
+#include <hip/hip_runtime.h>
+
+#include <type_traits>
+
+#include "../../../include/newt_ops.h"
+#include "newt_gfx950.h"
+
+namespace newt_ops {
+
+// Keeps the message of the calling thread's last failure; fixed storage, so
+// that reporting an error cannot fail itself.
+int fail(int status, const char* format, ...) __attribute__((format(printf, 2, 3)));
+
+// The status of a kernel launch just made.
+int launched(const char* what);
+
+// What is wrong with a cache's description, or null.
+const char* cache_wrong(const newt_kv_cache& c);
+
+// ---------------------------------------------------------------------------
+// workgroup reductions: each wave's partial through LDS, read back by all.
+// `slot` needs one float per wave; a second reduction takes another slot or a
+// barrier between.
+// ---------------------------------------------------------------------------
+template <typename Op, int WAVES>
+__device__ __forceinline__ float block_reduce(float v, float* slot) {
+  v = newt::lane_reduce<Op, 63>(v);
+  if constexpr (WAVES > 1) {
+    if ((threadIdx.x & 63) == 0) slot[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = slot[0];
+#pragma unroll
+    for (int i = 1; i < WAVES; ++i) v = Op::op(v, slot[i]);
+  }
+  return v;
+}
+
+// Four floats to four e4m3 bytes, rounded to nearest even by the hardware.
+__device__ __forceinline__ u32 to_e4m3x4(float a, float b, float c, float d) {
+  int w = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+  return (u32)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true);
+}
+
+}  // namespace newt_ops

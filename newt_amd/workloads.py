@@ -29,7 +29,12 @@ reference's examples/01-05), extended to the benchmark configurations:
                     scale <= 0
   dt_matmul         examples/deuteron/01_matmul.py (unchanged body): the tile
                     DSL traced to newt and autotuned against its eager oracle
-Everything is compiled by newt_amd's compiler to HIP for gfx950.
+Everything above is compiled by newt_amd's compiler to HIP for gfx950.
+
+Beside them stand the operators of a decoder's serving step, written by hand
+in HIP (newt_amd/serving.py): rmsnorm with the residual's addition and an 8-bit
+output, window_attention, the 8-bit cache with kv_append and cached_attention,
+and token_logprobs.
 """
 
 import functools
@@ -38,6 +43,9 @@ import torch
 
 import newt_amd as newt
 import newt_amd.language as nl
+
+from .serving import (KVCache, cached_attention, kv_append, kv_cache, rmsnorm,  # noqa: F401
+                      token_logprobs, window_attention)
 
 
 # ---------------------------------------------------------------------------
