@@ -83,51 +83,71 @@ struct Parts {
   }
 };
 
+constexpr int kMostSplits = 64;  // a lane of the joining wave for each
+
 // o = sum acc_s 2^(m_s - M) / sum l_s 2^(m_s - M); rows that saw nothing are 0.
-// One wave a row.
+// One wave a row: lane s takes split s's maximum and sum, then every lane its
+// dims of all accumulators, whose loads do not wait for each other.
 template <typename T, int D>
 __global__ void __launch_bounds__(256)
 join_splits_kernel(const void* workspace, void* out, Rows o, int64_t units, int splits, int rows,
                    int64_t row_tiles, int64_t q_len, int kv_heads, int group) {
   const Parts parts((void*)workspace, units, splits, rows, D);
   const int lane = threadIdx.x & 63;
+  // rows that exist: row tiles are full but for a unit's last one
+  const int64_t all_rows = q_len * group;
   const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (w >= units * rows) return;
-  const int64_t unit = w / rows;
-  const int row = (int)(w % rows);
-  const int64_t r = unit % row_tiles * rows + row;
-  const int64_t head = unit / row_tiles % kv_heads, b = unit / row_tiles / kv_heads;
-  if (r >= q_len * group) return;
+  if (w >= units / row_tiles * all_rows) return;
+  const int64_t r = w % all_rows, sequence_head = w / all_rows;
+  const int64_t unit = sequence_head * row_tiles + r / rows;
+  const int64_t at = unit * splits * rows + r % rows;  // and `rows` further a split
   constexpr int N = D / 64;
-  float M = -kInf;
-  for (int s = 0; s < splits; ++s)
-    M = newt::Max::op(M, parts.m[(unit * splits + s) * rows + row]);
-  const float ref = M == -kInf ? 0.0f : M;
-  float l = 0.0f, acc[N] = {};
+
+  const float m = lane < splits ? parts.m[at + (int64_t)lane * rows] : -kInf;
+  const float l = lane < splits ? parts.l[at + (int64_t)lane * rows] : 0.0f;
+  const float M = newt::lane_reduce<newt::Max, 63>(m);
+  // without a maximum a split has seen nothing, or NaN
+  const float f = m == -kInf ? 0.0f : __builtin_amdgcn_exp2f(m - M);
+  const float total = newt::lane_reduce<newt::Sum, 63>(m == -kInf ? l : l * f);
+  float acc[N] = {};
+  const float* from = parts.acc + at * D + lane * N;
+#pragma unroll 8
   for (int s = 0; s < splits; ++s) {
-    const int64_t at = (unit * splits + s) * rows + row;
-    const float f = __builtin_amdgcn_exp2f(parts.m[at] - ref);
-    if (parts.m[at] == -kInf) {
-      l += parts.l[at];  // 0, or NaN
-      continue;
-    }
-    l += parts.l[at] * f;
+    const float g = newt::bits_f32(__builtin_amdgcn_readlane(newt::f32_bits(f), s));
     float a[N];
-    newt::load_vec<float, N>(parts.acc + at * D + lane * N, a);
+    newt::load_vec<float, N>(from + (int64_t)s * rows * D, a);
 #pragma unroll
-    for (int i = 0; i < N; ++i) acc[i] += a[i] * f;
+    for (int i = 0; i < N; ++i) acc[i] += a[i] * g;
   }
   T t[N];
 #pragma unroll
-  for (int i = 0; i < N; ++i) t[i] = (T)(l == 0.0f ? 0.0f : acc[i] / l);
+  for (int i = 0; i < N; ++i) t[i] = (T)(total == 0.0f ? 0.0f : acc[i] / total);
+  const int64_t head = sequence_head % kv_heads, b = sequence_head / kv_heads;
   T* to = (T*)out + o.at(b, head * group + r % group, r / group) + lane * N;
   newt::store_vec<T, N>(to, t, newt::any_align());
+}
+
+// Splits of a program's tiles: `want` programs in all where `units` alone are
+// fewer, each split with at least `least` of the at most `tiles` tiles.
+inline int split_count(int64_t units, int64_t tiles, int64_t want, int64_t least) {
+  int64_t n = (want + units - 1) / units;
+  const int64_t most = (tiles + least - 1) / least;
+  n = n < most ? n : most;
+  return (int)(n < 1 ? 1 : n < kMostSplits ? n : kMostSplits);
+}
+
+// At most so many tiles can a program of `span` queries visit.
+inline int64_t most_tiles(int64_t keys, int64_t window, int64_t sinks, int64_t span) {
+  const int64_t all = (keys + kTile - 1) / kTile;
+  if (!window) return all;
+  const int64_t some = (window + span + 2 * kTile - 2) / kTile + (sinks + kTile - 1) / kTile;
+  return some < all ? some : all;
 }
 
 template <typename T, int D>
 int join_splits(const void* workspace, void* out, Rows o, int64_t units, int splits, int rows,
                 int64_t row_tiles, int64_t q_len, int kv_heads, int group, hipStream_t stream) {
-  const int64_t waves = units * rows;
+  const int64_t waves = units / row_tiles * q_len * group;
   join_splits_kernel<T, D><<<dim3((unsigned)((waves + 3) / 4)), dim3(256), 0, stream>>>(
       workspace, out, o, units, splits, rows, row_tiles, q_len, kv_heads, group);
   return launched("join_splits");

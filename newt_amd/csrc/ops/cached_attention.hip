@@ -324,7 +324,8 @@ Plan plan(const newt_cached_attention_params& p) {
   r.rows = rows > 16 ? 32 : 16;
   r.row_tiles = (rows + r.rows - 1) / r.rows;
   r.units = p.batch * p.cache.kv_heads * r.row_tiles;
-  r.splits = 1;
+  const int64_t tiles = most_tiles(p.table_width * p.cache.block_size, p.window, p.sinks, p.q_len);
+  r.splits = split_count(r.units, tiles, 1024, kWaves);
   return r;
 }
 
