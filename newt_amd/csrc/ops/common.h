@@ -40,6 +40,12 @@ __device__ __forceinline__ float block_reduce(float v, float* slot) {
   return v;
 }
 
+// The wave's index in its workgroup, as a number that the compiler knows to be
+// the same in all of its lanes.
+__device__ __forceinline__ int wave_id() {
+  return __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+}
+
 // Four floats to four e4m3 bytes, rounded to nearest even by the hardware.
 __device__ __forceinline__ u32 to_e4m3x4(float a, float b, float c, float d) {
   int w = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);

@@ -30,16 +30,39 @@ struct Entry {
   float value;
   int id;
   __device__ __forceinline__ bool before(const Entry& o) const {
-    return value > o.value || (value == o.value && id < o.id);
+    return (value > o.value) | ((value == o.value) & (id < o.id));
   }
 };
+
+// v of the lane that differs in bit M: rotations of 16 lanes, permlane swaps
+// and quad permutations, on the VALU but for M = 4.
+template <int M, typename V>
+__device__ __forceinline__ V partner(V v, int lane) {
+  if constexpr (M >= 16) {
+    V lo, hi;
+    newt::pair_lanes<M>(v, lo, hi);
+    return (lane & M) ? lo : hi;
+  } else if constexpr (M == 8) {
+    return __builtin_bit_cast(
+        V, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0x128, 0xF, 0xF, true));  // row_ror:8
+  } else {
+    return newt::xor_lane<M>(v);
+  }
+}
+
+// v of the lane below; lane 0 keeps its own
+template <typename V>
+__device__ __forceinline__ V below(V v) {
+  const int i = __builtin_bit_cast(int, v);
+  return __builtin_bit_cast(V, __builtin_amdgcn_update_dpp(i, i, 0x138, 0xF, 0xF, false));  // wave_shr:1
+}
 
 // One step of a bitonic network over the lanes: of each pair of lanes that
 // differ in bit M the one with that bit clear keeps the entry that comes first
 // (where `down`, else last).
 template <int M>
 __device__ __forceinline__ void exchange(Entry& e, bool down, int lane) {
-  const Entry o{newt::xor_lane<M>(e.value), newt::xor_lane<M>(e.id)};
+  const Entry o{partner<M>(e.value, lane), partner<M>(e.id, lane)};
   const bool keep_first = ((lane & M) == 0) == down;
   if (o.before(e) == keep_first) e = o;
 }
@@ -82,9 +105,20 @@ __device__ __forceinline__ void merge(Entry& e, const Entry& reversed, int lane)
 // A candidate, the same in every lane, behind all entries that come before it.
 __device__ __forceinline__ void insert(Entry& e, const Entry& c, int lane) {
   const int place = __popcll(__ballot(e.before(c)));
-  const Entry left{__shfl_up(e.value, 1), __shfl_up(e.id, 1)};
+  const Entry left{below(e.value), below(e.id)};
   if (lane > place) e = left;
   if (lane == place) e = c;
+}
+
+// d = (x - m) c by one fma where the product m c is well inside fp32's range:
+// it is rounded, by the same amount in all that is taken relative to this m, so
+// that the rounding cancels in every result. Rows of nothing but the types'
+// lowest numbers take the longer way.
+__device__ __forceinline__ bool near_zero(float m, float c) {
+  return __builtin_fabsf(m * c) < 1e38f;
+}
+__device__ __forceinline__ float distance(float x, float m, float c) {
+  return near_zero(m, c) ? __builtin_fmaf(x, c, -(m * c)) : (x - m) * c;
 }
 
 // The sums over what a lane, a wave or a split has seen.
@@ -94,7 +128,7 @@ struct Sums {
   // The same relative to the maximum `to` >= m.
   __device__ __forceinline__ void rescale(float to, float c) {
     if (!(to > m)) return;
-    const float d = (m - to) * c;
+    const float d = near_zero(to, c) ? m * c - to * c : (m - to) * c;
     const float f = __builtin_amdgcn_exp2f(d);
     if (f == 0.0f && S == S) {
       S = U = 0.0f;
@@ -117,7 +151,7 @@ struct Sums {
 template <typename T>
 __device__ __forceinline__ void finish(const newt_logprobs_params& p, int64_t row, const Sums& s,
                                        const Entry& e, int lane) {
-  const float inv = p.inv_temperature;
+  const float c = kLog2e * p.inv_temperature;
   // every logit -inf: 0 / 0, as a softmax over them gives
   const float lse = s.S > 0.0f ? __builtin_logf(s.S) : __builtin_nanf("");
   if (lane == 0) {
@@ -125,13 +159,14 @@ __device__ __forceinline__ void finish(const newt_logprobs_params& p, int64_t ro
     float logp = __builtin_nanf("");
     if (token == -1) logp = 0.0f;
     else if (token >= 0 && token < p.vocab)
-      logp = (newt::to_f32(((const T*)p.logits)[row * p.stride + token]) - s.m) * inv - lse;
+      logp = distance(newt::to_f32(((const T*)p.logits)[row * p.stride + token]), s.m, c) * kLn2 - lse;
     p.logp[row] = logp;
     p.entropy[row] = lse - kLn2 * (s.U / s.S);
   }
   if (lane < p.top) {
     const bool none = e.id == kNone;
-    p.top_logp[row * p.top + lane] = none ? __builtin_nanf("") : (e.value - s.m) * inv - lse;
+    p.top_logp[row * p.top + lane] =
+        none ? __builtin_nanf("") : distance(e.value, s.m, c) * kLn2 - lse;
     p.top_ids[row * p.top + lane] = none ? -1 : e.id;
   }
 }
@@ -142,16 +177,15 @@ struct Chunk {
   static constexpr int STEP = 64 * V;  // logits of a wave's chunk
   u32x4 raw;
 
-  // V logits from `at` on, -inf behind `hi`
-  __device__ __forceinline__ void load(const T* x, int64_t at, int64_t hi) {
-    if (at + V <= hi) {
-      raw = *reinterpret_cast<const typename newt::any_vec<T, V>::type*>(x + at);
-    } else {
-      T t[V];
+  __device__ __forceinline__ void load(const T* x) {
+    raw = *reinterpret_cast<const typename newt::any_vec<T, V>::type*>(x);
+  }
+  // `n` of V logits, -inf behind
+  __device__ __forceinline__ void load(const T* x, int64_t n) {
+    newt::vec_t<T, V> t;
 #pragma unroll
-      for (int i = 0; i < V; ++i) t[i] = at + i < hi ? x[at + i] : (T)-kInf;
-      raw = __builtin_bit_cast(u32x4, *reinterpret_cast<newt::vec_t<T, V>*>(t));
-    }
+    for (int i = 0; i < V; ++i) t.d[i] = i < n ? x[i] : (T)-kInf;
+    raw = __builtin_bit_cast(u32x4, t);
   }
   __device__ __forceinline__ void get(float* f) const {
     const auto t = __builtin_bit_cast(newt::vec_t<T, V>, raw);
@@ -172,26 +206,22 @@ struct Wave {
   Entry last{-kInf, kNone};   // the last entry that counts
   bool begun = false;
 
-  // Candidates of a chunk, in the order of their ids. `taken` marks, in the
-  // first chunk, the logit that a lane gave to the list already.
-  __device__ __forceinline__ void candidates(const float* f, float most, int64_t at, int taken) {
-    // `most` may equal the last entry and still come before it, but later ids
-    // never come before earlier ones unless there are entries that are none
-    const bool equal = taken >= 0 || last.id == kNone;
-    u64 found = __ballot(equal ? most >= last.value : most > last.value);
-    while (found) {
-      const int from = __builtin_ctzll(found);
-      found &= found - 1;
-      const int skip = __builtin_amdgcn_readlane(taken, from);
+  // Candidates of a chunk into the list, whose last entry that counts decides
+  // which ones are. `taken`: the logit that the lane gave to the list already.
+  __device__ __forceinline__ void candidates(const float* f, int64_t at, int taken) {
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const Entry x{uniform(f[i], from), (int)(at + from * V + i)};
-        if (i != skip && at + from * V + i < hi && x.before(last)) {  // never NaN
-          insert(e, x, lane);
-          last = Entry{uniform(e.value, top - 1), __builtin_amdgcn_readlane(e.id, top - 1)};
-        }
+    for (int i = 0; i < V; ++i) {
+      const int id = (int)(at + lane * V + i);
+      const bool in = (i != taken) & (at + lane * V + i < hi);
+      const Entry x{f[i], id};  // NaN comes before nothing
+      u64 found = __ballot(in & x.before(last));
+      while (found) {
+        const int from = __builtin_ctzll(found);
+        insert(e, Entry{uniform(f[i], from), __builtin_amdgcn_readlane(id, from)}, lane);
+        last = Entry{uniform(e.value, top - 1), __builtin_amdgcn_readlane(e.id, top - 1)};
+        found &= found - 1;
+        found &= __ballot(x.before(last));
       }
-      if (!equal) found &= __ballot(most > last.value);
     }
   }
 
@@ -208,13 +238,8 @@ struct Wave {
         e = Entry{taken < 0 ? -kInf : most, taken < 0 ? kNone : (int)(at + lane * V + taken)};
         sort(e, lane);
         last = Entry{uniform(e.value, top - 1), __builtin_amdgcn_readlane(e.id, top - 1)};
-        if (taken < 0) taken = V;  // nothing to leave out, but this is the first chunk
-        most = -kInf;
-#pragma unroll
-        for (int i = 0; i < V; ++i)
-          if (i != taken) most = __builtin_fmaxf(most, f[i]);
       }
-      candidates(f, most, at, taken);
+      candidates(f, at, taken);
     }
     s.rescale(highest, c);
     if (!top) last.value = s.m;
@@ -228,14 +253,24 @@ struct Wave {
     for (int i = 1; i < V; ++i) most = __builtin_fmaxf(most, f[i]);
     most = __builtin_fmaxf(most, -kInf);  // of NaN alone: nothing
     // top > 0 and entries missing: anything may still come in
-    if (__ballot(most > last.value) || (top && last.id == kNone)) slow(f, most, at);
+    if (__ballot(most > last.value) != 0 || (top && last.id == kNone)) slow(f, most, at);
     const float m = s.m == -kInf ? 0.0f : s.m;
+    float d[V];
+    if (near_zero(newt::bits_f32(__builtin_amdgcn_readfirstlane(newt::f32_bits(m))), c)) {
+      const float mc = m * c;
+#pragma unroll
+      for (int i = 0; i < V; ++i) d[i] = __builtin_fmaf(f[i], c, -mc);
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i) d[i] = (f[i] - m) * c;
+    }
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      const float d = (f[i] - m) * c;
-      const float x = __builtin_amdgcn_exp2f(d);  // NaN stays NaN
+      const float x = __builtin_amdgcn_exp2f(d[i]);  // NaN stays NaN
       s.S += x;
-      s.U += x * __builtin_fmaxf(d, -200.0f);  // 2^-inf * -inf counts as 0
+      // 2^-inf * -inf counts as 0; d is at most a rounding above 0 (med3: one
+      // instruction where fmaxf first quiets a NaN)
+      s.U += x * __builtin_amdgcn_fmed3f(d[i], -200.0f, 4.0f);
     }
   }
 };
@@ -244,7 +279,7 @@ template <typename T>
 __global__ void __launch_bounds__(64 * kWaves)
 logprobs_kernel(newt_logprobs_params p, int splits, int64_t per_split) {
   constexpr int STEP = Chunk<T>::STEP, V = Chunk<T>::V;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = wave_id();
   const int64_t row = blockIdx.x / splits;
   const int split = blockIdx.x % splits;
   const int64_t lo = split * per_split;
@@ -253,25 +288,32 @@ logprobs_kernel(newt_logprobs_params p, int splits, int64_t per_split) {
   const int top = p.top;
   const float c = kLog2e * p.inv_temperature;
 
-  // chunks of the waves lie side by side; two are on their way while two are
-  // worked on
-  constexpr int AHEAD = 2;
+  // chunks of the waves lie side by side; AHEAD of them are on their way while
+  // one is worked on, and none of those asks for bounds
+  constexpr int AHEAD = 4;
   Wave<T> w{top, lane, hi, c};
+  const int64_t step = kWaves * STEP, first = lo + wave * STEP;
+  const int whole = first + STEP <= hi ? (int)((hi - STEP - first) / step) + 1 : 0;
+  const T* from = x + first + lane * V;
   Chunk<T> next[AHEAD];
-  const int64_t step = kWaves * STEP;
-  int64_t at = lo + wave * STEP;
+  if (whole) {
+    // behind the last whole chunk that one is loaded again, to no use
 #pragma unroll
-  for (int i = 0; i < AHEAD; ++i) next[i].load(x, at + i * step + lane * V, hi);
-  for (; at < hi; at += AHEAD * step) {
-    Chunk<T> now[AHEAD];
+    for (int i = 0; i < AHEAD; ++i) next[i].load(from + (i < whole ? i : whole - 1) * step);
+    for (int j = 0; j < whole; j += AHEAD) {
 #pragma unroll
-    for (int i = 0; i < AHEAD; ++i) now[i] = next[i];
-#pragma unroll
-    for (int i = 0; i < AHEAD; ++i)
-      next[i].load(x, at + (AHEAD + i) * step + lane * V, hi);
-#pragma unroll
-    for (int i = 0; i < AHEAD; ++i)
-      if (at + i * step < hi) w.take(now[i], at + i * step);
+      for (int i = 0; i < AHEAD; ++i) {
+        const Chunk<T> now = next[i];
+        const int to = j + i + AHEAD;
+        next[i].load(from + (to < whole ? to : whole - 1) * step);
+        if (j + i < whole) w.take(now, first + (j + i) * step);
+      }
+    }
+  }
+  if (first + whole * step < hi) {
+    Chunk<T> end;
+    end.load(from + whole * step, hi - (first + whole * step) - lane * V);
+    w.take(end, first + whole * step);
   }
 
   Sums s = w.s;
@@ -302,34 +344,47 @@ logprobs_kernel(newt_logprobs_params p, int splits, int64_t per_split) {
   if (lane < top) to[lane] = e;
 }
 
-// One workgroup a row joins its splits: each wave some of their lists, then
-// the first wave those of all.
+// One workgroup a row joins its splits: four lists by each wave, then four of
+// theirs by each of the first waves, then the rest by the first.
 template <typename T>
-__global__ void __launch_bounds__(64 * kWaves)
-logprobs_join_kernel(newt_logprobs_params p, int splits) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+__global__ void __launch_bounds__(1024) logprobs_join_kernel(newt_logprobs_params p, int splits) {
+  constexpr int WAVES = kMostSplits / 4;
+  const int lane = threadIdx.x & 63, wave = wave_id();
   const int64_t row = blockIdx.x;
   const int top = p.top;
   const float c = kLog2e * p.inv_temperature;
+  const float* sums = (const float*)p.workspace + (row * splits + lane) * 4;
+  Sums s{-kInf, 0.0f, 0.0f};
+  if (wave == 0 && lane < splits) s = Sums{sums[0], sums[1], sums[2]};
   const Entry* from = (const Entry*)((const float*)p.workspace + p.rows * splits * 4) +
                       row * splits * top;
   const Entry none{-kInf, kNone};
   Entry e = none;
   if (top) {
-    __shared__ Entry entries[kWaves][64];
-    if (wave < splits && lane < top) e = from[wave * top + lane];
-    for (int i = wave + kWaves; i < splits; i += kWaves)
-      merge(e, 63 - lane < top ? from[i * top + 63 - lane] : none, lane);
-    entries[wave][lane] = e;
-    __syncthreads();
-    if (wave != 0) return;
-    for (int i = 1; i < kWaves; ++i) merge(e, entries[i][63 - lane], lane);
-  } else if (wave != 0) {
-    return;
+    __shared__ Entry entries[WAVES][64];
+    Entry list[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int at = i == 0 ? lane : 63 - lane, split = wave + i * WAVES;
+      list[i] = at < top && split < splits ? from[split * top + at] : none;
+    }
+    e = list[0];
+#pragma unroll
+    for (int i = 1; i < 4; ++i)
+      if (wave + i * WAVES < splits) merge(e, list[i], lane);
+    int lists = WAVES;  // of which the first min(lists, splits) hold anything
+#pragma unroll
+    for (; lists > 1; lists /= 4) {
+      if (wave < lists) entries[wave][lane] = e;
+      __syncthreads();
+      if (wave < lists / 4)
+#pragma unroll
+        for (int i = 1; i < 4; ++i)
+          if (wave + i * (lists / 4) < splits) merge(e, entries[wave + i * (lists / 4)][63 - lane], lane);
+      __syncthreads();
+    }
   }
-  const float* sums = (const float*)p.workspace + (row * splits + lane) * 4;
-  Sums s{-kInf, 0.0f, 0.0f};
-  if (lane < splits) s = Sums{sums[0], sums[1], sums[2]};
+  if (wave != 0) return;
   s.join(c);
   finish<T>(p, row, s, e, lane);
 }
@@ -359,7 +414,7 @@ int launch(const newt_logprobs_params& p, hipStream_t stream) {
   logprobs_kernel<T><<<dim3((unsigned)(p.rows * splits)), dim3(64 * kWaves), 0, stream>>>(p, splits,
                                                                                           per);
   if (splits > 1)
-    logprobs_join_kernel<T><<<dim3((unsigned)p.rows), dim3(64 * kWaves), 0, stream>>>(p, splits);
+    logprobs_join_kernel<T><<<dim3((unsigned)p.rows), dim3(1024), 0, stream>>>(p, splits);
   return launched("newt_token_logprobs");
 }
 
