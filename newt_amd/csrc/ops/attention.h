@@ -14,6 +14,8 @@ namespace newt_ops {
 constexpr float kLog2e = 1.44269504088896341f;
 constexpr float kInf = __builtin_inff();
 constexpr int kTile = 64;  // keys of a tile
+constexpr int kLimit = 1 << 30;       // of lengths, positions and windows
+constexpr int kNoWindow = 0x7fffffff; // sees all keys before it
 
 // A row's maximum may lag behind by this much (in powers of two) before sums
 // and accumulators are rescaled: 2^8 more in a weight costs no precision in
@@ -21,50 +23,58 @@ constexpr int kTile = 64;  // keys of a tile
 constexpr float kSlack = 8.0f;
 
 // The keys that the rows of a program see: sinks [0, sinks) and [lo, hi).
+// Positions, lengths and windows stay below 2^30, so sums of two fit an int.
 struct Range {
-  int64_t first, last;  // positions of the program's first and last query
-  int64_t lo, hi, sinks;
-  int64_t window;       // 0: none
-  int64_t sink_tiles, lo_tile, tiles;
+  int first, last;  // positions of the program's first and last query
+  int lo, hi, sinks;
+  int window;       // kNoWindow: none
+  int sink_tiles, lo_tile, tiles;
 
-  __device__ __forceinline__ Range(int64_t first_, int64_t last_, int64_t keys, int64_t window_,
-                                   int64_t sinks_)
+  __device__ __forceinline__ Range(int first_, int last_, int keys, int window_, int sinks_)
       : first(first_), last(last_), sinks(sinks_), window(window_) {
     hi = last + 1 < keys ? last + 1 : keys;
-    lo = window && first - window + 1 > 0 ? first - window + 1 : 0;
+    lo = first >= window ? first - window + 1 : 0;
     if (hi < 0) hi = 0;
     if (sinks > hi) sinks = hi;
     lo_tile = lo / kTile;
-    const int64_t hi_tile = (hi + kTile - 1) / kTile;
+    const int hi_tile = (hi + kTile - 1) / kTile;
     sink_tiles = (sinks + kTile - 1) / kTile;
     if (sink_tiles > lo_tile) sink_tiles = lo_tile;
     tiles = sink_tiles + (hi_tile > lo_tile ? hi_tile - lo_tile : 0);
   }
   // first key of the i-th tile
-  __device__ __forceinline__ int64_t tile(int64_t i) const {
+  __device__ __forceinline__ int tile(int i) const {
     return (i < sink_tiles ? i : i - sink_tiles + lo_tile) * kTile;
   }
   // whether every row sees every key of the tile from `key` on
-  __device__ __forceinline__ bool whole(int64_t key) const {
+  __device__ __forceinline__ bool whole(int key) const {
     return key + kTile <= hi && key + kTile - 1 <= first &&
-           (!window || key > last - window || key + kTile <= sinks);
+           ((u32)(last - key) < (u32)window || key + kTile <= sinks);
   }
-  __device__ __forceinline__ bool sees(int64_t position, int64_t key) const {
-    return key <= position && key < hi && (!window || position - key < window || key < sinks);
+  __device__ __forceinline__ bool sees(int position, int key) const {
+    // position - key in [0, window), by one unsigned comparison, or a sink
+    return (((u32)(position - key) < (u32)window) | ((key < sinks) & (key <= position))) & (key < hi);
   }
   // whether any row sees the key
-  __device__ __forceinline__ bool any(int64_t key) const {
-    return key < hi && (key >= lo || key < sinks);
+  __device__ __forceinline__ bool any(int key) const {
+    return (key < hi) & ((key >= lo) | (key < sinks));
   }
 };
 
 // Where rows of queries and outputs lie.
 struct Rows {
   int64_t stride_b, stride_h, stride_t;
-  __device__ __forceinline__ int64_t at(int64_t b, int64_t head, int64_t i) const {
+  __device__ __forceinline__ int64_t at(int b, int head, int i) const {
     return b * stride_b + head * stride_h + i * stride_t;
   }
 };
+
+// Workgroups go round the 8 dies of the chip, each with an L2 of its own; this
+// gives each die a run of neighbouring programs, which share keys and values.
+__device__ __forceinline__ int by_die(int i, int n) {
+  const int die = i & 7, each = n >> 3, more = n & 7;
+  return die * each + (die < more ? die : more) + (i >> 3);
+}
 
 // Partial results of `splits` programs for `rows` rows each: accumulators
 // [unit, split, row, D], then maxima and sums [unit, split, row] each.
@@ -91,15 +101,14 @@ constexpr int kMostSplits = 64;  // a lane of the joining wave for each
 template <typename T, int D>
 __global__ void __launch_bounds__(256)
 join_splits_kernel(const void* workspace, void* out, Rows o, int64_t units, int splits, int rows,
-                   int64_t row_tiles, int64_t q_len, int kv_heads, int group) {
+                   int row_tiles, int all_rows, int kv_heads, int group) {
   const Parts parts((void*)workspace, units, splits, rows, D);
   const int lane = threadIdx.x & 63;
   // rows that exist: row tiles are full but for a unit's last one
-  const int64_t all_rows = q_len * group;
-  const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (w >= units / row_tiles * all_rows) return;
-  const int64_t r = w % all_rows, sequence_head = w / all_rows;
-  const int64_t unit = sequence_head * row_tiles + r / rows;
+  const u32 w = blockIdx.x * 4 + wave_id();
+  if (w >= (u32)units / row_tiles * all_rows) return;
+  const u32 r = w % all_rows, sequence_head = w / all_rows;
+  const int64_t unit = (int64_t)sequence_head * row_tiles + r / rows;
   const int64_t at = unit * splits * rows + r % rows;  // and `rows` further a split
   constexpr int N = D / 64;
 
@@ -122,7 +131,7 @@ join_splits_kernel(const void* workspace, void* out, Rows o, int64_t units, int 
   T t[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) t[i] = (T)(total == 0.0f ? 0.0f : acc[i] / total);
-  const int64_t head = sequence_head % kv_heads, b = sequence_head / kv_heads;
+  const u32 head = sequence_head % kv_heads, b = sequence_head / kv_heads;
   T* to = (T*)out + o.at(b, head * group + r % group, r / group) + lane * N;
   newt::store_vec<T, N>(to, t, newt::any_align());
 }
@@ -144,12 +153,27 @@ inline int64_t most_tiles(int64_t keys, int64_t window, int64_t sinks, int64_t s
   return some < all ? some : all;
 }
 
+// The programs of a launch: `rows` of a KV head's query rows each, and a row's
+// tiles in `splits`. unit = (sequence * kv_heads + head) * row_tiles + row tile.
+struct Plan {
+  int row_tiles, rows, all_rows, splits;
+  int64_t units;
+  Plan(int64_t batch, int64_t q_len, int kv_heads, int group, int rows_)
+      : rows(rows_), splits(1) {
+    all_rows = (int)(q_len * group);
+    row_tiles = (all_rows + rows - 1) / rows;
+    units = batch * kv_heads * row_tiles;
+  }
+  // what no launch takes; q_len * heads below 2^31 is checked before
+  bool too_large() const { return units * splits > 0x7fffffff || units * rows > 0x7fffffff; }
+};
+
 template <typename T, int D>
-int join_splits(const void* workspace, void* out, Rows o, int64_t units, int splits, int rows,
-                int64_t row_tiles, int64_t q_len, int kv_heads, int group, hipStream_t stream) {
-  const int64_t waves = units / row_tiles * q_len * group;
+int join_splits(const void* workspace, void* out, Rows o, const Plan& r, int kv_heads, int group,
+                hipStream_t stream) {
+  const int64_t waves = r.units / r.row_tiles * r.all_rows;
   join_splits_kernel<T, D><<<dim3((unsigned)((waves + 3) / 4)), dim3(256), 0, stream>>>(
-      workspace, out, o, units, splits, rows, row_tiles, q_len, kv_heads, group);
+      workspace, out, o, r.units, r.splits, r.rows, r.row_tiles, r.all_rows, kv_heads, group);
   return launched("join_splits");
 }
 

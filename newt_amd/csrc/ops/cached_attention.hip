@@ -58,45 +58,46 @@ constexpr int kWaves = 4;
 
 template <typename T, int D, int MT>
 __global__ void __launch_bounds__(64 * kWaves)
-cached_attention_kernel(newt_cached_attention_params p, int splits, int64_t row_tiles) {
+cached_attention_kernel(newt_cached_attention_params p, int splits, int row_tiles) {
   typedef typename frag<T>::type TX;
   constexpr bool kExact = sizeof(T) == 2 && !__is_same(T, bf16);
   constexpr int ROWS = 16 * MT;
   constexpr int STEPS = D / 32;   // of the score product
   constexpr int DT = D / 16;      // tiles of head dims
   constexpr int KV4 = D / 64;     // 16-byte pieces of a key row a lane holds
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = wave_id();
   const int n = lane & 15, g = lane >> 4;
   const int split = blockIdx.x % splits;
-  const int64_t unit = blockIdx.x / splits;
-  const int64_t row_tile = unit % row_tiles;
+  const int unit = blockIdx.x / splits;
+  const int row_tile = unit % row_tiles;
   const int kv_heads = p.cache.kv_heads, group = p.heads / kv_heads;
-  const int head = (int)(unit / row_tiles % kv_heads);
-  const int64_t b = unit / row_tiles / kv_heads;
+  const int head = unit / row_tiles % kv_heads;
+  const int b = unit / row_tiles / kv_heads;
   const int size = p.cache.block_size, shift = __builtin_ctz(size);
-  const int64_t all_rows = p.q_len * group;
+  const int q_len = (int)p.q_len, all_rows = q_len * group;
 
-  const int64_t len = p.lens[b];
-  const int64_t r0 = row_tile * ROWS;
-  const int64_t r1 = r0 + ROWS < all_rows ? r0 + ROWS : all_rows;
-  const Range range(len - p.q_len + r0 / group, len - p.q_len + (r1 - 1) / group,
-                    len < p.table_width * size ? len : p.table_width * size, p.window, p.sinks);
+  const int len = p.lens[b] > 0 ? p.lens[b] : 0;
+  const int held = (int)(p.table_width * size);  // positions that the table has
+  const int r0 = row_tile * ROWS;
+  const int r1 = r0 + ROWS < all_rows ? r0 + ROWS : all_rows;
+  const Range range(len - q_len + r0 / group, len - q_len + (r1 - 1) / group,
+                    len < held ? len : held, p.window ? (int)p.window : kNoWindow, (int)p.sinks);
 
   // queries, and each lane's rows' positions
   TX q[MT][STEPS];
-  int64_t position[MT];
+  int position[MT];
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) {
-    const int64_t r = r0 + 16 * mt + n;
+    const int r = r0 + 16 * mt + n;
     const bool live = r < all_rows;
-    position[mt] = live ? len - p.q_len + r / group : -1;
+    position[mt] = live ? len - q_len + r / group : -1;
     const T* from = (const T*)p.q + (live ? Rows{p.q_stride_b, p.q_stride_h, p.q_stride_t}.at(
                                                 b, head * group + r % group, r / group) : 0) +
                     D / 4 * g;
 #pragma unroll
     for (int s = 0; s < STEPS; ++s) {
-      T t[8] = {};
-      if (live) newt::load_vec<T, 8>(from + 8 * s, t, newt::any_align());
+      T t[8];  // rows behind the last one take the first one's, and see nothing
+      newt::load_vec<T, 8>(from + 8 * s, t, newt::any_align());
       __builtin_memcpy(&q[mt][s], t, 16);
     }
   }
@@ -113,18 +114,18 @@ cached_attention_kernel(newt_cached_attention_params p, int splits, int64_t row_
   const float to_log2 = p.scale * kLog2e;
   const int32_t* table = p.table + b * p.table_stride;
 
-  const int64_t per = (range.tiles + splits - 1) / splits;
-  const int64_t end = (split + 1) * per < range.tiles ? (split + 1) * per : range.tiles;
-  for (int64_t i = split * per + wave; i < end; i += kWaves) {
-    const int64_t key = range.tile(i);
+  const int per = (range.tiles + splits - 1) / splits;
+  const int end = (split + 1) * per < range.tiles ? (split + 1) * per : range.tiles;
+  for (int i = split * per + wave; i < end; i += kWaves) {
+    const int key = range.tile(i);
     const bool whole = range.whole(key);
     // the blocks of this lane's keys (tokens 16 (n / 4) on) and values (16 g on)
     int64_t page[2];
     bool in[2];
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      const int64_t token = key + 16 * (j ? g : n >> 2);
-      const int64_t slot = token >> shift;
+      const int token = key + 16 * (j ? g : n >> 2);
+      const int slot = token >> shift;
       in[j] = token < range.hi;
       int32_t block = in[j] ? table[slot] : 0;
       if (block < 0 || block >= p.cache.blocks) {
@@ -275,7 +276,7 @@ cached_attention_kernel(newt_cached_attention_params p, int splits, int64_t row_
     __syncthreads();
     // 16 threads a row, each D / 16 of its dims in runs of 4
     const int row = threadIdx.x >> 4, part = threadIdx.x & 15;
-    const int64_t r = r0 + 16 * mt + row;
+    const int r = r0 + 16 * mt + row;
     if (r < all_rows) {
       float most = sm[0][row];
 #pragma unroll
@@ -285,7 +286,7 @@ cached_attention_kernel(newt_cached_attention_params p, int splits, int64_t row_
       for (int w = 0; w < kWaves; ++w)
         total += sm[w][row] == -kInf ? sl[w][row]
                                      : sl[w][row] * __builtin_amdgcn_exp2f(sm[w][row] - most);
-      const int64_t at = (unit * splits + split) * ROWS + 16 * mt + row;
+      const int64_t at = ((int64_t)unit * splits + split) * ROWS + 16 * mt + row;
       if (splits > 1 && part == 0) {
         parts.m[at] = most;
         parts.l[at] = total;
@@ -311,19 +312,11 @@ cached_attention_kernel(newt_cached_attention_params p, int splits, int64_t row_
   }
 }
 
-struct Plan {
-  int64_t row_tiles, units;
-  int splits, rows;
-};
-
 // Rows of a program and splits of its tiles, from sizes that the host knows:
 // the table's width bounds the lengths.
 Plan plan(const newt_cached_attention_params& p) {
-  Plan r;
-  const int64_t rows = p.q_len * (p.heads / p.cache.kv_heads);
-  r.rows = rows > 16 ? 32 : 16;
-  r.row_tiles = (rows + r.rows - 1) / r.rows;
-  r.units = p.batch * p.cache.kv_heads * r.row_tiles;
+  const int group = p.heads / p.cache.kv_heads;
+  Plan r(p.batch, p.q_len, p.cache.kv_heads, group, p.q_len * group > 16 ? 32 : 16);
   const int64_t tiles = most_tiles(p.table_width * p.cache.block_size, p.window, p.sinks, p.q_len);
   r.splits = split_count(r.units, tiles, 1024, kWaves);
   return r;
@@ -334,17 +327,15 @@ int launch(const newt_cached_attention_params& p, hipStream_t stream) {
   const Plan r = plan(p);
   if (r.splits > 1 && !p.workspace)
     return fail(NEWT_ERR_INVALID, "newt_cached_attention: null workspace");
-  if (r.units * r.splits > 0x7fffffff)
-    return fail(NEWT_ERR_INVALID, "newt_cached_attention: too many queries");
+  if (r.too_large()) return fail(NEWT_ERR_INVALID, "newt_cached_attention: too many queries");
   const dim3 grid((unsigned)(r.units * r.splits)), block(64 * kWaves);
   if (r.rows == 16)
     cached_attention_kernel<T, D, 1><<<grid, block, 0, stream>>>(p, r.splits, r.row_tiles);
   else
     cached_attention_kernel<T, D, 2><<<grid, block, 0, stream>>>(p, r.splits, r.row_tiles);
   if (r.splits > 1)
-    return join_splits<T, D>(p.workspace, p.out, {p.o_stride_b, p.o_stride_h, p.o_stride_t},
-                             r.units, r.splits, r.rows, r.row_tiles, p.q_len, p.cache.kv_heads,
-                             p.heads / p.cache.kv_heads, stream);
+    return join_splits<T, D>(p.workspace, p.out, {p.o_stride_b, p.o_stride_h, p.o_stride_t}, r,
+                             p.cache.kv_heads, p.heads / p.cache.kv_heads, stream);
   return launched("newt_cached_attention");
 }
 
@@ -362,6 +353,9 @@ const char* wrong(const newt_cached_attention_params& p) {
   if (p.batch < 0 || p.q_len < 0 || p.table_width < 0 || p.window < 0 || p.sinks < 0)
     return "negative size";
   if (p.heads <= 0 || p.heads % p.cache.kv_heads) return "heads have to be a multiple of kv_heads";
+  if (p.q_len * p.heads >= kLimit || p.table_width * p.cache.block_size >= kLimit ||
+      p.window >= kLimit || p.sinks >= kLimit)
+    return "sizes stay below 2^30";
   return nullptr;
 }
 

@@ -20,117 +20,165 @@ template <typename T> struct frag;
 template <> struct frag<bf16> { typedef bf16x8 type; };
 template <> struct frag<f16> { typedef f16x8 type; };
 
-template <typename T, int D, int WAVES>
+// Whole 16-byte pieces of rows go from memory to LDS by themselves (DIRECT)
+// where rows and tensors are aligned to them; else through registers.
+template <typename T, int D, int WAVES, bool DIRECT>
 struct Program {
   typedef typename frag<T>::type TX;
   static constexpr int THREADS = 64 * WAVES;
   static constexpr int ROWS = 32 * WAVES;
   static constexpr int STEPS = D / 16;
   static constexpr int DT = D / 32;
+  static constexpr int STAGE = 2 * kTile * D;  // numbers of a stage: keys, then values
   typedef newt::LdsTile<T, D> KTile;
   typedef newt::LdsTileR<T, D> VTile;
 
   const newt_window_attention_params& p;
-  T* k_lds;
-  T* v_lds;
+  T* even;  // two stages of LDS, two arrays: the compiler then knows that what
+  T* odd;   // is on its way into one is not what is read from the other
   const T* k;
   const T* v;
   const Range& range;
+  const int wave;
   TX q[STEPS];
-  int64_t position;
+  int position;
   float m, l;
   f32x16 acc[DT];
 
-  // the tile's keys and values from global memory, rows behind the last
-  // visible key as zeros
-  __device__ __forceinline__ void stage(int64_t key) {
-    constexpr int CHUNKS = kTile * D / 8;
+  // A tile's keys and values into stage `to`, rows behind the last visible key
+  // as zeros.
+  __device__ __forceinline__ void stage(int key, T* k_lds) const {
+    constexpr int ROUNDS = kTile * D / 8 / THREADS;
+    const int rows = range.hi - key;
+    const int lane = threadIdx.x & 63;
+    T* v_lds = k_lds + kTile * D;
+    const T* k_from = k + key * p.k_stride_t;
+    const T* v_from = v + key * p.v_stride_t;
 #pragma unroll
-    for (int c = threadIdx.x; c < CHUNKS; c += THREADS) {
-      const int row = c / (D / 8), d = c % (D / 8) * 8;
-      T a[8] = {}, b[8] = {};
-      if (key + row < range.hi) {
-        newt::load_vec<T, 8>(k + (key + row) * p.k_stride_t + d, a, newt::any_align());
-        newt::load_vec<T, 8>(v + (key + row) * p.v_stride_t + d, b, newt::any_align());
+    for (int c = 0; c < ROUNDS; ++c) {
+      // the 16 bytes of LDS at `slot` hold this row and column
+      const int first = c * THREADS + 64 * wave, slot = first + lane;
+      int row, d;
+      newt::lds_tile_slot<T, D>(slot, row, d);
+      if constexpr (DIRECT) {
+        newt::lds_dma16_masked(k_from, (u32)(row * (int)p.k_stride_t + d) * sizeof(T), row < rows,
+                               k_lds + first * 8);
+      } else {
+        T x[8] = {};
+        if (row < rows)
+          newt::load_vec<T, 8>(k_from + row * p.k_stride_t + d, x, newt::any_align());
+        newt::store_vec<T, 8>(k_lds + slot * 8, x);
       }
-      newt::store_vec<T, 8>(k_lds + KTile::off(row, d), a);
-      newt::store_vec<T, 8>(v_lds + VTile::off(row, d), b);
+    }
+#pragma unroll
+    for (int c = 0; c < ROUNDS; ++c) {
+      const int first = c * THREADS + 64 * wave, slot = first + lane;
+      int row, d;
+      VTile::slot(slot, row, d);
+      if constexpr (DIRECT) {
+        newt::lds_dma16_masked(v_from, (u32)(row * (int)p.v_stride_t + d) * sizeof(T), row < rows,
+                               v_lds + first * 8);
+      } else {
+        T x[8] = {};
+        if (row < rows)
+          newt::load_vec<T, 8>(v_from + row * p.v_stride_t + d, x, newt::any_align());
+        newt::store_vec<T, 8>(v_lds + slot * 8, x);
+      }
     }
   }
 
+  // `to_log2` > 0: the rows' maxima are those of the unscaled scores.
   template <bool CAREFUL>
-  __device__ __forceinline__ void attend(int64_t from, int64_t to) {
-    const int lane = threadIdx.x & 63, half = lane >> 5;
-    const float to_log2 = p.scale * kLog2e;
+  __device__ __forceinline__ void attend(int from, int to, float to_log2) {
     m = -kInf;
     l = 0.0f;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) acc[dt] = (f32x16)(0.0f);
-    for (int64_t i = from; i < to; ++i) {
-      const int64_t key = range.tile(i);
-      __syncthreads();
-      stage(key);
-      __syncthreads();
-      f32x16 s[2];
-#pragma unroll
-      for (int kh = 0; kh < 2; ++kh) {
-        s[kh] = (f32x16)(0.0f);
-#pragma unroll
-        for (int st = 0; st < STEPS; ++st)
-          s[kh] = newt::mfma_32x32x16(
-              __builtin_bit_cast(TX, newt::lds_frag_k<T, D, 32>(k_lds, 32 * kh, 16 * st, lane)),
-              q[st], s[kh]);
+    if constexpr (CAREFUL) {
+      for (int i = from; i < to; ++i) {
+        __syncthreads();
+        stage(range.tile(i), even);
+        __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
+        __syncthreads();
+        tile<true>(range.tile(i), even, to_log2);
       }
-      const bool masked = !range.whole(key);
-      // bit 16 kh + e: whether the row sees the key of s[kh][e]
-      u32 seen = ~0u;
-      float most = -kInf;
-#pragma unroll
-      for (int kh = 0; kh < 2; ++kh)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) s[kh][e] *= to_log2;
-      if (masked || CAREFUL) {
-#pragma unroll
-        for (int kh = 0; kh < 2; ++kh)
-#pragma unroll
-          for (int e = 0; e < 16; ++e)
-            if (!range.sees(position, key + 32 * kh + 8 * (e / 4) + 4 * half + e % 4)) {
-              s[kh][e] = -kInf;
-              seen &= ~(1u << (16 * kh + e));
-            }
+    } else {
+      if (from < to) stage(range.tile(from), even);
+      for (int i = from; i < to; i += 2) {
+        step(i, to, even, odd, to_log2);
+        if (i + 1 < to) step(i + 1, to, odd, even, to_log2);
       }
+    }
+  }
+
+  // One tile, while the next one is on its way.
+  __device__ __forceinline__ void step(int i, int to, T* now, T* next, float to_log2) {
+    // this tile's pieces have arrived, and no wave still reads the other stage
+    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
+    __syncthreads();
+    if (i + 1 < to) stage(range.tile(i + 1), next);
+    tile<false>(range.tile(i), now, to_log2);
+  }
+
+  template <bool CAREFUL>
+  __device__ __forceinline__ void tile(int key, const T* k_lds, float to_log2) {
+    const int lane = threadIdx.x & 63, half = lane >> 5;
+    const T* v_lds = k_lds + kTile * D;
+    f32x16 s[2];
 #pragma unroll
-      for (int kh = 0; kh < 2; ++kh)
+    for (int kh = 0; kh < 2; ++kh) {
+      s[kh] = (f32x16)(0.0f);
 #pragma unroll
-        for (int e = 0; e < 16; ++e) most = __builtin_fmaxf(most, s[kh][e]);
-      most = newt::lane_reduce<newt::Max, 32>(most);
-      if (__ballot(most > m + kSlack)) {
-        const float to_m = __builtin_fmaxf(m, most);
-        const float f = m == -kInf ? 0.0f : __builtin_amdgcn_exp2f(m - to_m);
-        l *= f;
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt) acc[dt] *= f;
-        m = to_m;
-      }
-      const float ref = m == -kInf ? 0.0f : m;
-      TX w[4];
+      for (int st = 0; st < STEPS; ++st)
+        s[kh] = newt::mfma_32x32x16(
+            __builtin_bit_cast(TX, newt::lds_frag_k<T, D, 32>(k_lds, 32 * kh, 16 * st, lane)),
+            q[st], s[kh]);
+    }
+    // bit 16 kh + e: whether the row sees the key of s[kh][e]
+    u32 seen = ~0u;
+    if (CAREFUL || !range.whole(key)) {
 #pragma unroll
       for (int kh = 0; kh < 2; ++kh)
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          const float x = __builtin_amdgcn_exp2f(s[kh][e] - ref);
-          l += x;
-          w[2 * kh + e / 8][e % 8] = (T)x;
-        }
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-        for (int ks = 0; ks < 4; ++ks) {
-          i16x8 a = newt::lds_frag_r_perm32<T, D>(v_lds, 32 * dt, 16 * ks, lane);
-          if constexpr (CAREFUL) a = keep_apart(a, seen >> (8 * ks), acc[dt]);
-          acc[dt] = newt::mfma_32x32x16(__builtin_bit_cast(TX, a), w[ks], acc[dt]);
+          const bool sees = range.sees(position, key + 32 * kh + 8 * (e / 4) + 4 * half + e % 4);
+          s[kh][e] = sees ? s[kh][e] : -kInf;
+          if constexpr (CAREFUL)
+            if (!sees) seen &= ~(1u << (16 * kh + e));
         }
     }
+    float most = s[0][0];
+#pragma unroll
+    for (int kh = 0; kh < 2; ++kh)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) most = __builtin_fmaxf(most, s[kh][e]);
+    most = newt::lane_reduce<newt::Max, 32>(most) * to_log2;
+    if (__ballot(most > m + kSlack)) {
+      const float to_m = __builtin_fmaxf(m, most);
+      const float f = m == -kInf ? 0.0f : __builtin_amdgcn_exp2f(m - to_m);
+      l *= f;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) acc[dt] *= f;
+      m = to_m;
+    }
+    const float ref = m == -kInf ? 0.0f : m;
+    TX w[4];
+#pragma unroll
+    for (int kh = 0; kh < 2; ++kh)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kh][e], to_log2, -ref));
+        l += x;
+        w[2 * kh + e / 8][e % 8] = (T)x;
+      }
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks) {
+        i16x8 a = newt::lds_frag_r_perm32<T, D>(v_lds, 32 * dt, 16 * ks, lane);
+        if constexpr (CAREFUL) a = keep_apart(a, seen >> (8 * ks), acc[dt]);
+        acc[dt] = newt::mfma_32x32x16(__builtin_bit_cast(TX, a), w[ks], acc[dt]);
+      }
   }
 
   // The operand without its infinities and NaN, which go into the
@@ -164,55 +212,67 @@ struct Program {
   }
 };
 
-template <typename T, int D, int WAVES>
-__global__ void __launch_bounds__(64 * WAVES)
-window_attention_kernel(newt_window_attention_params p, int splits, int64_t row_tiles) {
-  typedef Program<T, D, WAVES> P;
-  __shared__ __attribute__((aligned(16))) T k_lds[kTile * D];
-  __shared__ __attribute__((aligned(16))) T v_lds[kTile * D];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
-  const int split = blockIdx.x % splits;
-  const int64_t unit = blockIdx.x / splits;
-  const int64_t row_tile = unit % row_tiles;
+template <typename T, int D, int WAVES, bool DIRECT>
+__global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2)
+window_attention_kernel(newt_window_attention_params p, int splits, int row_tiles) {
+  typedef Program<T, D, WAVES, DIRECT> P;
+  __shared__ __attribute__((aligned(16))) T even[P::STAGE];
+  __shared__ __attribute__((aligned(16))) T odd[P::STAGE];
+  const int lane = threadIdx.x & 63, wave = wave_id(), half = lane >> 5;
+  const int program = by_die(blockIdx.x, gridDim.x);
+  const int split = program % splits;
+  const int unit = program / splits;
+  const int row_tile = unit % row_tiles;
   const int group = p.heads / p.kv_heads;
-  const int head = (int)(unit / row_tiles % p.kv_heads);
-  const int64_t b = unit / row_tiles / p.kv_heads;
-  const int64_t all_rows = p.q_len * group;
-  const int64_t start = p.q_start ? p.q_start[b] : p.kv_len - p.q_len;
-  const int64_t r0 = row_tile * P::ROWS;
-  const int64_t r1 = r0 + P::ROWS < all_rows ? r0 + P::ROWS : all_rows;
-  const Range range(start + r0 / group, start + (r1 - 1) / group, p.kv_len, p.window, p.sinks);
+  const int head = unit / row_tiles % p.kv_heads;
+  const int b = unit / row_tiles / p.kv_heads;
+  const int q_len = (int)p.q_len, all_rows = q_len * group;
+  int start = (int)(p.kv_len - p.q_len);
+  if (p.q_start) {
+    start = p.q_start[b];
+    start = start < -kLimit ? -kLimit : start > kLimit ? kLimit : start;
+  }
+  const int r0 = row_tile * P::ROWS;
+  const int r1 = r0 + P::ROWS < all_rows ? r0 + P::ROWS : all_rows;
+  const Range range(start + r0 / group, start + (r1 - 1) / group, (int)p.kv_len,
+                    p.window ? (int)p.window : kNoWindow, (int)p.sinks);
 
-  P t{p, k_lds, v_lds, (const T*)p.k + b * p.k_stride_b + head * p.k_stride_h,
-      (const T*)p.v + b * p.v_stride_b + head * p.v_stride_h, range};
-  const int64_t r = r0 + 32 * wave + (lane & 31);
+  P t{p, even, odd, (const T*)p.k + b * p.k_stride_b + head * p.k_stride_h,
+      (const T*)p.v + b * p.v_stride_b + head * p.v_stride_h, range, wave};
+  const int r = r0 + 32 * wave + (lane & 31);
   const bool live = r < all_rows;
   t.position = live ? start + r / group : -1;
   const T* q = (const T*)p.q + (live ? Rows{p.q_stride_b, p.q_stride_h, p.q_stride_t}.at(
                                            b, head * group + r % group, r / group) : 0);
+  // a negative scale is taken out of the queries, and one of 0 would make NaN
+  // of masked scores: any tiny one gives equal weights
+  const bool negative = p.scale < 0.0f;
 #pragma unroll
   for (int s = 0; s < P::STEPS; ++s) {
-    T x[8] = {};
-    if (live) newt::load_vec<T, 8>(q + 16 * s + 8 * half, x, newt::any_align());
-    __builtin_memcpy(&t.q[s], x, 16);
+    T x[8];  // rows behind the last one take the first one's, and see nothing
+    newt::load_vec<T, 8>(q + 16 * s + 8 * half, x, newt::any_align());
+#pragma unroll
+    for (int i = 0; i < 8; ++i) t.q[s][i] = negative ? -x[i] : x[i];
   }
+  const float to_log2 =
+      __builtin_fmaxf(__builtin_fabsf(p.scale) * kLog2e, 1e-37f);
 
-  const int64_t per = (range.tiles + splits - 1) / splits;
-  const int64_t from = split * per;
-  const int64_t to = from + per < range.tiles ? from + per : range.tiles;
-  t.template attend<false>(from, to);
+  const int per = (range.tiles + splits - 1) / splits;
+  const int from = split * per;
+  const int to = from + per < range.tiles ? from + per : range.tiles;
+  t.template attend<false>(from, to, to_log2);
   float check = 0.0f;  // NaN where an accumulator is not finite
 #pragma unroll
   for (int dt = 0; dt < P::DT; ++dt)
 #pragma unroll
     for (int e = 0; e < 16; ++e) check += t.acc[dt][e] * 0.0f;
-  if (__syncthreads_or(!(check == 0.0f))) t.template attend<true>(from, to);
+  if (__syncthreads_or(!(check == 0.0f))) t.template attend<true>(from, to, to_log2);
 
   const float l = newt::lane_reduce<newt::Sum, 32>(t.l);
   if (!live) return;
   if (splits > 1) {
     const Parts parts(p.workspace, (int64_t)(gridDim.x / splits), splits, P::ROWS, D);
-    const int64_t at = (unit * splits + split) * P::ROWS + 32 * wave + (lane & 31);
+    const int64_t at = ((int64_t)unit * splits + split) * P::ROWS + 32 * wave + (lane & 31);
     if (half == 0) {
       parts.m[at] = t.m;
       parts.l[at] = l;
@@ -238,19 +298,20 @@ window_attention_kernel(newt_window_attention_params p, int splits, int64_t row_
     }
 }
 
-struct Plan {
-  int64_t row_tiles, units;
-  int splits, rows;
-};
-
 Plan plan(const newt_window_attention_params& p) {
-  Plan r;
-  const int64_t rows = p.q_len * (p.heads / p.kv_heads);
-  r.rows = 128;
-  r.row_tiles = (rows + r.rows - 1) / r.rows;
-  r.units = p.batch * p.kv_heads * r.row_tiles;
-  r.splits = 1;
+  Plan r(p.batch, p.q_len, p.kv_heads, p.heads / p.kv_heads, 128);
+  const int64_t tiles = most_tiles(p.kv_len, p.window, p.sinks, p.q_len);
+  r.splits = split_count(r.units, tiles, 512, 4);
   return r;
+}
+
+// Whether every piece of 8 numbers that a tile is staged in is aligned.
+bool direct(const newt_window_attention_params& p) {
+  const int64_t strides = p.k_stride_b | p.k_stride_h | p.k_stride_t | p.v_stride_b |
+                          p.v_stride_h | p.v_stride_t;
+  return strides % 8 == 0 && (((uintptr_t)p.k | (uintptr_t)p.v) & 15) == 0 &&
+         // and lies within 2^31 bytes of its tile's first
+         p.k_stride_t < (1 << 22) && p.v_stride_t < (1 << 22);
 }
 
 template <typename T, int D>
@@ -258,14 +319,15 @@ int launch(const newt_window_attention_params& p, hipStream_t stream) {
   const Plan r = plan(p);
   if (r.splits > 1 && !p.workspace)
     return fail(NEWT_ERR_INVALID, "newt_window_attention: null workspace");
-  if (r.units * r.splits > 0x7fffffff)
-    return fail(NEWT_ERR_INVALID, "newt_window_attention: too many queries");
-  window_attention_kernel<T, D, 4><<<dim3((unsigned)(r.units * r.splits)), dim3(256), 0, stream>>>(
-      p, r.splits, r.row_tiles);
+  if (r.too_large()) return fail(NEWT_ERR_INVALID, "newt_window_attention: too many queries");
+  const dim3 grid((unsigned)(r.units * r.splits)), block(256);
+  if (direct(p))
+    window_attention_kernel<T, D, 4, true><<<grid, block, 0, stream>>>(p, r.splits, r.row_tiles);
+  else
+    window_attention_kernel<T, D, 4, false><<<grid, block, 0, stream>>>(p, r.splits, r.row_tiles);
   if (r.splits > 1)
-    return join_splits<T, D>(p.workspace, p.out, {p.o_stride_b, p.o_stride_h, p.o_stride_t},
-                             r.units, r.splits, r.rows, r.row_tiles, p.q_len, p.kv_heads,
-                             p.heads / p.kv_heads, stream);
+    return join_splits<T, D>(p.workspace, p.out, {p.o_stride_b, p.o_stride_h, p.o_stride_t}, r,
+                             p.kv_heads, p.heads / p.kv_heads, stream);
   return launched("newt_window_attention");
 }
 
@@ -285,6 +347,9 @@ const char* wrong(const newt_window_attention_params& p) {
     return "head_dim is 64, 128 or 256";
   if (p.heads <= 0 || p.kv_heads <= 0 || p.heads % p.kv_heads)
     return "heads have to be a multiple of kv_heads";
+  if (p.q_len * p.heads >= kLimit || p.kv_len >= kLimit || p.window >= kLimit || p.sinks >= kLimit)
+    return "sizes stay below 2^30";
+  if (p.k_stride_t < 0 || p.v_stride_t < 0) return "negative stride";
   return nullptr;
 }
 

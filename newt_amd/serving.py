@@ -100,7 +100,7 @@ def _shape(what, name, t, shape, dtype=None):
 def _whole(what, name, value, least):
     if isinstance(value, bool) or not isinstance(value, int):
         raise TypeError(f"{what}: {name} must be an int")
-    if not least <= value < 2 ** 31:
+    if not least <= value < 2 ** 30:
         raise ValueError(f"{what}: {name}={value} is out of range")
 
 
@@ -278,7 +278,7 @@ def _pages(what, device, cache, block_table, batch):
     width = block_table.shape[1]
     if width > 1 and block_table.stride(1) != 1:
         raise ValueError(f"{what}: rows of block_table need unit stride")
-    if width * size >= 2 ** 31:
+    if width * size >= 2 ** 30:
         raise ValueError(f"{what}: sequences of {width} blocks are too long")
     fields = (kp, vp, ks.data_ptr(), vs.data_ptr(), blocks, heads, size, dim, 0)
     return fields, heads, size, dim, width, block_table.stride(0)
@@ -368,6 +368,8 @@ def cached_attention(q, cache, block_table, lens, window=None, sinks=0, scale=No
                                                            block_table, B)
     if D != dim or H == 0 or H % heads:
         raise ValueError(f"cached_attention: {H} heads of {D} dims over a cache of {heads} of {dim}")
+    if S * H >= 2 ** 30:
+        raise ValueError("cached_attention: too many queries")
     _per_sequence("cached_attention", "lens", lens, B)
     if fields[4] == 0 and width:
         raise ValueError("cached_attention: the cache has no blocks")
@@ -414,7 +416,7 @@ def window_attention(q, k, v, window=None, sinks=0, scale=None, q_start=None, ou
     _shape("window_attention", "v", v, (B, heads, Sk, D), q.dtype)
     if heads == 0 or H == 0 or H % heads:
         raise ValueError(f"window_attention: {H} query heads over {heads}")
-    if Sk >= 2 ** 31 or S >= 2 ** 31:
+    if Sk >= 2 ** 30 or S * H >= 2 ** 30:
         raise ValueError("window_attention: sequences are too long")
     if q_start is not None:
         _per_sequence("window_attention", "q_start", q_start, B)
