@@ -110,7 +110,6 @@ join_splits_kernel(const void* workspace, void* out, Rows o, int64_t units, int 
   const u32 r = w % all_rows, sequence_head = w / all_rows;
   const int64_t unit = (int64_t)sequence_head * row_tiles + r / rows;
   const int64_t at = unit * splits * rows + r % rows;  // and `rows` further a split
-  constexpr int N = D / 64;
 
   const float m = lane < splits ? parts.m[at + (int64_t)lane * rows] : -kInf;
   const float l = lane < splits ? parts.l[at + (int64_t)lane * rows] : 0.0f;
@@ -118,22 +117,37 @@ join_splits_kernel(const void* workspace, void* out, Rows o, int64_t units, int 
   // without a maximum a split has seen nothing, or NaN
   const float f = m == -kInf ? 0.0f : __builtin_amdgcn_exp2f(m - M);
   const float total = newt::lane_reduce<newt::Sum, 63>(m == -kInf ? l : l * f);
-  float acc[N] = {};
-  const float* from = parts.acc + at * D + lane * N;
-#pragma unroll 8
-  for (int s = 0; s < splits; ++s) {
-    const float g = newt::bits_f32(__builtin_amdgcn_readlane(newt::f32_bits(f), s));
-    float a[N];
-    newt::load_vec<float, N>(from + (int64_t)s * rows * D, a);
+  // 16 bytes a lane: the wave reads SIDE splits at a time, AT_ONCE such pieces
+  // without waiting in between
+  constexpr int WIDE = D / 4, SIDE = 64 / WIDE, AT_ONCE = 8;
+  const int side = lane / WIDE, d = lane % WIDE * 4;
+  f32x4 acc = (f32x4)(0.0f);
+  const float* from = parts.acc + at * D + d;
+  for (int s = 0; s < splits; s += SIDE * AT_ONCE) {
+    f32x4 a[AT_ONCE];
+    float g[AT_ONCE];
 #pragma unroll
-    for (int i = 0; i < N; ++i) acc[i] += a[i] * g;
+    for (int j = 0; j < AT_ONCE; ++j) {
+      const int split = s + j * SIDE + side;
+      a[j] = *(const f32x4*)(from + (int64_t)(split < splits ? split : 0) * rows * D);
+      g[j] = __shfl(f, split);
+    }
+#pragma unroll
+    for (int j = 0; j < AT_ONCE; ++j)
+      acc += s + j * SIDE + side < splits ? a[j] * g[j] : (f32x4)(0.0f);
   }
-  T t[N];
 #pragma unroll
-  for (int i = 0; i < N; ++i) t[i] = (T)(total == 0.0f ? 0.0f : acc[i] / total);
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (SIDE > 2) acc[i] = newt::lane_reduce<newt::Sum, 16>(acc[i]);
+    if constexpr (SIDE > 1) acc[i] = newt::lane_reduce<newt::Sum, 32>(acc[i]);
+  }
+  if (side) return;
+  T t[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) t[i] = (T)(total == 0.0f ? 0.0f : acc[i] / total);
   const u32 head = sequence_head % kv_heads, b = sequence_head / kv_heads;
-  T* to = (T*)out + o.at(b, head * group + r % group, r / group) + lane * N;
-  newt::store_vec<T, N>(to, t, newt::any_align());
+  T* to = (T*)out + o.at(b, head * group + r % group, r / group) + d;
+  newt::store_vec<T, 4>(to, t, newt::any_align());
 }
 
 // Splits of a program's tiles: `want` programs in all where `units` alone are

@@ -137,15 +137,27 @@ struct Program {
     // bit 16 kh + e: whether the row sees the key of s[kh][e]
     u32 seen = ~0u;
     if (CAREFUL || !range.whole(key)) {
+      const int at = key + 4 * half;
+      const auto offset = [](int kh, int e) { return 32 * kh + 8 * (e / 4) + e % 4; };
+      if (!CAREFUL && key >= range.sinks && range.hi > range.last) {
+        // no sinks here, and the keys go on to the last query: the window alone
+        const int back = position - at;
 #pragma unroll
-      for (int kh = 0; kh < 2; ++kh)
+        for (int kh = 0; kh < 2; ++kh)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const bool sees = range.sees(position, key + 32 * kh + 8 * (e / 4) + 4 * half + e % 4);
-          s[kh][e] = sees ? s[kh][e] : -kInf;
-          if constexpr (CAREFUL)
-            if (!sees) seen &= ~(1u << (16 * kh + e));
-        }
+          for (int e = 0; e < 16; ++e)
+            s[kh][e] = (u32)(back - offset(kh, e)) < (u32)range.window ? s[kh][e] : -kInf;
+      } else {
+#pragma unroll
+        for (int kh = 0; kh < 2; ++kh)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const bool sees = range.sees(position, at + offset(kh, e));
+            s[kh][e] = sees ? s[kh][e] : -kInf;
+            if constexpr (CAREFUL)
+              if (!sees) seen &= ~(1u << (16 * kh + e));
+          }
+      }
     }
     float most = s[0][0];
 #pragma unroll
