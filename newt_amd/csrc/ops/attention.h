@@ -150,15 +150,6 @@ join_splits_kernel(const void* workspace, void* out, Rows o, int64_t units, int 
   newt::store_vec<T, 4>(to, t, newt::any_align());
 }
 
-// Splits of a program's tiles: `want` programs in all where `units` alone are
-// fewer, each split with at least `least` of the at most `tiles` tiles.
-inline int split_count(int64_t units, int64_t tiles, int64_t want, int64_t least) {
-  int64_t n = (want + units - 1) / units;
-  const int64_t most = (tiles + least - 1) / least;
-  n = n < most ? n : most;
-  return (int)(n < 1 ? 1 : n < kMostSplits ? n : kMostSplits);
-}
-
 // At most so many tiles can a program of `span` queries visit.
 inline int64_t most_tiles(int64_t keys, int64_t window, int64_t sinks, int64_t span) {
   const int64_t all = (keys + kTile - 1) / kTile;

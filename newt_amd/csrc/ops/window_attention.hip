@@ -49,6 +49,10 @@ struct Program {
   // as zeros.
   __device__ __forceinline__ void stage(int key, T* k_lds) const {
     constexpr int ROUNDS = kTile * D / 8 / THREADS;
+    constexpr int STEP = THREADS / (D / 8);  // rows of a round
+    // the swizzles go by 16 rows: rounds that are a multiple of that apart have
+    // the same lane offsets, and differ by a scalar
+    constexpr int KINDS = STEP < 16 ? 16 / STEP : 1;
     const int rows = range.hi - key;
     const int lane = threadIdx.x & 63;
     T* v_lds = k_lds + kTile * D;
@@ -57,33 +61,26 @@ struct Program {
 #pragma unroll
     for (int c = 0; c < ROUNDS; ++c) {
       // the 16 bytes of LDS at `slot` hold this row and column
-      const int first = c * THREADS + 64 * wave, slot = first + lane;
+      const int kind = c % KINDS, up = (c - kind) * STEP;
+      const int first = c * THREADS + 64 * wave, slot = kind * THREADS + 64 * wave + lane;
       int row, d;
       newt::lds_tile_slot<T, D>(slot, row, d);
-      if constexpr (DIRECT) {
-        newt::lds_dma16_masked(k_from, (u32)(row * (int)p.k_stride_t + d) * sizeof(T), row < rows,
-                               k_lds + first * 8);
-      } else {
-        T x[8] = {};
-        if (row < rows)
-          newt::load_vec<T, 8>(k_from + row * p.k_stride_t + d, x, newt::any_align());
-        newt::store_vec<T, 8>(k_lds + slot * 8, x);
-      }
-    }
-#pragma unroll
-    for (int c = 0; c < ROUNDS; ++c) {
-      const int first = c * THREADS + 64 * wave, slot = first + lane;
-      int row, d;
+      put(k_from + up * p.k_stride_t, row, d, p.k_stride_t, row < rows - up,
+          k_lds + first * 8);
       VTile::slot(slot, row, d);
-      if constexpr (DIRECT) {
-        newt::lds_dma16_masked(v_from, (u32)(row * (int)p.v_stride_t + d) * sizeof(T), row < rows,
-                               v_lds + first * 8);
-      } else {
-        T x[8] = {};
-        if (row < rows)
-          newt::load_vec<T, 8>(v_from + row * p.v_stride_t + d, x, newt::any_align());
-        newt::store_vec<T, 8>(v_lds + slot * 8, x);
-      }
+      put(v_from + up * p.v_stride_t, row, d, p.v_stride_t, row < rows - up,
+          v_lds + first * 8);
+    }
+  }
+  // 8 numbers of a row to this lane's 16 bytes of the wave's at `to`, or zeros.
+  __device__ __forceinline__ static void put(const T* from, int row, int d, int64_t stride, bool in,
+                                             T* to) {
+    if constexpr (DIRECT) {
+      newt::lds_dma16_masked(from, (u32)(row * (int)stride + d) * sizeof(T), in, to);
+    } else {
+      T x[8] = {};
+      if (in) newt::load_vec<T, 8>(from + row * stride + d, x, newt::any_align());
+      newt::store_vec<T, 8>(to + (threadIdx.x & 63) * 8, x);
     }
   }
 
@@ -111,31 +108,32 @@ struct Program {
     }
   }
 
-  // One tile, while the next one is on its way.
-  __device__ __forceinline__ void step(int i, int to, T* now, T* next, float to_log2) {
-    // this tile's pieces have arrived, and no wave still reads the other stage
-    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
-    __syncthreads();
-    if (i + 1 < to) stage(range.tile(i + 1), next);
-    tile<false>(range.tile(i), now, to_log2);
+  __device__ __forceinline__ static float add(const bf16x8& w, float l) {
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    const bf16x2 one = {(bf16)1.0f, (bf16)1.0f};
+#pragma unroll
+    for (int j = 0; j < 8; j += 2)
+      l = __builtin_amdgcn_fdot2_f32_bf16(bf16x2{w[j], w[j + 1]}, one, l, false);
+    return l;
+  }
+  __device__ __forceinline__ static float add(const f16x8& w, float l) {
+    typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+    const f16x2 one = {(f16)1.0f, (f16)1.0f};
+#pragma unroll
+    for (int j = 0; j < 8; j += 2)
+      l = __builtin_amdgcn_fdot2(f16x2{w[j], w[j + 1]}, one, l, false);
+    return l;
   }
 
+  // A tile's scores to weights, masked where a row does not see a key. (The
+  // branch costs 32 register moves; a copy of the code behind it for either way,
+  // without them, is slower, 352 against 316 us for 4 x 32 x 4096 x 128 in a
+  // window of 1024: exponentials then no longer run beside the products.)
   template <bool CAREFUL>
-  __device__ __forceinline__ void tile(int key, const T* k_lds, float to_log2) {
-    const int lane = threadIdx.x & 63, half = lane >> 5;
-    const T* v_lds = k_lds + kTile * D;
-    f32x16 s[2];
-#pragma unroll
-    for (int kh = 0; kh < 2; ++kh) {
-      s[kh] = (f32x16)(0.0f);
-#pragma unroll
-      for (int st = 0; st < STEPS; ++st)
-        s[kh] = newt::mfma_32x32x16(
-            __builtin_bit_cast(TX, newt::lds_frag_k<T, D, 32>(k_lds, 32 * kh, 16 * st, lane)),
-            q[st], s[kh]);
-    }
+  __device__ __forceinline__ void weigh(f32x16 (&s)[2], int key, float to_log2, TX (&w)[4],
+                                        u32& seen) {
+    const int half = (threadIdx.x & 63) >> 5;
     // bit 16 kh + e: whether the row sees the key of s[kh][e]
-    u32 seen = ~0u;
     if (CAREFUL || !range.whole(key)) {
       const int at = key + 4 * half;
       const auto offset = [](int kh, int e) { return 32 * kh + 8 * (e / 4) + e % 4; };
@@ -174,19 +172,47 @@ struct Program {
       m = to_m;
     }
     const float ref = m == -kInf ? 0.0f : m;
-    TX w[4];
 #pragma unroll
     for (int kh = 0; kh < 2; ++kh)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kh][e], to_log2, -ref));
-        l += x;
-        w[2 * kh + e / 8][e % 8] = (T)x;
-      }
+      for (int e = 0; e < 16; ++e)
+        w[2 * kh + e / 8][e % 8] =
+            (T)__builtin_amdgcn_exp2f(__builtin_fmaf(s[kh][e], to_log2, -ref));
+    // the sum of the weights as the product takes them, two at a time
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt)
+    for (int i = 0; i < 4; ++i) l = add(w[i], l);
+  }
+
+  // One tile, while the next one is on its way.
+  __device__ __forceinline__ void step(int i, int to, T* now, T* next, float to_log2) {
+    // this tile's pieces have arrived, and no wave still reads the other stage
+    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
+    __syncthreads();
+    if (i + 1 < to) stage(range.tile(i + 1), next);
+    tile<false>(range.tile(i), now, to_log2);
+  }
+
+  template <bool CAREFUL>
+  __device__ __forceinline__ void tile(int key, const T* k_lds, float to_log2) {
+    const int lane = threadIdx.x & 63;
+    const T* v_lds = k_lds + kTile * D;
+    f32x16 s[2];
 #pragma unroll
-      for (int ks = 0; ks < 4; ++ks) {
+    for (int kh = 0; kh < 2; ++kh) {
+      s[kh] = (f32x16)(0.0f);
+#pragma unroll
+      for (int st = 0; st < STEPS; ++st)
+        s[kh] = newt::mfma_32x32x16(
+            __builtin_bit_cast(TX, newt::lds_frag_k<T, D, 32>(k_lds, 32 * kh, 16 * st, lane)),
+            q[st], s[kh]);
+    }
+    u32 seen = ~0u;
+    TX w[4];
+    weigh<CAREFUL>(s, key, to_log2, w, seen);
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks)
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) {
         i16x8 a = newt::lds_frag_r_perm32<T, D>(v_lds, 32 * dt, 16 * ks, lane);
         if constexpr (CAREFUL) a = keep_apart(a, seen >> (8 * ks), acc[dt]);
         acc[dt] = newt::mfma_32x32x16(__builtin_bit_cast(TX, a), w[ks], acc[dt]);
@@ -310,13 +336,6 @@ window_attention_kernel(newt_window_attention_params p, int splits, int row_tile
     }
 }
 
-Plan plan(const newt_window_attention_params& p) {
-  Plan r(p.batch, p.q_len, p.kv_heads, p.heads / p.kv_heads, 128);
-  const int64_t tiles = most_tiles(p.kv_len, p.window, p.sinks, p.q_len);
-  r.splits = split_count(r.units, tiles, 512, 4);
-  return r;
-}
-
 // Whether every piece of 8 numbers that a tile is staged in is aligned.
 bool direct(const newt_window_attention_params& p) {
   const int64_t strides = p.k_stride_b | p.k_stride_h | p.k_stride_t | p.v_stride_b |
@@ -326,6 +345,40 @@ bool direct(const newt_window_attention_params& p) {
          p.k_stride_t < (1 << 22) && p.v_stride_t < (1 << 22);
 }
 
+// Splits of the rows' tiles. Up to 256 programs have a CU each; a program's
+// tile takes about D / 100 us (1.27 for 128 head dims, 0.93 for 64), the kernel
+// that joins the splits 3.5 us and what writing and reading the partial results
+// at 2.5 TB/s takes: us for 1, 2, 4, 8, 16, 32 splits of
+//   one token over 8192 keys, 8 KV heads, 4 query heads each: 162 / 86 / 47 /
+//   28 / 18 / 14; 16 sequences, window 4096: 87 / 52 / 49 / 51 / 52 / 63;
+//   128 of 4096: 86 / 52 / 34 / 29 / 29 / 41; 512 of 2048, window 512: 20 / 31;
+//   3 x 16 heads of 64, 333 of 1999, window 500: 17 / 29.
+// From 512 programs of 256 rows on (two for each CU, one after the other), 8
+// waves share each tile: 4 x 32 x 4096 x 128 in a window of 1024 327 -> 315 us.
+Plan plan(const newt_window_attention_params& p) {
+  const int group = p.heads / p.kv_heads;
+  Plan r(p.batch, p.q_len, p.kv_heads, group, 256);
+  if (p.head_dim <= 128 && r.units >= 512 && direct(p)) return r;
+  r = Plan(p.batch, p.q_len, p.kv_heads, group, 128);
+  const int64_t span = p.q_len < 128 ? p.q_len : (127 / group) + 2;
+  const int64_t tiles = most_tiles(p.kv_len, p.window, p.sinks, span);
+  // few rows wait for memory more than for products: two programs to a CU
+  int64_t most = r.units ? (r.all_rows <= 32 ? 512 : 256) / r.units : 1;
+  most = most < tiles ? most : tiles;
+  most = most < kMostSplits ? most : kMostSplits;
+  const double tile = 0.6 + p.head_dim * 0.0052;
+  const double each = 2.0 * p.batch * p.kv_heads * r.all_rows * (p.head_dim + 2) * 4 / 2.5e6;
+  double least = tiles * tile;
+  for (int n = 2; n <= most; ++n) {
+    const double cost = (tiles + n - 1) / n * tile + 3.5 + n * each;
+    if (cost < least) {
+      least = cost;
+      r.splits = n;
+    }
+  }
+  return r;
+}
+
 template <typename T, int D>
 int launch(const newt_window_attention_params& p, hipStream_t stream) {
   const Plan r = plan(p);
@@ -333,6 +386,12 @@ int launch(const newt_window_attention_params& p, hipStream_t stream) {
     return fail(NEWT_ERR_INVALID, "newt_window_attention: null workspace");
   if (r.too_large()) return fail(NEWT_ERR_INVALID, "newt_window_attention: too many queries");
   const dim3 grid((unsigned)(r.units * r.splits)), block(256);
+  if constexpr (D <= 128) {
+    if (r.rows == 256) {
+      window_attention_kernel<T, D, 8, true><<<grid, dim3(512), 0, stream>>>(p, 1, r.row_tiles);
+      return launched("newt_window_attention");
+    }
+  }
   if (direct(p))
     window_attention_kernel<T, D, 4, true><<<grid, block, 0, stream>>>(p, r.splits, r.row_tiles);
   else

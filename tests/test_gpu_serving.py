@@ -685,3 +685,21 @@ def test_graphs_and_streams():
     torch.cuda.synchronize()
     for a, b in zip(got, eager):
         assert same_values(a, b)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_window_many_rows(D):
+    """Launches of 256-row programs: sampled queries of every head, at the
+    window's edges and elsewhere, and NaN behind what a query sees."""
+    B, H, KV, S = 2, 64, 32, 1111
+    q = rnd(B, H, S, D, dtype=torch.bfloat16, seed=1)
+    k, v = rnd(B, KV, S, D, dtype=torch.bfloat16, seed=2), rnd(B, KV, S, D, dtype=torch.bfloat16, seed=3)
+    v[1, 3, 700] = float("nan")
+    got = W().window_attention(q, k, v, window=200, sinks=5)
+    at = [0, 1, 199, 200, 204, 205, 500, 699, 700, 899, 900, 1110]
+    for b in range(B):
+        want, a = orc.attention(q[b][:, at], k[b], v[b], at, 200, 5)
+        check_attention(got[b][:, at], want, a, torch.bfloat16, False, S, 0.0)
+    rows = torch.arange(S, device="cuda")
+    assert torch.equal(got[1, 6, :, 0].isnan(), (rows >= 700) & (rows < 900))
+    assert int(got.isnan().sum()) == 2 * 200 * D
