@@ -10,6 +10,8 @@
     first kernel launch.
   * libnewt_ops.so - the hand-written operators (include/newt_ops.h, csrc/ops),
     compiled by hipcc for gfx950, a file at a time side by side.
+  * _newt_ops - the operators' ordinary calls from tensors to launch (a CPython
+    extension on torch's C++ headers, linked to libnewt_ops.so); g++ builds it.
 
 Run: python -m newt_amd.build
 """
@@ -132,6 +134,24 @@ def build_operators():
     return out
 
 
+def build_calls():
+    """The operators' calls in C++ (csrc/newt_pyops.cpp)."""
+    import sysconfig
+    import torch
+    from torch.utils import cpp_extension
+    src = os.path.join(CSRC, "newt_pyops.cpp")
+    out = os.path.join(CSRC, "_newt_ops" + sysconfig.get_config_var("EXT_SUFFIX"))
+    tlib = os.path.join(os.path.dirname(torch.__file__), "lib")
+    includes = [f"-I{p}" for p in (*cpp_extension.include_paths(),
+                                   sysconfig.get_paths()["include"], f"{ROCM}/include")]
+    _run(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-w", "-D__HIP_PLATFORM_AMD__",
+          f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *includes, src, "-o",
+          out + ".tmp", f"-L{CSRC}", "-l:libnewt_ops.so", f"-L{tlib}", "-lc10", "-ltorch_cpu",
+          "-ltorch_python", "-Wl,-rpath,$ORIGIN"])
+    os.replace(out + ".tmp", out)
+    return out
+
+
 def build(verbose=True):
     lib = build_library()
     if verbose:
@@ -142,6 +162,9 @@ def build(verbose=True):
     operators = build_operators()
     if verbose:
         print("built", operators)
+    calls = build_calls()
+    if verbose:
+        print("built", calls)
     co = check_device_header()
     if verbose:
         print("device header compiled for gfx950:", co)

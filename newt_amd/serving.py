@@ -73,6 +73,41 @@ def lib():
     return L
 
 
+class _Fast:
+    """The operators' ordinary calls in C++ (csrc/newt_pyops.cpp, the _newt_ops
+    extension): each returns None for what is not plainly right, which the
+    Python of this file then looks into. Where the extension is not built, all
+    calls go through Python."""
+
+    module = None
+
+    @classmethod
+    def load(cls):
+        lib()
+        try:
+            import importlib.util
+            import sysconfig
+            path = os.path.join(os.path.dirname(LIB_PATH),
+                                "_newt_ops" + sysconfig.get_config_var("EXT_SUFFIX"))
+            spec = importlib.util.spec_from_file_location("_newt_ops", path)
+            module = importlib.util.module_from_spec(spec)
+            spec.loader.exec_module(module)
+        except (ImportError, OSError):
+            module = False
+        cls.module = module
+        return module
+
+
+def _fast(name, *args):
+    module = _Fast.module
+    if module is None:
+        module = _Fast.load()
+    if not module:
+        return None
+    device = _Dev.device()
+    return getattr(module, name)(*args, device, _Dev.stream(device))
+
+
 def _call(entry, what, params, device):
     status = entry(params, _Dev.stream(device))
     if status:
@@ -123,6 +158,10 @@ def rmsnorm(x, w, eps=1e-6, residual=None, out_dtype=None, group=None, out=None,
     scale in 8 bits, with fp32 scales [M, 1] of whole rows, or [M, N / group] of
     `group` (32, 64, 128, 256) columns each: scale = max(amax |y| / 448, 2^-126),
     amax over numbers. `hidden` given may be x or residual itself."""
+    r = _fast("rmsnorm", x, w, eps, residual, -1 if out_dtype is None else
+              _DTYPE.get(out_dtype, -2), group, out, hidden)
+    if r is not None:
+        return r
     device = _Dev.device()
     _tensors("rmsnorm", device, x=x, w=w, residual=residual, out=out, hidden=hidden)
     if x.dim() != 2 or x.shape[1] == 0:
@@ -185,6 +224,9 @@ def token_logprobs(logits, tokens, top=0, temperature=1.0):
     -inf have probability 0. A row that holds nothing else, a NaN or +inf gets
     NaN for all its values; NaN logits are not among its top_ids (-1 where
     there are too few others)."""
+    r = _fast("token_logprobs", logits, tokens, top, temperature)
+    if r is not None:
+        return r
     device = _Dev.device()
     _tensors("token_logprobs", device, logits=logits, tokens=tokens)
     if logits.dim() != 2 or logits.shape[1] == 0:
@@ -305,6 +347,8 @@ def kv_append(cache, k, v, block_table, start, count=None):
     position lies behind the table, or in a block that is not in the cache,
     are dropped, and all of a sequence with a negative start. No two sequences
     of a call may write to one block."""
+    if _fast("kv_append", cache, k, v, block_table, start, count):
+        return
     device = _Dev.device()
     _tensors("kv_append", device, k=k, v=v, start=start, count=count)
     if k.dim() != 4:
@@ -360,6 +404,9 @@ def cached_attention(q, cache, block_table, lens, window=None, sinks=0, scale=No
     not in the cache, are not seen; blocks that hold no visible token are not
     read, and their table entries may be anything. scale defaults to
     head_dim^-0.5."""
+    r = _fast("cached_attention", q, cache, block_table, lens, window, sinks, scale, out)
+    if r is not None:
+        return r
     device = _Dev.device()
     _tensors("cached_attention", device, q=q, lens=lens, out=out)
     out, window, scale = _queries("cached_attention", q, out, window, sinks, scale)
@@ -402,6 +449,9 @@ def window_attention(q, k, v, window=None, sinks=0, scale=None, q_start=None, ou
     never matter: what k and v hold behind the last query's position, or before
     every window, may be anything. Query heads share KV heads as in
     cached_attention. scale defaults to head_dim^-0.5."""
+    r = _fast("window_attention", q, k, v, window, sinks, scale, q_start, out)
+    if r is not None:
+        return r
     device = _Dev.device()
     _tensors("window_attention", device, q=q, k=k, v=v, q_start=q_start, out=out)
     out, window, scale = _queries("window_attention", q, out, window, sinks, scale)

@@ -29,6 +29,7 @@ def calls(monkeypatch):
         raise Launched(what)
     monkeypatch.setattr(serving, "_tensors", lambda *a, **k: None)
     monkeypatch.setattr(serving, "_call", call)
+    monkeypatch.setattr(serving, "_fast", lambda *a: None)
     monkeypatch.setattr(serving._Dev, "device", classmethod(lambda cls: 0))
     return None
 
@@ -39,7 +40,10 @@ def refused(kind, match, f, *args, **kw):
 
 
 def test_tensors_have_to_be_on_the_gpu(monkeypatch):
+    """Through the C++ calls too, which leave such tensors to Python."""
     monkeypatch.setattr(serving._Dev, "device", classmethod(lambda cls: 0))
+    monkeypatch.setattr(serving._Dev, "stream", staticmethod(lambda device: 0))
+    assert serving._Fast.load()
     x, t = torch.zeros(2, 64), torch.zeros(2, dtype=torch.int64)
     refused(TypeError, "current GPU", workloads.rmsnorm, x, x[0])
     refused(TypeError, "must be a tensor", workloads.rmsnorm, [1.0], x[0])
