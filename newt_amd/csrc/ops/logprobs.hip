@@ -7,8 +7,8 @@
 // one comparison a chunk: only a chunk that holds something larger than the
 // last entry that counts takes the slow path, which inserts it and, where the
 // maximum grew, rescales S and U. The list begins with the sorted largest
-// logits of each lane in the first chunk; after that n logits in no order make
-// about top * ln(n / 512) insertions. Lists are joined by bitonic merges.
+// logits of each lane in the first four chunks; after that n logits in no order
+// make about top * ln(n / 2048) insertions. Lists are joined by bitonic merges.
 #include "common.h"
 
 namespace newt_ops {
@@ -18,7 +18,6 @@ constexpr float kLog2e = 1.44269504088896341f;
 constexpr float kLn2 = 0.693147180559945309f;
 constexpr float kInf = __builtin_inff();
 constexpr int kNone = 0x7fffffff;  // the id of an entry that is none: behind all others
-constexpr int kWaves = 4;
 constexpr int kMostSplits = 64;
 
 __device__ __forceinline__ float uniform(float v, int lane) {
@@ -177,8 +176,9 @@ struct Chunk {
   static constexpr int STEP = 64 * V;  // logits of a wave's chunk
   u32x4 raw;
 
+  // V logits at a 16-byte address; no other program reads them
   __device__ __forceinline__ void load(const T* x) {
-    raw = *reinterpret_cast<const typename newt::any_vec<T, V>::type*>(x);
+    raw = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(x));
   }
   // `n` of V logits, -inf behind
   __device__ __forceinline__ void load(const T* x, int64_t n) {
@@ -199,52 +199,65 @@ template <typename T>
 struct Wave {
   static constexpr int V = Chunk<T>::V;
   const int top, lane;
-  const int64_t hi;
   const float c;
+  int64_t hi;
   Sums s{-kInf, 0.0f, 0.0f};  // m is the wave's, S and U the lane's
   Entry e{-kInf, kNone};
   Entry last{-kInf, kNone};   // the last entry that counts
-  bool begun = false;
+  int taken = kNone;          // the logit that the lane gave to the list in begin()
+
+  __device__ __forceinline__ void find_last() {
+    last = Entry{uniform(e.value, top - 1), __builtin_amdgcn_readlane(e.id, top - 1)};
+  }
+
+  // Each lane's first largest logit of the first `n` chunks begins the list:
+  // with 64 sorted ones of up to 2048, few of the others come before the last.
+  template <int N>
+  __device__ __forceinline__ void begin(const Chunk<T> (&chunks)[N], int n, int64_t at,
+                                        int64_t step) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      if (j >= n) break;
+      float f[V];
+      chunks[j].get(f);
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const int64_t id = at + j * step + lane * V + i;
+        const bool better = (f[i] > e.value) | ((e.id == kNone) & (f[i] == f[i]));  // never NaN
+        if (better & (id < hi)) e = Entry{f[i], (int)id};
+      }
+    }
+    taken = e.id;
+    s.m = newt::lane_reduce<newt::Max, 63>(e.value);
+    if (!top) {
+      last.value = s.m;
+      return;
+    }
+    sort(e, lane);
+    find_last();
+  }
 
   // Candidates of a chunk into the list, whose last entry that counts decides
-  // which ones are. `taken`: the logit that the lane gave to the list already.
-  __device__ __forceinline__ void candidates(const float* f, int64_t at, int taken) {
+  // which ones are.
+  __device__ __forceinline__ void candidates(const float* f, int64_t at) {
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       const int id = (int)(at + lane * V + i);
-      const bool in = (i != taken) & (at + lane * V + i < hi);
       const Entry x{f[i], id};  // NaN comes before nothing
-      u64 found = __ballot(in & x.before(last));
+      u64 found = __ballot(x.before(last) & (id != taken) & (at + lane * V + i < hi));
       while (found) {
         const int from = __builtin_ctzll(found);
         insert(e, Entry{uniform(f[i], from), __builtin_amdgcn_readlane(id, from)}, lane);
-        last = Entry{uniform(e.value, top - 1), __builtin_amdgcn_readlane(e.id, top - 1)};
+        find_last();
         found &= found - 1;
         found &= __ballot(x.before(last));
       }
     }
   }
 
-  __device__ __forceinline__ void slow(const float* f, float most, int64_t at) {
-    const float highest = newt::lane_reduce<newt::Max, 63>(most);
-    if (top) {
-      int taken = -1;
-      if (!begun) {
-        begun = true;
-        // each lane's first largest logit begins the list
-#pragma unroll
-        for (int i = V - 1; i >= 0; --i)
-          if (f[i] == most && at + lane * V + i < hi) taken = i;
-        e = Entry{taken < 0 ? -kInf : most, taken < 0 ? kNone : (int)(at + lane * V + taken)};
-        sort(e, lane);
-        last = Entry{uniform(e.value, top - 1), __builtin_amdgcn_readlane(e.id, top - 1)};
-      }
-      candidates(f, at, taken);
-    }
-    s.rescale(highest, c);
-    if (!top) last.value = s.m;
-  }
-
+  // With EARLY, a chunk that ids of the list lie behind or among: an equal logit
+  // may come before the last entry.
+  template <bool EARLY>
   __device__ __forceinline__ void take(const Chunk<T>& chunk, int64_t at) {
     float f[V];
     chunk.get(f);
@@ -252,8 +265,12 @@ struct Wave {
 #pragma unroll
     for (int i = 1; i < V; ++i) most = __builtin_fmaxf(most, f[i]);
     most = __builtin_fmaxf(most, -kInf);  // of NaN alone: nothing
-    // top > 0 and entries missing: anything may still come in
-    if (__ballot(most > last.value) != 0 || (top && last.id == kNone)) slow(f, most, at);
+    // entries missing (fewer logits than alternatives so far): anything may come in
+    if (EARLY || __ballot(most > last.value) != 0 || (top && last.id == kNone)) {
+      if (top) candidates(f, at);
+      s.rescale(newt::lane_reduce<newt::Max, 63>(most), c);
+      if (!top) last.value = s.m;
+    }
     const float m = s.m == -kInf ? 0.0f : s.m;
     float d[V];
     if (near_zero(newt::bits_f32(__builtin_amdgcn_readfirstlane(newt::f32_bits(m))), c)) {
@@ -275,8 +292,8 @@ struct Wave {
   }
 };
 
-template <typename T>
-__global__ void __launch_bounds__(64 * kWaves)
+template <typename T, int WAVES>
+__global__ void __launch_bounds__(64 * WAVES)
 logprobs_kernel(newt_logprobs_params p, int splits, int64_t per_split) {
   constexpr int STEP = Chunk<T>::STEP, V = Chunk<T>::V;
   const int lane = threadIdx.x & 63, wave = wave_id();
@@ -288,47 +305,61 @@ logprobs_kernel(newt_logprobs_params p, int splits, int64_t per_split) {
   const int top = p.top;
   const float c = kLog2e * p.inv_temperature;
 
-  // chunks of the waves lie side by side; AHEAD of them are on their way while
-  // one is worked on, and none of those asks for bounds
+  // Rows of an odd length begin anywhere: the first wave takes what lies before
+  // the first 16-byte address. From there on the waves' chunks lie side by
+  // side; AHEAD of them are on their way while one is worked on, and none of
+  // those asks for bounds.
   constexpr int AHEAD = 4;
-  Wave<T> w{top, lane, hi, c};
-  const int64_t step = kWaves * STEP, first = lo + wave * STEP;
+  Wave<T> w{top, lane, c, hi};
+  const int past = (int)((uintptr_t)(x + lo) % 16 / sizeof(T));
+  int64_t start = past ? lo + V - past : lo;
+  start = start < hi ? start : hi;
+  const int64_t step = WAVES * STEP, first = start + wave * STEP;
   const int whole = first + STEP <= hi ? (int)((hi - STEP - first) / step) + 1 : 0;
+  const int64_t behind = first + whole * step;  // the last chunk that is not whole, if any
   const T* from = x + first + lane * V;
-  Chunk<T> next[AHEAD];
+  Chunk<T> next[AHEAD], end[1];
   if (whole) {
     // behind the last whole chunk that one is loaded again, to no use
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i) next[i].load(from + (i < whole ? i : whole - 1) * step);
-    for (int j = 0; j < whole; j += AHEAD) {
+  }
+  if (behind < hi) end[0].load(from + whole * step, hi - behind - lane * V);
+  if (whole) w.begin(next, whole < AHEAD ? whole : AHEAD, first, step);
+  else if (behind < hi) w.begin(end, 1, behind, 0);
+  if (wave == 0 && start > lo) {
+    Chunk<T> head;
+    head.load(x + lo + lane * V, start - lo - lane * V);
+    w.hi = start;
+    w.template take<true>(head, lo);
+    w.hi = hi;
+  }
+  for (int j = 0; j < whole; j += AHEAD) {
 #pragma unroll
-      for (int i = 0; i < AHEAD; ++i) {
-        const Chunk<T> now = next[i];
-        const int to = j + i + AHEAD;
-        next[i].load(from + (to < whole ? to : whole - 1) * step);
-        if (j + i < whole) w.take(now, first + (j + i) * step);
-      }
+    for (int i = 0; i < AHEAD; ++i) {
+      const Chunk<T> now = next[i];
+      const int to = j + i + AHEAD;
+      next[i].load(from + (to < whole ? to : whole - 1) * step);
+      if (j + i >= whole) continue;
+      if (j == 0) w.template take<true>(now, first + i * step);
+      else w.template take<false>(now, first + (j + i) * step);
     }
   }
-  if (first + whole * step < hi) {
-    Chunk<T> end;
-    end.load(from + whole * step, hi - (first + whole * step) - lane * V);
-    w.take(end, first + whole * step);
-  }
+  if (behind < hi) w.template take<true>(end[0], behind);
 
   Sums s = w.s;
   Entry e = w.e;
   s.join(c);
-  __shared__ Sums sums[kWaves];
-  __shared__ Entry entries[kWaves][64];
+  __shared__ Sums sums[WAVES];
+  __shared__ Entry entries[WAVES][64];
   if (lane == 0) sums[wave] = s;
   entries[wave][lane] = e;
   __syncthreads();
   if (wave != 0) return;
-  s = lane < kWaves ? sums[lane] : Sums{-kInf, 0.0f, 0.0f};
+  s = lane < WAVES ? sums[lane] : Sums{-kInf, 0.0f, 0.0f};
   s.join(c);
   if (top)
-    for (int i = 1; i < kWaves; ++i) merge(e, entries[i][63 - lane], lane);
+    for (int i = 1; i < WAVES; ++i) merge(e, entries[i][63 - lane], lane);
   if (splits == 1) {
     finish<T>(p, row, s, e, lane);
     return;
@@ -389,32 +420,41 @@ __global__ void __launch_bounds__(1024) logprobs_join_kernel(newt_logprobs_param
   finish<T>(p, row, s, e, lane);
 }
 
-// How a row is shared out: enough workgroups to fill the chip where there are
-// few rows, each with at least 4096 logits.
-void plan(int64_t rows, int64_t vocab, int* splits, int64_t* per_split) {
-  int64_t n = rows ? (1024 + rows - 1) / rows : 1;
-  const int64_t most = (vocab + 4095) / 4096;
-  n = n < most ? n : most;
-  n = n < 1 ? 1 : n < kMostSplits ? n : kMostSplits;
-  int64_t per = (vocab + n - 1) / n;
-  per = (per + 7) / 8 * 8;
-  *splits = (int)((vocab + per - 1) / per);
-  *per_split = per;
+// How rows are shared out: to 16 waves for each CU, as the list that each wave
+// begins, and joins with the others', costs it as much as 10000 logits do. Few
+// rows go to several workgroups each, with at least 8192 logits.
+struct Plan {
+  int waves, splits;
+  int64_t per_split;
+  Plan(int64_t rows, int64_t vocab) {
+    waves = rows >= 4096 ? 1 : rows >= 2048 ? 2 : 4;
+    int64_t n = rows ? (512 + rows - 1) / rows : 1;
+    const int64_t most = (vocab + 8191) / 8192;
+    n = n < most ? n : most;
+    n = n < 1 ? 1 : n < kMostSplits ? n : kMostSplits;
+    per_split = ((vocab + n - 1) / n + 7) / 8 * 8;
+    splits = (int)((vocab + per_split - 1) / per_split);
+  }
+};
+
+template <typename T, int WAVES>
+void start(const newt_logprobs_params& p, const Plan& r, hipStream_t stream) {
+  logprobs_kernel<T, WAVES><<<dim3((unsigned)(p.rows * r.splits)), dim3(64 * WAVES), 0, stream>>>(
+      p, r.splits, r.per_split);
 }
 
 template <typename T>
 int launch(const newt_logprobs_params& p, hipStream_t stream) {
-  int splits;
-  int64_t per;
-  plan(p.rows, p.vocab, &splits, &per);
-  if (splits > 1 && !p.workspace)
+  const Plan r(p.rows, p.vocab);
+  if (r.splits > 1 && !p.workspace)
     return fail(NEWT_ERR_INVALID, "newt_token_logprobs: null workspace");
-  if (p.rows * splits > 0x7fffffff)
+  if (p.rows * r.splits > 0x7fffffff)
     return fail(NEWT_ERR_INVALID, "newt_token_logprobs: too many rows");
-  logprobs_kernel<T><<<dim3((unsigned)(p.rows * splits)), dim3(64 * kWaves), 0, stream>>>(p, splits,
-                                                                                          per);
-  if (splits > 1)
-    logprobs_join_kernel<T><<<dim3((unsigned)p.rows), dim3(1024), 0, stream>>>(p, splits);
+  if (r.waves == 1) start<T, 1>(p, r, stream);
+  else if (r.waves == 2) start<T, 2>(p, r, stream);
+  else start<T, 4>(p, r, stream);
+  if (r.splits > 1)
+    logprobs_join_kernel<T><<<dim3((unsigned)p.rows), dim3(1024), 0, stream>>>(p, r.splits);
   return launched("newt_token_logprobs");
 }
 
@@ -423,10 +463,8 @@ int launch(const newt_logprobs_params& p, hipStream_t stream) {
 
 extern "C" size_t newt_token_logprobs_workspace(int64_t rows, int64_t vocab, int32_t top, int32_t) {
   if (rows <= 0 || vocab <= 0) return 0;
-  int splits;
-  int64_t per;
-  newt_ops::plan(rows, vocab, &splits, &per);
-  return splits > 1 ? (size_t)rows * splits * (2 * top + 4) * sizeof(float) : 0;
+  const newt_ops::Plan r(rows, vocab);
+  return r.splits > 1 ? (size_t)rows * r.splits * (2 * top + 4) * sizeof(float) : 0;
 }
 
 extern "C" int newt_token_logprobs(const newt_logprobs_params* params, void* stream) {

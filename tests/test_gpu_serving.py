@@ -703,3 +703,19 @@ def test_window_many_rows(D):
     rows = torch.arange(S, device="cuda")
     assert torch.equal(got[1, 6, :, 0].isnan(), (rows >= 700) & (rows < 900))
     assert int(got.isnan().sum()) == 2 * 200 * D
+
+
+def test_logprobs_uneven_parts():
+    """Rows whose parts differ by much, so that some waves hold none of the
+    alternatives and larger numbers come late: stairs up and down, a few large
+    logits in front, all of them at the end."""
+    V = 30001
+    g = torch.Generator(device="cuda").manual_seed(3)
+    noise = torch.randn(6, V, generator=g, device="cuda")
+    at = torch.arange(V, device="cuda")
+    base = torch.stack([at // 512 * 3.0, -(at // 512) * 3.0, (at // 512 % 4) * 40.0,
+                        torch.where(at < 9, 300.0, 0.0), torch.where(at > V - 9, 300.0, -300.0),
+                        ((at // 512 % 4) == 3) * 25.0])
+    check_logprobs(base + noise, torch.full((6,), 17, device="cuda"), 20)
+    check_logprobs((base + noise)[:, 3:], torch.full((6,), 17, device="cuda"), 5)
+    check_logprobs((base * 0.1 + noise).half(), torch.full((6,), 17, device="cuda"), 0)
