@@ -177,9 +177,8 @@ template <typename T, int D>
 int join_splits(const void* workspace, void* out, Rows o, const Plan& r, int kv_heads, int group,
                 hipStream_t stream) {
   const int64_t waves = r.units / r.row_tiles * r.all_rows;
-  join_splits_kernel<T, D><<<dim3((unsigned)((waves + 3) / 4)), dim3(256), 0, stream>>>(
-      workspace, out, o, r.units, r.splits, r.rows, r.row_tiles, r.all_rows, kv_heads, group);
-  return launched("join_splits");
+  return run("newt_window_attention", join_splits_kernel<T, D>, (waves + 3) / 4, 256, 0, stream,
+             workspace, out, o, r.units, r.splits, r.rows, r.row_tiles, r.all_rows, kv_heads, group);
 }
 
 }  // namespace newt_ops

@@ -713,15 +713,13 @@ size_t workspace_of(const Launch& r) {
 
 template <typename T, int D, int MT>
 int launch(const newt_cached_attention_params& p, const Launch& r, hipStream_t stream) {
-  cached_attention_kernel<T, D, MT>
-      <<<dim3((unsigned)(r.shares ? r.shares : r.units)), dim3(64 * kWaves), 0, stream>>>(
-          p, r.row_tiles, r.shares);
-  if (r.shares) {
-    const int64_t waves = p.batch * p.heads * p.q_len;
-    cached_join_kernel<T, D, 16 * MT><<<dim3((unsigned)((waves + 3) / 4)), dim3(256), 0, stream>>>(
-        p, r.row_tiles, r.shares);
-  }
-  return launched("newt_cached_attention");
+  const char* const what = "newt_cached_attention";
+  const int status = run(what, cached_attention_kernel<T, D, MT>, r.shares ? r.shares : r.units,
+                         64 * kWaves, 0, stream, p, r.row_tiles, r.shares);
+  if (status != NEWT_OK || !r.shares) return status;
+  const int64_t waves = p.batch * p.heads * p.q_len;
+  return run(what, cached_join_kernel<T, D, 16 * MT>, (waves + 3) / 4, 256, 0, stream, p,
+             r.row_tiles, r.shares);
 }
 
 template <typename T, int D>

@@ -16,8 +16,21 @@ namespace newt_ops {
 // that reporting an error cannot fail itself.
 int fail(int status, const char* format, ...) __attribute__((format(printf, 2, 3)));
 
-// The status of a kernel launch just made.
-int launched(const char* what);
+int hip_fail(hipError_t e, const char* what);
+
+template <typename T> struct same { typedef T type; };
+
+// Launches a kernel and gives this launch's own status: what other code's
+// calls have left behind is not looked at.
+template <typename... P>
+int run(const char* what, void (*kernel)(P...), int64_t grid, int block, unsigned lds,
+        hipStream_t stream, typename same<P>::type... args) {
+  void* list[] = {static_cast<void*>(&args)...};
+  const hipError_t e = hipLaunchKernel(reinterpret_cast<const void*>(kernel),
+                                       dim3((unsigned)grid), dim3((unsigned)block), list, lds,
+                                       stream);
+  return e == hipSuccess ? NEWT_OK : hip_fail(e, what);
+}
 
 // What is wrong with a cache's description, or null.
 const char* cache_wrong(const newt_kv_cache& c);

@@ -18,9 +18,7 @@ int fail(int status, const char* format, ...) {
   return status;
 }
 
-int launched(const char* what) {
-  hipError_t e = hipGetLastError();
-  if (e == hipSuccess) return NEWT_OK;
+int hip_fail(hipError_t e, const char* what) {
   return fail(static_cast<int>(e), "%s: %s (%s)", what, hipGetErrorName(e), hipGetErrorString(e));
 }
 

@@ -41,7 +41,7 @@ __device__ __forceinline__ u32 scaled(u32 w, float f) {
 }
 
 // The part of a call that one workgroup does: one block of one sequence, one
-// head, its keys (blockIdx.z 0) or values (1).
+// head, its keys or its values.
 template <typename T>
 struct Part {
   bool live = false;
@@ -53,14 +53,16 @@ struct Part {
   float* scale;
 
   __device__ __forceinline__ Part(const newt_kv_append_params& p, int slots) {
-    const int b = blockIdx.x / slots, head = blockIdx.y;
+    const u32 heads = p.cache.kv_heads, at_head = blockIdx.x >> 1;
+    const u32 head = at_head % heads, slot_of = at_head / heads % (u32)slots;
+    const u32 b = at_head / heads / (u32)slots;
     const int size = p.cache.block_size, D = p.cache.head_dim;
-    values = blockIdx.z != 0;
+    values = blockIdx.x & 1;
     const int64_t start = p.start[b];
     int64_t count = p.count ? p.count[b] : p.tokens;
     count = count < p.tokens ? count : p.tokens;
     if (start < 0 || count <= 0) return;
-    const int64_t at = start / size + blockIdx.x % slots;  // the block's place in the sequence
+    const int64_t at = start / size + slot_of;  // the block's place in the sequence
     const int64_t first = at * size;
     if (first >= start + count || at >= p.table_width) return;
     const int64_t block = p.table[b * p.table_stride + at];
@@ -183,8 +185,14 @@ __global__ void __launch_bounds__(THREADS) kv_append_kernel(newt_kv_append_param
 #pragma unroll
     for (int i = 0; i < 8; ++i) top = newt::Max::op(top, finite_abs(newt::to_f32(x[c][i])));
   const float scale = part.template rescale<THREADS>(top, size, D);
-  const float by = 1.0f / scale;  // exact: a power of two from 2^-100 to 2^120
-  const auto put = [&](int c, int i) { return or_nan(newt::to_f32(x[c][i]) * by); };
+  // the scales made here are powers of two, whose reciprocals are exact; a
+  // larger one that the block came with need not be
+  const float by = 1.0f / scale;
+  const bool power = (newt::f32_bits(scale) & 0x7fffffu) == 0;
+  const auto put = [&](int c, int i) {
+    const float v = newt::to_f32(x[c][i]);
+    return or_nan(power ? v * by : v / scale);
+  };
 
   if (!part.values) {
 #pragma unroll
@@ -228,19 +236,17 @@ int launch(const newt_kv_append_params& p, hipStream_t stream) {
   const int size = p.cache.block_size;
   // blocks that `tokens` consecutive ones can reach
   const int64_t slots = (p.tokens + size - 2) / size + 1;
-  if (slots * p.batch > 0x7fffffff)
-    return fail(NEWT_ERR_INVALID, "newt_kv_append: too many tokens");
-  const dim3 grid((unsigned)(slots * p.batch), (unsigned)p.cache.kv_heads, 2);
+  // one program for each of them, each head, keys and values
+  const int64_t grid = slots * p.batch * p.cache.kv_heads * 2;
+  if (grid > 0x7fffffff) return fail(NEWT_ERR_INVALID, "newt_kv_append: too many tokens");
   const unsigned lds = size * D + D / 8 * 16;
-  if (p.tokens <= 4)
-    kv_append_few_kernel<T, D><<<grid, dim3(64), 0, stream>>>(p, (int)slots);
-  else if (size * D <= 8192)
-    kv_append_kernel<T, D, 256, 4><<<grid, dim3(256), lds, stream>>>(p, (int)slots);
-  else if (size * D <= 16384)
-    kv_append_kernel<T, D, 256, 8><<<grid, dim3(256), lds, stream>>>(p, (int)slots);
-  else
-    kv_append_kernel<T, D, 1024, 8><<<grid, dim3(1024), lds, stream>>>(p, (int)slots);
-  return launched("newt_kv_append");
+  const char* const what = "newt_kv_append";
+  if (p.tokens <= 4) return run(what, kv_append_few_kernel<T, D>, grid, 64, 0, stream, p, (int)slots);
+  if (size * D <= 8192)
+    return run(what, kv_append_kernel<T, D, 256, 4>, grid, 256, lds, stream, p, (int)slots);
+  if (size * D <= 16384)
+    return run(what, kv_append_kernel<T, D, 256, 8>, grid, 256, lds, stream, p, (int)slots);
+  return run(what, kv_append_kernel<T, D, 1024, 8>, grid, 1024, lds, stream, p, (int)slots);
 }
 
 template <typename T>

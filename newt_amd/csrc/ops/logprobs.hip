@@ -9,6 +9,9 @@
 // maximum grew, rescales S and U. The list begins with the sorted largest
 // logits of each lane in the first four chunks; after that n logits in no order
 // make about top * ln(n / 2048) insertions. Lists are joined by bitonic merges.
+// bf16 2048 x 100003, two sets in turn: 87 us (4.7 TB/s) without alternatives,
+// 95 with 5, 125 with 20; reading alone would take 58. 1 x 128000: 8 us without,
+// 15 with 20, of them 5 in the second kernel.
 #include "common.h"
 
 namespace newt_ops {
@@ -438,9 +441,9 @@ struct Plan {
 };
 
 template <typename T, int WAVES>
-void start(const newt_logprobs_params& p, const Plan& r, hipStream_t stream) {
-  logprobs_kernel<T, WAVES><<<dim3((unsigned)(p.rows * r.splits)), dim3(64 * WAVES), 0, stream>>>(
-      p, r.splits, r.per_split);
+int start(const newt_logprobs_params& p, const Plan& r, hipStream_t stream) {
+  return run("newt_token_logprobs", logprobs_kernel<T, WAVES>, p.rows * r.splits, 64 * WAVES, 0,
+             stream, p, r.splits, r.per_split);
 }
 
 template <typename T>
@@ -450,12 +453,11 @@ int launch(const newt_logprobs_params& p, hipStream_t stream) {
     return fail(NEWT_ERR_INVALID, "newt_token_logprobs: null workspace");
   if (p.rows * r.splits > 0x7fffffff)
     return fail(NEWT_ERR_INVALID, "newt_token_logprobs: too many rows");
-  if (r.waves == 1) start<T, 1>(p, r, stream);
-  else if (r.waves == 2) start<T, 2>(p, r, stream);
-  else start<T, 4>(p, r, stream);
-  if (r.splits > 1)
-    logprobs_join_kernel<T><<<dim3((unsigned)p.rows), dim3(1024), 0, stream>>>(p, r.splits);
-  return launched("newt_token_logprobs");
+  const int status = r.waves == 1   ? start<T, 1>(p, r, stream)
+                     : r.waves == 2 ? start<T, 2>(p, r, stream)
+                                    : start<T, 4>(p, r, stream);
+  if (status != NEWT_OK || r.splits == 1) return status;
+  return run("newt_token_logprobs", logprobs_join_kernel<T>, p.rows, 1024, 0, stream, p, r.splits);
 }
 
 }  // namespace

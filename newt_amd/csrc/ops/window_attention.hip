@@ -385,21 +385,20 @@ int launch(const newt_window_attention_params& p, hipStream_t stream) {
   if (r.splits > 1 && !p.workspace)
     return fail(NEWT_ERR_INVALID, "newt_window_attention: null workspace");
   if (r.too_large()) return fail(NEWT_ERR_INVALID, "newt_window_attention: too many queries");
-  const dim3 grid((unsigned)(r.units * r.splits)), block(256);
-  if constexpr (D <= 128) {
-    if (r.rows == 256) {
-      window_attention_kernel<T, D, 8, true><<<grid, dim3(512), 0, stream>>>(p, 1, r.row_tiles);
-      return launched("newt_window_attention");
-    }
-  }
-  if (direct(p))
-    window_attention_kernel<T, D, 4, true><<<grid, block, 0, stream>>>(p, r.splits, r.row_tiles);
-  else
-    window_attention_kernel<T, D, 4, false><<<grid, block, 0, stream>>>(p, r.splits, r.row_tiles);
-  if (r.splits > 1)
-    return join_splits<T, D>(p.workspace, p.out, {p.o_stride_b, p.o_stride_h, p.o_stride_t}, r,
-                             p.kv_heads, p.heads / p.kv_heads, stream);
-  return launched("newt_window_attention");
+  const char* const what = "newt_window_attention";
+  const int64_t grid = r.units * r.splits;
+  if constexpr (D <= 128)
+    if (r.rows == 256)
+      return run(what, window_attention_kernel<T, D, 8, true>, grid, 512, 0, stream, p, 1,
+                 r.row_tiles);
+  const int status =
+      direct(p) ? run(what, window_attention_kernel<T, D, 4, true>, grid, 256, 0, stream, p,
+                      r.splits, r.row_tiles)
+                : run(what, window_attention_kernel<T, D, 4, false>, grid, 256, 0, stream, p,
+                      r.splits, r.row_tiles);
+  if (status != NEWT_OK || r.splits == 1) return status;
+  return join_splits<T, D>(p.workspace, p.out, {p.o_stride_b, p.o_stride_h, p.o_stride_t}, r,
+                           p.kv_heads, p.heads / p.kv_heads, stream);
 }
 
 template <typename T>

@@ -719,3 +719,24 @@ def test_logprobs_uneven_parts():
     check_logprobs(base + noise, torch.full((6,), 17, device="cuda"), 20)
     check_logprobs((base + noise)[:, 3:], torch.full((6,), 17, device="cuda"), 5)
     check_logprobs((base * 0.1 + noise).half(), torch.full((6,), 17, device="cuda"), 0)
+
+
+def test_append_to_calibrated_scales():
+    """Blocks whose scales are no powers of two: kept while they do, whatever
+    the new tokens' own need is."""
+    for S in (3, 40):
+        cache = make_cache(12, 2, 32, 64, seed=S, low=-7, high=-3)
+        for c in cache[2:]:
+            c.mul_(1.37)
+        for c in cache[:2]:
+            c.copy_(torch.where(c.float().isnan(), 0.0, c.float()).to(E4M3))
+        table = torch.randperm(12, device="cuda").to(torch.int32).view(3, 4)
+        k, v = rnd(3, 2, S, 64, seed=S), rnd(3, 2, S, 64, seed=S + 1) * 30
+        want = orc.append(cache, k, v, table, ints(5, 31, 70))
+        W().kv_append(cache, k, v, table, ints(5, 31, 70))
+        got = numbers(cache)
+        assert torch.equal(got[2], want[2]) and torch.equal(got[3], want[3])
+        for a, b in zip(got[:2], want[:2]):
+            # a quotient in fp32 may round to the other side of a tie
+            assert float((a != b).double().mean()) <= 1e-4
+            assert bool(((a - b).abs() <= 2.0 ** -3 * b.abs() + 2.0 ** -9).all())
