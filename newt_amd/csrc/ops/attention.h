@@ -23,7 +23,8 @@ constexpr int kNoWindow = 0x7fffffff; // sees all keys before it
 constexpr float kSlack = 8.0f;
 
 // The keys that the rows of a program see: sinks [0, sinks) and [lo, hi).
-// Positions, lengths and windows stay below 2^30, so sums of two fit an int.
+// Windows, sinks and `keys` stay below 2^30; positions need not, but fit an int
+// with the tiles that a caller asks for behind the last one.
 struct Range {
   int first, last;  // positions of the program's first and last query
   int lo, hi, sinks;

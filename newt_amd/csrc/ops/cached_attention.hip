@@ -86,11 +86,18 @@ struct Deal {
         window(p.window ? (int)p.window : kNoWindow), sinks((int)p.sinks), shares(shares_),
         lane(threadIdx.x & 63), len0(lane < batch ? lens[lane] : 0) {}
 
+  // Lengths may be any number. Those near 2^31 are taken a little shorter, so
+  // that the key numbers of tiles asked for ahead, up to 10 tiles behind the
+  // range, fit an int; tables hold fewer than 2^30 tokens, so nothing else
+  // changes.
+  __device__ __forceinline__ static int bounded(int n) {
+    constexpr int most = 0x7fffffff - 16 * kTile;
+    return n < 0 ? 0 : n < most ? n : most;
+  }
   // A length, by the same wave-wide load for all that ask where there are up to
   // 64 sequences.
   __device__ __forceinline__ int length(int b) const {
-    const int n = b < 64 ? lane_of(len0, b) : lens[b];
-    return n > 0 ? n : 0;
+    return bounded(b < 64 ? lane_of(len0, b) : lens[b]);
   }
   // tiles of a sequence, for all of its row tiles
   __device__ __forceinline__ int tiles_of(int len) const {
@@ -100,8 +107,7 @@ struct Deal {
   // those of the lane's own sequence of 64 from `c` on
   __device__ __forceinline__ int own_tiles(int c) const {
     if (c + lane >= batch) return 0;
-    const int n = c ? lens[c + lane] : len0;
-    return tiles_of(n > 0 ? n : 0);
+    return tiles_of(bounded(c ? lens[c + lane] : len0));
   }
   struct Tiles {
     __device__ __forceinline__ int operator()(int tiles) const { return tiles; }

@@ -740,3 +740,22 @@ def test_append_to_calibrated_scales():
             # a quotient in fp32 may round to the other side of a tie
             assert float((a != b).double().mean()) <= 1e-4
             assert bool(((a - b).abs() <= 2.0 ** -3 * b.abs() + 2.0 ** -9).all())
+
+
+@pytest.mark.parametrize("B", [3, 70])
+@pytest.mark.parametrize("slots", [4, 40])
+def test_cached_lengths_of_any_size(B, slots):
+    """Lengths up to 2^31 - 1, far behind the table's end: by units and by
+    shares, with more sequences than a wave has lanes."""
+    some = (2 ** 31 - 1, 2 ** 31 - 65, 2 ** 30, 2 ** 30 + 77, 100, -2 ** 31, 2 ** 31 - 1024)
+    lens = [some[b % len(some)] for b in range(B)]
+    cache, table = fill_cache(1, 64, 64, [64 * slots] * 3, seed=slots)
+    table = table[torch.arange(B, device="cuda") % 3].contiguous()
+    q = rnd(B, 2, 2, 64, dtype=torch.bfloat16, seed=B)
+    held = 64 * slots
+    for window, sinks in ((None, 0), (64, 4), (500, 130), (2 ** 30 - 1, 0)):
+        got = W().cached_attention(q, cache, table, ints(*lens), window=window, sinks=sinks)
+        for b, n in enumerate(lens):
+            keys, values, has = orc.cached(cache, table, b, max(0, min(n, held)))
+            want, a = orc.attention(q[b], keys, values, range(n - 2, n), window, sinks, None, has)
+            check_attention(got[b], want, a, q.dtype, True, held, 0.0)
