@@ -268,7 +268,9 @@ window_attention_kernel(newt_window_attention_params p, int splits, int row_tile
   int start = (int)(p.kv_len - p.q_len);
   if (p.q_start) {
     start = p.q_start[b];
-    start = start < -kLimit ? -kLimit : start > kLimit ? kLimit : start;
+    // so that the queries' positions fit an int
+    const int most = 0x7ffffffe - q_len;
+    start = start < -kLimit ? -kLimit : start > most ? most : start;
   }
   const int r0 = row_tile * P::ROWS;
   const int r1 = r0 + P::ROWS < all_rows ? r0 + P::ROWS : all_rows;

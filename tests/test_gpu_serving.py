@@ -759,3 +759,12 @@ def test_cached_lengths_of_any_size(B, slots):
             keys, values, has = orc.cached(cache, table, b, max(0, min(n, held)))
             want, a = orc.attention(q[b], keys, values, range(n - 2, n), window, sinks, None, has)
             check_attention(got[b], want, a, q.dtype, True, held, 0.0)
+
+
+def test_window_positions_of_any_size():
+    """Queries far behind the keys or in front of them all."""
+    starts = ints(2 ** 31 - 1, 2 ** 30, 2 ** 30 + 90, -2 ** 31, -2 ** 30, 2 ** 31 - 200)
+    q = rnd(6, 2, 3, 64, dtype=torch.bfloat16, seed=1)
+    k, v = (rnd(6, 1, 150, 64, dtype=torch.bfloat16, seed=i) for i in (2, 3))
+    for window, sinks in ((None, 0), (64, 0), (64, 70), (2 ** 30 - 1, 0), (2 ** 30 - 1, 3)):
+        check_window(q, k, v, window=window, sinks=sinks, start=starts)
