@@ -151,6 +151,17 @@ join_splits_kernel(const void* workspace, void* out, Rows o, int64_t units, int 
   newt::store_vec<T, 4>(to, t, newt::any_align());
 }
 
+// What both operators refuse of their queries, outputs and scale; null: nothing.
+template <typename P>
+const char* queries_wrong(const P& p) {
+  if ((p.batch > 1 && p.o_stride_b == 0) || (p.heads > 1 && p.o_stride_h == 0) ||
+      (p.q_len > 1 && p.o_stride_t == 0))
+    return "rows of out overlap";
+  // scores and their exponents stay finite for ordinary queries and keys
+  if (!(__builtin_fabsf(p.scale) < 0x1p100f)) return "scale has to be finite, below 2^100";
+  return nullptr;
+}
+
 // At most so many tiles can a program of `span` queries visit.
 inline int64_t most_tiles(int64_t keys, int64_t window, int64_t sinks, int64_t span) {
   const int64_t all = (keys + kTile - 1) / kTile;

@@ -757,7 +757,7 @@ const char* wrong(const newt_cached_attention_params& p) {
   if (p.q_len * p.heads >= kLimit || p.table_width * p.cache.block_size >= kLimit ||
       p.window >= kLimit || p.sinks >= kLimit)
     return "sizes stay below 2^30";
-  return nullptr;
+  return queries_wrong(p);
 }
 
 }  // namespace

@@ -30,6 +30,7 @@ const char* cache_wrong(const newt_kv_cache& c) {
     return "head_dim is 64, 128 or 256";
   if (c.blocks < 0 || c.kv_heads <= 0 || c.kv_heads > 65535) return "bad number of blocks or heads";
   if (c.blocks && (!c.k || !c.v || !c.k_scale || !c.v_scale)) return "null cache tensor";
+  if (((uintptr_t)c.k | (uintptr_t)c.v) & 15) return "keys and values have to be aligned to 16 bytes";
   return nullptr;
 }
 

@@ -402,8 +402,8 @@ def cached_attention(q, cache, block_table, lens, window=None, sinks=0, scale=No
     neighbouring query heads. A query that sees nothing (its position is
     negative) gets zeros. Tokens behind the table, and those of blocks that are
     not in the cache, are not seen; blocks that hold no visible token are not
-    read, and their table entries may be anything. scale defaults to
-    head_dim^-0.5."""
+    read, and their table entries may be anything. scale (finite) defaults to
+    head_dim^-0.5. Rows of an `out` given must not overlap each other."""
     r = _fast("cached_attention", q, cache, block_table, lens, window, sinks, scale, out)
     if r is not None:
         return r
@@ -448,7 +448,7 @@ def window_attention(q, k, v, window=None, sinks=0, scale=None, q_start=None, ou
     query sees are not read where a whole tile of 64 of them is unseen, and
     never matter: what k and v hold behind the last query's position, or before
     every window, may be anything. Query heads share KV heads as in
-    cached_attention. scale defaults to head_dim^-0.5."""
+    cached_attention; scale and `out` are as there."""
     r = _fast("window_attention", q, k, v, window, sinks, scale, q_start, out)
     if r is not None:
         return r

@@ -768,3 +768,95 @@ def test_window_positions_of_any_size():
     k, v = (rnd(6, 1, 150, 64, dtype=torch.bfloat16, seed=i) for i in (2, 3))
     for window, sinks in ((None, 0), (64, 0), (64, 70), (2 ** 30 - 1, 0), (2 ** 30 - 1, 3)):
         check_window(q, k, v, window=window, sinks=sinks, start=starts)
+
+
+def test_attention_refuses_expanded_outputs():
+    """As Python errors, whichever way the call takes."""
+    q = rnd(2, 4, 3, 64, dtype=torch.bfloat16)
+    k = rnd(2, 2, 70, 64, dtype=torch.bfloat16)
+    cache, table = fill_cache(2, 64, 64, (64, 64), seed=1)
+    one = torch.empty(1, 4, 3, 64, dtype=torch.bfloat16, device="cuda").expand(2, 4, 3, 64)
+    with pytest.raises(ValueError, match="overlap"):
+        W().window_attention(q, k, k, out=one)
+    with pytest.raises(ValueError, match="overlap"):
+        W().cached_attention(q, cache, table, ints(64, 64), out=one)
+    with pytest.raises(ValueError, match="scale"):
+        W().window_attention(q, k, k, scale=float("inf"))
+    # read-only operands may be expanded
+    check_window(q, k[:, :1].expand(2, 2, 70, 64), k[:1].expand(2, 2, 70, 64))
+    check_window(q[:, :, :1].expand(2, 4, 3, 64), k[:, :, :1].expand(2, 2, 70, 64), k)
+
+
+def test_cached_many_sequences_and_rows():
+    """More sequences than a wave has lanes, of uneven lengths, in runs and in
+    parts, and row tiles of many queries over a long cache."""
+    for B, longest, KV, H, S, D in ((130, 900, 2, 4, 1, 64), (300, 130, 1, 1, 2, 64),
+                                    (66, 6000, 1, 4, 1, 128), (2, 5000, 2, 8, 40, 64),
+                                    (3, 2500, 1, 8, 5, 256)):
+        lens = [1 + (b * 7919) % longest for b in range(B)]
+        lens[B // 2] = 0
+        cache, table = fill_cache(KV, 64, D, lens, seed=B, outlier=False)
+        q = rnd(B, H, S, D, dtype=torch.bfloat16, seed=B)
+        check_cached(q, cache, table, lens)
+        if S > 1:
+            check_cached(q, cache, table, lens, window=700, sinks=3)
+
+
+def test_offsets_past_32_bits():
+    """Rows, keys and blocks whose byte offsets, and element offsets of the
+    8-bit cache, pass 2^32."""
+    bf16 = torch.bfloat16
+    blocks = 2 ** 19 + 5  # of 8192 bytes
+    cache = W().kv_cache(blocks, 1, 128)
+    table = torch.tensor([[blocks - 1, 3, blocks - 2]], dtype=torch.int32, device="cuda")
+    k, v = rnd(1, 1, 150, 128, dtype=bf16, seed=1), rnd(1, 1, 150, 128, dtype=bf16, seed=2)
+    W().kv_append(cache, k, v, table, ints(0))
+    small = W().kv_cache(3, 1, 128)
+    order = torch.tensor([[2, 0, 1]], dtype=torch.int32, device="cuda")
+    W().kv_append(small, k, v, order, ints(0))
+    for big, little in zip(cache, small):
+        for at, to in ((blocks - 1, 2), (3, 0), (blocks - 2, 1)):
+            assert torch.equal(big[at].view(torch.uint8), little[to].view(torch.uint8))
+    q = rnd(1, 4, 2, 128, dtype=bf16, seed=3)
+    assert torch.equal(W().cached_attention(q, cache, table, ints(150)),
+                       W().cached_attention(q, small, order, ints(150)))
+    del cache, big
+    # 2^32 bytes and more from the first key to the last: a stride of 2^23 numbers
+    keys = torch.zeros(300 * 2 ** 23, dtype=bf16, device="cuda").view(300, 2 ** 23)
+    k, v = rnd(1, 1, 300, 64, dtype=bf16, seed=4), rnd(1, 1, 300, 64, dtype=bf16, seed=5)
+    keys[:, :64], keys[:, 64:128] = k[0, 0], v[0, 0]
+    q = rnd(1, 2, 70, 64, dtype=bf16, seed=6)
+    far = [keys[:, i:i + 64].view(1, 1, 300, 64) for i in (0, 64)]
+    assert torch.equal(W().window_attention(q, *far, window=90, sinks=3),
+                       W().window_attention(q, k, v, window=90, sinks=3))
+    # and rows of the norm and of the logits
+    x = keys[:, :1000]
+    w = torch.ones(1000, dtype=bf16, device="cuda")
+    assert torch.equal(W().rmsnorm(x, w)[0], W().rmsnorm(x.contiguous(), w)[0])
+    t = torch.arange(300, device="cuda")
+    for a, b in zip(W().token_logprobs(x, t, top=4), W().token_logprobs(x.contiguous(), t, top=4)):
+        assert torch.equal(a, b)
+
+
+def test_calls_of_both_paths_agree(monkeypatch):
+    """The calls made in C++ and those made in Python give the same bytes."""
+    from newt_amd import serving
+    bf16 = torch.bfloat16
+    x, r, w = (rnd(7, 512, dtype=bf16, seed=i) for i in (1, 2, 3))
+    q, k = rnd(2, 4, 5, 64, dtype=bf16, seed=4), rnd(2, 2, 900, 64, dtype=bf16, seed=5)
+    logits, t = rnd(3, 30000, dtype=bf16, seed=6), torch.tensor([5, -1, 29999], device="cuda")
+    table = torch.arange(30, device="cuda").to(torch.int32).view(2, 15)
+
+    def calls():
+        cache = W().kv_cache(30, 2, 64)
+        W().kv_append(cache, k, k, table, ints(0, 3), ints(900, 800))
+        return [*W().rmsnorm(x, w[0], residual=r, out_dtype=E4M3, group=128),
+                *W().token_logprobs(logits, t, top=6, temperature=0.7),
+                W().window_attention(q, k, k, window=300, sinks=4, q_start=ints(800, 20)),
+                W().cached_attention(q, cache, table, ints(900, 803), window=500, sinks=2), *cache]
+
+    fast = calls()
+    monkeypatch.setattr(serving, "_fast", lambda *a: None)
+    for a, b in zip(fast, calls()):
+        assert a.dtype == b.dtype and a.stride() == b.stride()
+        assert torch.equal(a.contiguous().view(torch.uint8), b.contiguous().view(torch.uint8))

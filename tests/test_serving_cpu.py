@@ -326,3 +326,31 @@ def test_attention_definition():
     torch.testing.assert_close(a, w @ v.abs())
     o, _ = orc.attention(q, k, v, range(-3, 2))
     assert bool((o[:, :3] == 0).all()) and bool((o[:, 3:] != 0).any())
+
+
+def test_attention_refuses_overlapping_rows_and_scales():
+    """Rows of an output that share memory, which programs would write at once,
+    and scales that are not finite: an error before the GPU is touched."""
+    L = serving.lib()
+    P = 4096
+    cache = [P, P, P, P, 4, 2, 16, 64, 0]
+
+    def cached(o=(512, 128, 64), batch=2, q_len=2, heads=4, scale=1.0):
+        return L.newt_cached_attention(serving._CACHED.pack(
+            *cache, P, P, P, P, 0, batch, q_len, 1, 1, 512, 128, 64, *o, 0, 0, scale, heads, 2, 0),
+            None)
+
+    def window(o=(512, 128, 64), batch=2, q_len=2, heads=4, scale=1.0):
+        return L.newt_window_attention(serving._WINDOW.pack(
+            P, P, P, P, 0, 0, batch, q_len, 1, *[64] * 9, *o, 0, 0, scale, heads, 2, 64, 2, 0), None)
+
+    cache[0] = P + 8
+    assert cached() == 10002 and b"aligned" in L.newt_ops_last_error()
+    cache[0] = P
+    for call in (cached, window):
+        for o in ((0, 128, 64), (512, 0, 64), (512, 128, 0)):
+            assert call(o) == 10002
+            assert b"overlap" in L.newt_ops_last_error()
+        for scale in (float("inf"), -float("inf"), float("nan"), 2.0 ** 100):
+            assert call(scale=scale) == 10002
+            assert b"scale" in L.newt_ops_last_error()
