@@ -130,7 +130,13 @@ struct Sums {
   // The same relative to the maximum `to` >= m.
   __device__ __forceinline__ void rescale(float to, float c) {
     if (!(to > m)) return;
-    const float d = near_zero(to, c) ? m * c - to * c : (m - to) * c;
+    float d;
+    {
+      // both products rounded, as those that S and U are relative to: an fma of
+      // one would leave the other's rounding in them, 2^-25 |m c| each time
+#pragma clang fp contract(off)
+      d = near_zero(to, c) ? m * c - to * c : (m - to) * c;
+    }
     const float f = __builtin_amdgcn_exp2f(d);
     if (f == 0.0f && S == S) {
       S = U = 0.0f;

@@ -860,3 +860,17 @@ def test_calls_of_both_paths_agree(monkeypatch):
     for a, b in zip(fast, calls()):
         assert a.dtype == b.dtype and a.stride() == b.stride()
         assert torch.equal(a.contiguous().view(torch.uint8), b.contiguous().view(torch.uint8))
+
+
+@pytest.mark.parametrize("V", [4000, 70001])
+@pytest.mark.parametrize("offset,temperature", [(1e3, 1.0), (-1e3, 1.0), (1e4, 1.0), (-1e4, 1.0),
+                                                (1e5, 1.0), (-1e5, 1.0), (20.0, 0.02),
+                                                (-20.0, 0.02)])
+def test_logprobs_far_from_zero(V, offset, temperature):
+    """fp32 rows around a common offset: what a row's results are relative to
+    drops out, so the bound is that of rows around 0. Maxima differ between
+    waves and splits, and in half of the rows grow towards the end."""
+    x = rnd(8, V, seed=V, scale=3.0)
+    x[4:] += torch.linspace(0, 6, V, device="cuda")
+    check_logprobs(x * temperature + offset, torch.arange(8, device="cuda") * (V // 8), 5,
+                   temperature=temperature)
