@@ -22,6 +22,16 @@ constexpr int kNoWindow = 0x7fffffff; // sees all keys before it
 // fp32 sums and stays far below fp16's largest number.
 constexpr float kSlack = 8.0f;
 
+// Weights are 2^(score c - m) by one fma, where m is the largest score times c,
+// rounded: by up to half a step, 2^-1 below this. A row whose m lies beyond it is
+// done again with each score times c rounded first, so that the largest one's
+// exponent is 0 whatever the scale.
+constexpr float kExact = 8388608.0f;  // 2^23
+
+__device__ __forceinline__ bool beyond_exact(float m) {
+  return (__builtin_fabsf(m) > kExact) & (m != -kInf);
+}
+
 // The keys that the rows of a program see: sinks [0, sinks) and [lo, hi).
 // Windows, sinks and `keys` stay below 2^30; positions need not, but fit an int
 // with the tiles that a caller asks for behind the last one.

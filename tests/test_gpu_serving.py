@@ -874,3 +874,18 @@ def test_logprobs_far_from_zero(V, offset, temperature):
     x[4:] += torch.linspace(0, 6, V, device="cuda")
     check_logprobs(x * temperature + offset, torch.arange(8, device="cuda") * (V // 8), 5,
                    temperature=temperature)
+
+
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("scale", [1e4, 1e7, -1e8, 3e9, 1e15, 1e28])
+def test_window_large_scores(dtype, scale):
+    """Scores far above 2^24, whose products with log2(e) are rounded by more
+    than the exponent of a weight can be off: whole numbers, so that a row's
+    weights are equal among its largest scores and 0 elsewhere."""
+    g = torch.Generator(device="cuda").manual_seed(7)
+    q, k = (torch.randint(-3, 4, s, generator=g, device="cuda").to(dtype)
+            for s in ((2, 4, 70, 64), (2, 2, 300, 64)))
+    v = rnd(2, 2, 300, 64, dtype=dtype, seed=8)
+    check_window(q, k, v, scale=scale)
+    check_window(q, k, v, window=100, sinks=3, scale=scale)
+    check_window(q[:, :, :1], k, v, scale=scale)
