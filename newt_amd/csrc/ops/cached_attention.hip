@@ -363,7 +363,7 @@ struct Wave {
 #pragma unroll
       for (int j = 1; j < 16; ++j) most = __builtin_fmaxf(most, s[mt][j / 4][j % 4]);
       most = newt::lane_reduce<newt::Max, 48>(most * k_scale);
-      if (__ballot(most > m[mt] + kSlack)) {
+      if (__ballot(most > m[mt] + (CAREFUL ? 0.0f : kSlack))) {
         const float to = __builtin_fmaxf(m[mt], most);
         const float f = m[mt] == -kInf ? 0.0f : __builtin_amdgcn_exp2f(m[mt] - to);
         l[mt] *= f;
@@ -439,17 +439,20 @@ struct Wave {
       tile<true, false>(range, range.tile(i), range.tile(i + kWaves), range.tile(i + 2 * kWaves));
     tile<false, false>(range, range.tile(i), 0, 0);
     // 0 times NaN is NaN: where there is any in a sum or an accumulator, again,
-    // with the NaN among values and scales kept from the rows that do not see them
+    // with the NaN among values and scales kept from the rows that do not see
+    // them; and where scores are beyond kExact
     float check = 0.0f;
+    bool again = false;
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
       check += l[mt] * 0.0f;
+      again |= beyond_exact(m[mt]);
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
         for (int e = 0; e < 4; ++e) check += acc[mt][dt][e] * 0.0f;
     }
-    if (!__ballot(!(check == 0.0f))) return;
+    if (!__ballot(!(check == 0.0f) | again)) return;
     clear();
     for (i = from; i < to; i += kWaves) {
       ask_blocks(range.tile(i), range.hi);

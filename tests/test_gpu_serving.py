@@ -889,3 +889,17 @@ def test_window_large_scores(dtype, scale):
     check_window(q, k, v, scale=scale)
     check_window(q, k, v, window=100, sinks=3, scale=scale)
     check_window(q[:, :, :1], k, v, scale=scale)
+
+
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("scale", [1e4, 1e7, -1e8, 3e9, 1e15, 1e25])
+def test_cached_large_scores(dtype, scale):
+    """As test_window_large_scores, over whole numbers times powers of two."""
+    lens = (300, 1, 64, 2500)
+    cache, table = fill_cache(2, 64, 64, lens, seed=3, outlier=False)
+    g = torch.Generator(device="cuda").manual_seed(7)
+    cache.k.copy_(torch.randint(-3, 4, cache.k.shape, generator=g, device="cuda").to(E4M3))
+    for S in (1, 5):
+        q = torch.randint(-3, 4, (4, 4, S, 64), generator=g, device="cuda").to(dtype)
+        check_cached(q, cache, table, lens, scale=scale)
+        check_cached(q, cache, table, lens, window=100, sinks=3, scale=scale)
