@@ -34,6 +34,11 @@ struct Program {
   static constexpr int STEPS = D / 16;
   static constexpr int DT = D / 32;
   static constexpr int STAGE = 2 * kTile * D;  // numbers of a stage: keys, then values
+  // fp16 weights, and with them their sums and products, are 2^7 times as large,
+  // up to 2^(7 + kSlack): those from 2^-21 of the largest on keep all bits of the
+  // type, and smaller ones are off by 2^-32 of it at most, where without this a
+  // row lost all weights below 2^-25, however many. bf16 has the range by itself.
+  static constexpr float kLift = __is_same(T, bf16) ? 0.0f : 7.0f;
   typedef newt::LdsTile<T, D> KTile;
   typedef newt::LdsTileR<T, D> VTile;
 
@@ -185,8 +190,10 @@ struct Program {
     for (int kh = 0; kh < 2; ++kh)
 #pragma unroll
       for (int e = 0; e < 16; ++e)
-        w[2 * kh + e / 8][e % 8] =
-            (T)__builtin_amdgcn_exp2f(__builtin_fmaf(s[kh][e], to_log2, -ref));
+        w[2 * kh + e / 8][e % 8] = (T)__builtin_amdgcn_exp2f(
+            // maxima beyond kExact would lose the lift to rounding
+            CAREFUL ? (s[kh][e] - ref) + kLift
+                    : __builtin_fmaf(s[kh][e], to_log2, kLift - ref));
     // the sum of the weights as the product takes them, two at a time
 #pragma unroll
     for (int i = 0; i < 4; ++i) l = add(w[i], l);

@@ -903,3 +903,22 @@ def test_cached_large_scores(dtype, scale):
         q = torch.randint(-3, 4, (4, 4, S, 64), generator=g, device="cuda").to(dtype)
         check_cached(q, cache, table, lens, scale=scale)
         check_cached(q, cache, table, lens, window=100, sinks=3, scale=scale)
+
+
+def test_window_small_weights():
+    """fp16: one key that outweighs each of the others by e^18 and comes before
+    them, and 2^16 others whose values alone are not 0. A weight is off by
+    2^-11 of itself, from 2^-21 of the largest on; below by 2^-32 of that."""
+    n, D = 2 ** 16 + 1, 64
+    q, k, v = (torch.zeros(1, 1, m, D, dtype=torch.float16, device="cuda") for m in (1, n, n))
+    q[..., 0] = 1.0
+    k[0, 0, 1:, 0] = -18.0
+    v[0, 0, 1:] = rnd(n - 1, D, dtype=torch.float16, seed=1).abs()
+    # so many sequences that a row's keys are all one program's
+    got = W().window_attention(q.expand(4, 128, 1, D), k.expand(4, 128, n, D),
+                               v.expand(4, 128, n, D), scale=1.0)
+    want, a = orc.attention(q[0], k[0], v[0], [n - 1], scale=1.0)
+    tol = ((2.0 ** -11 + (D + 64) * 64 * 2.0 ** -24) * a + 2.0 ** -11 * want.abs() + 2.0 ** -25
+           + n * 2.0 ** -32 * float(v.max()))
+    assert bool(((got.double() - want).abs() <= tol).all())
+    assert torch.equal(got, got[:1, :1].expand_as(got))
