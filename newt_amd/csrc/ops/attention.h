@@ -7,6 +7,8 @@
 // a program share each key and value tile and a single token still fills G
 // rows.
 #pragma once
+#include <utility>
+
 #include "common.h"
 
 namespace newt_ops {
@@ -161,11 +163,31 @@ join_splits_kernel(const void* workspace, void* out, Rows o, int64_t units, int 
   newt::store_vec<T, 4>(to, t, newt::any_align());
 }
 
+// Whether rows of `dim` numbers in three dimensions share memory, which several
+// programs would write at once: a dimension, from the smallest stride on, has to
+// step over all that those before it reach. Slices, permutations and the like of
+// a tensor without overlaps do.
+inline bool rows_overlap(int dim, int64_t n0, int64_t s0, int64_t n1, int64_t s1, int64_t n2,
+                         int64_t s2) {
+  struct { int64_t n, stride; } d[3] = {{n0, s0}, {n1, s1}, {n2, s2}};
+  for (auto& e : d) e.stride = e.stride < 0 ? -e.stride : e.stride;
+  const auto order = [&](int i, int j) { if (d[j].stride < d[i].stride) std::swap(d[i], d[j]); };
+  order(0, 1);
+  order(1, 2);
+  order(0, 1);
+  double reach = dim;  // what strides of any size cannot exceed
+  for (const auto& e : d) {
+    if (e.n <= 1) continue;
+    if ((double)e.stride < reach) return true;
+    reach += (double)(e.n - 1) * (double)e.stride;
+  }
+  return false;
+}
+
 // What both operators refuse of their queries, outputs and scale; null: nothing.
 template <typename P>
-const char* queries_wrong(const P& p) {
-  if ((p.batch > 1 && p.o_stride_b == 0) || (p.heads > 1 && p.o_stride_h == 0) ||
-      (p.q_len > 1 && p.o_stride_t == 0))
+const char* queries_wrong(const P& p, int head_dim) {
+  if (rows_overlap(head_dim, p.batch, p.o_stride_b, p.heads, p.o_stride_h, p.q_len, p.o_stride_t))
     return "rows of out overlap";
   // scores and their exponents stay finite for ordinary queries and keys
   if (!(__builtin_fabsf(p.scale) < 0x1p100f)) return "scale has to be finite, below 2^100";

@@ -762,7 +762,7 @@ const char* wrong(const newt_cached_attention_params& p) {
   if (p.q_len * p.heads >= kLimit || p.table_width * p.cache.block_size >= kLimit ||
       p.window >= kLimit || p.sinks >= kLimit)
     return "sizes stay below 2^30";
-  return queries_wrong(p);
+  return queries_wrong(p, p.cache.head_dim);
 }
 
 }  // namespace

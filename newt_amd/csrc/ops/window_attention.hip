@@ -439,7 +439,7 @@ const char* wrong(const newt_window_attention_params& p) {
   if (p.q_len * p.heads >= kLimit || p.kv_len >= kLimit || p.window >= kLimit || p.sinks >= kLimit)
     return "sizes stay below 2^30";
   if (p.k_stride_t < 0 || p.v_stride_t < 0) return "negative stride";
-  return queries_wrong(p);
+  return queries_wrong(p, p.head_dim);
 }
 
 }  // namespace

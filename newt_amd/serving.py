@@ -403,7 +403,8 @@ def cached_attention(q, cache, block_table, lens, window=None, sinks=0, scale=No
     negative) gets zeros. Tokens behind the table, and those of blocks that are
     not in the cache, are not seen; blocks that hold no visible token are not
     read, and their table entries may be anything. scale (finite) defaults to
-    head_dim^-0.5. Rows of an `out` given must not overlap each other."""
+    head_dim^-0.5. Rows of an `out` given must not overlap each other, not
+    even in part: each of its strides steps over what the smaller ones reach."""
     r = _fast("cached_attention", q, cache, block_table, lens, window, sinks, scale, out)
     if r is not None:
         return r

@@ -354,3 +354,36 @@ def test_attention_refuses_overlapping_rows_and_scales():
         for scale in (float("inf"), -float("inf"), float("nan"), 2.0 ** 100):
             assert call(scale=scale) == 10002
             assert b"scale" in L.newt_ops_last_error()
+
+
+def test_attention_refuses_rows_that_overlap_in_part():
+    """Rows of an output that share some of their memory, in any order of the
+    dimensions; what slices and permutations of a tensor give is taken."""
+    L = serving.lib()
+    P = 4096
+    cache = [P, P, P, P, 4, 2, 16, 64, 0]
+
+    def cached(o, batch=2, q_len=2, heads=4):
+        # without a table: the check of the strides comes before that of null tensors
+        return L.newt_cached_attention(serving._CACHED.pack(
+            *cache, 0, P, P, P, 0, batch, q_len, 1, 1, 512, 128, 64, *o, 0, 0, 1.0, heads, 2, 0),
+            None)
+
+    def window(o, batch=2, q_len=2, heads=4):
+        return L.newt_window_attention(serving._WINDOW.pack(
+            0, P, P, P, 0, 0, batch, q_len, 1, *[64] * 9, *o, 0, 0, 1.0, heads, 2, 64, 2, 0), None)
+
+    for call in (cached, window):
+        for o in ((512, 128, 63), (512, 127, 64), (511, 128, 64), (512, 128, 1), (64, 128, 64),
+                  (512, 64, 255), (64, 96, 512)):
+            assert call(o) == 10002
+            assert b"overlap" in L.newt_ops_last_error(), o
+        for o in ((512, 128, 64), (512, 64, 256), (64, 128, 512), (64, 256, 128), (128, 512, 64),
+                  (1000, 200, 70)):
+            assert call(o) == 10002
+            assert b"null tensor" in L.newt_ops_last_error(), o
+        # dimensions of one have no stride
+        assert call((0, 0, 64), batch=1, heads=2, q_len=2) == 10002
+        assert b"overlap" in L.newt_ops_last_error()
+        assert call((0, 64, 0), batch=1, q_len=1) == 10002
+        assert b"null tensor" in L.newt_ops_last_error()
