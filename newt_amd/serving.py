@@ -414,7 +414,7 @@ def cached_attention(q, cache, block_table, lens, window=None, sinks=0, scale=No
     B, H, S, D = q.shape
     fields, heads, size, dim, width, table_stride = _pages("cached_attention", device, cache,
                                                            block_table, B)
-    if D != dim or H == 0 or H % heads:
+    if D != dim or heads == 0 or H == 0 or H % heads:
         raise ValueError(f"cached_attention: {H} heads of {D} dims over a cache of {heads} of {dim}")
     if S * H >= 2 ** 30:
         raise ValueError("cached_attention: too many queries")

@@ -387,3 +387,12 @@ def test_attention_refuses_rows_that_overlap_in_part():
         assert b"overlap" in L.newt_ops_last_error()
         assert call((0, 64, 0), batch=1, q_len=1) == 10002
         assert b"null tensor" in L.newt_ops_last_error()
+
+
+def test_cache_without_heads(calls):
+    """A ValueError, as for other heads that do not go together."""
+    q, table = torch.zeros(2, 4, 3, 64, dtype=BF16), torch.zeros(2, 1, dtype=torch.int32)
+    cache = workloads.KVCache(*(c[:, :0].contiguous() for c in workloads.kv_cache(
+        3, 2, 64, device="cpu")))
+    lens = torch.zeros(2, dtype=torch.int32)
+    refused(ValueError, "heads", workloads.cached_attention, q, cache, table, lens)
