@@ -115,12 +115,13 @@ def _call(entry, what, params, device):
         raise (ValueError if status >= 10000 else _hip.HIPError)(f"{what}: {detail}")
 
 
-def _tensors(what, device, **tensors):
+def _tensors(what, device, optional=None, **tensors):
+    """All are tensors on the current GPU; `optional` ones may be None."""
+    tensors.update((name, t) for name, t in (optional or {}).items() if t is not None)
     for name, t in tensors.items():
-        if t is None:
-            continue
         if not isinstance(t, torch.Tensor):
             raise TypeError(f"{what}: {name} must be a tensor")
+    for name, t in tensors.items():
         if not t.is_cuda or t.device.index != device:
             raise TypeError(f"{what}: {name} must be on the current GPU")
 
@@ -163,7 +164,7 @@ def rmsnorm(x, w, eps=1e-6, residual=None, out_dtype=None, group=None, out=None,
     if r is not None:
         return r
     device = _Dev.device()
-    _tensors("rmsnorm", device, x=x, w=w, residual=residual, out=out, hidden=hidden)
+    _tensors("rmsnorm", device, {"residual": residual, "out": out, "hidden": hidden}, x=x, w=w)
     if x.dim() != 2 or x.shape[1] == 0:
         raise ValueError(f"rmsnorm: x has shape {tuple(x.shape)}, not [M, N]")
     dtype = x.dtype
@@ -292,10 +293,18 @@ def kv_cache(blocks, kv_heads, head_dim, block_size=64, device=None):
                    zeros(blocks, kv_heads, head_dim, block_size), *scales)
 
 
-def _pages(what, device, cache, block_table, batch):
+def _cache_tensors(what, cache, block_table):
+    """What _tensors looks at of a cache and its table."""
+    if not isinstance(cache, (tuple, list)):
+        raise TypeError(f"{what}: cache must be a KVCache")
+    if len(cache) != 4:
+        raise ValueError(f"{what}: a cache has 4 tensors, not {len(cache)}")
+    return dict(zip(("k_cache", "v_cache", "k_scale", "v_scale"), cache), block_table=block_table)
+
+
+def _pages(what, cache, block_table, batch):
     """The checked cache as packed fields, the table's width and stride."""
     k, v, ks, vs = cache
-    _tensors(what, device, k_cache=k, v_cache=v, k_scale=ks, v_scale=vs, block_table=block_table)
     if k.dim() != 4:
         raise ValueError(f"{what}: the cache's keys have shape {tuple(k.shape)}, not [blocks, "
                          f"kv_heads, block_size, head_dim]")
@@ -350,12 +359,12 @@ def kv_append(cache, k, v, block_table, start, count=None):
     if _fast("kv_append", cache, k, v, block_table, start, count):
         return
     device = _Dev.device()
-    _tensors("kv_append", device, k=k, v=v, start=start, count=count)
+    _tensors("kv_append", device, {"count": count}, k=k, v=v, start=start,
+             **_cache_tensors("kv_append", cache, block_table))
     if k.dim() != 4:
         raise ValueError(f"kv_append: k has shape {tuple(k.shape)}, not [B, kv_heads, S, head_dim]")
     B, _, S, _ = k.shape
-    fields, heads, size, dim, width, table_stride = _pages("kv_append", device, cache, block_table,
-                                                           B)
+    fields, heads, size, dim, width, table_stride = _pages("kv_append", cache, block_table, B)
     if k.dtype not in _DTYPE or k.dtype == E4M3:
         raise TypeError(f"kv_append: k is {k.dtype}")
     _shape("kv_append", "k", k, (B, heads, S, dim))
@@ -409,11 +418,12 @@ def cached_attention(q, cache, block_table, lens, window=None, sinks=0, scale=No
     if r is not None:
         return r
     device = _Dev.device()
-    _tensors("cached_attention", device, q=q, lens=lens, out=out)
+    _tensors("cached_attention", device, {"out": out}, q=q, lens=lens,
+             **_cache_tensors("cached_attention", cache, block_table))
     out, window, scale = _queries("cached_attention", q, out, window, sinks, scale)
     B, H, S, D = q.shape
-    fields, heads, size, dim, width, table_stride = _pages("cached_attention", device, cache,
-                                                           block_table, B)
+    fields, heads, size, dim, width, table_stride = _pages("cached_attention", cache, block_table,
+                                                           B)
     if D != dim or heads == 0 or H == 0 or H % heads:
         raise ValueError(f"cached_attention: {H} heads of {D} dims over a cache of {heads} of {dim}")
     if S * H >= 2 ** 30:
@@ -454,7 +464,7 @@ def window_attention(q, k, v, window=None, sinks=0, scale=None, q_start=None, ou
     if r is not None:
         return r
     device = _Dev.device()
-    _tensors("window_attention", device, q=q, k=k, v=v, q_start=q_start, out=out)
+    _tensors("window_attention", device, {"q_start": q_start, "out": out}, q=q, k=k, v=v)
     out, window, scale = _queries("window_attention", q, out, window, sinks, scale)
     B, H, S, D = q.shape
     if D not in _HEAD_DIMS:

@@ -396,3 +396,38 @@ def test_cache_without_heads(calls):
         3, 2, 64, device="cpu")))
     lens = torch.zeros(2, dtype=torch.int32)
     refused(ValueError, "heads", workloads.cached_attention, q, cache, table, lens)
+
+
+def test_required_tensors(monkeypatch):
+    """None and other things in the place of a tensor that a call needs."""
+    monkeypatch.setattr(serving._Dev, "device", classmethod(lambda cls: 0))
+    monkeypatch.setattr(serving._Dev, "stream", staticmethod(lambda device: 0))
+    x, t = torch.zeros(2, 64), torch.zeros(2, dtype=torch.int64)
+    q, lens = torch.zeros(2, 2, 3, 64, dtype=BF16), torch.zeros(2, dtype=torch.int32)
+    cache, table = workloads.kv_cache(2, 2, 64, device="cpu"), lens.view(2, 1)
+    calls = {workloads.rmsnorm: {"x": x, "w": x[0]},
+             workloads.token_logprobs: {"logits": x, "tokens": t},
+             workloads.kv_append: {"cache": cache, "k": q, "v": q, "block_table": table,
+                                   "start": lens},
+             workloads.cached_attention: {"q": q, "cache": cache, "block_table": table,
+                                          "lens": lens},
+             workloads.window_attention: {"q": q, "k": q, "v": q}}
+    for f, args in calls.items():
+        refused(TypeError, "current GPU", f, **args)
+        for name in args:
+            if name == "cache":
+                for wrong in (None, 3):
+                    refused(TypeError, None, f, **{**args, name: wrong})
+                refused(ValueError, None, f, **{**args, name: cache[:3]})
+                for field in cache._fields:
+                    refused(TypeError, "must be a tensor", f,
+                            **{**args, name: cache._replace(**{field: None})})
+                continue
+            for wrong in (None, 1.0, [1, 2]):
+                refused(TypeError, "must be a tensor", f, **{**args, name: wrong})
+    for f, names in ((workloads.rmsnorm, ("residual", "out", "hidden")),
+                     (workloads.kv_append, ("count",)), (workloads.cached_attention, ("out",)),
+                     (workloads.window_attention, ("q_start", "out"))):
+        for name in names:
+            refused(TypeError, "current GPU", f, **{**calls[f], name: None})
+            refused(TypeError, "must be a tensor", f, **{**calls[f], name: 1.0})
