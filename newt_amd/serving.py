@@ -23,6 +23,7 @@ One step of a decoder layer over the 8-bit cache:
 
 import ctypes
 import functools
+import math
 import os
 import struct
 from typing import NamedTuple
@@ -140,6 +141,14 @@ def _whole(what, name, value, least):
         raise ValueError(f"{what}: {name}={value} is out of range")
 
 
+def _fp32(value):
+    """A number as fp32 holds it, infinite beyond its range, as a cast in C++."""
+    try:
+        return ctypes.c_float(float(value)).value
+    except OverflowError:  # an int that no double holds
+        return math.inf if value > 0 else -math.inf
+
+
 def _ptr(t):
     return 0 if t is None else t.data_ptr()
 
@@ -206,8 +215,8 @@ def rmsnorm(x, w, eps=1e-6, residual=None, out_dtype=None, group=None, out=None,
         raise ValueError("rmsnorm: rows of an output overlap")
     _call(lib().newt_rmsnorm, "rmsnorm", _RMSNORM.pack(
         x.data_ptr(), _ptr(residual), w.data_ptr(), out.data_ptr(), _ptr(hidden), _ptr(scale),
-        M, N, sx[0], sr[0], so[0], sh[0], eps, _DTYPE[dtype], _DTYPE[w.dtype], _DTYPE[out_dtype],
-        group or 0, 0), device)
+        M, N, sx[0], sr[0], so[0], sh[0], _fp32(eps), _DTYPE[dtype], _DTYPE[w.dtype],
+        _DTYPE[out_dtype], group or 0, 0), device)
     return out, scale, hidden
 
 
@@ -397,7 +406,7 @@ def _queries(what, q, out, window, sinks, scale):
         _shape(what, "out", out, q.shape, q.dtype)
     if q.stride(3) != 1 or out.stride(3) != 1:
         raise ValueError(f"{what}: q and out need unit stride along head_dim")
-    return out, window or 0, q.shape[3] ** -0.5 if scale is None else float(scale)
+    return out, window or 0, q.shape[3] ** -0.5 if scale is None else _fp32(scale)
 
 
 def cached_attention(q, cache, block_table, lens, window=None, sinks=0, scale=None, out=None):

@@ -431,3 +431,33 @@ def test_required_tensors(monkeypatch):
         for name in names:
             refused(TypeError, "current GPU", f, **{**calls[f], name: None})
             refused(TypeError, "must be a tensor", f, **{**calls[f], name: 1.0})
+
+
+LAUNCH = serving._call  # before a test takes its place
+
+
+def test_numbers_beyond_fp32(calls, monkeypatch):
+    """A scale that fp32 does not hold is refused as one that is not finite; an
+    eps that it does not hold is infinite, as in the calls made in C++. What is
+    no number is a TypeError or ValueError."""
+    launched = []
+    monkeypatch.setattr(serving, "_call", lambda entry, what, params, device:
+                        launched.append(params) if what == "rmsnorm" else
+                        LAUNCH(entry, what, params, device))
+    monkeypatch.setattr(serving._Dev, "stream", staticmethod(lambda device: 0))
+    q, lens = torch.zeros(2, 2, 3, 64, dtype=BF16), torch.zeros(2, dtype=torch.int32)
+    cache, table = workloads.kv_cache(2, 2, 64, device="cpu"), lens.view(2, 1)
+    for scale in (1e39, -1e300, float("inf"), float("nan"), 10 ** 40):
+        refused(ValueError, "scale", workloads.cached_attention, q, cache, table, lens, scale=scale)
+        refused(ValueError, "scale", workloads.window_attention, q, q, q, scale=scale)
+    for wrong in ("a", [1.0]):
+        for f, args in ((workloads.window_attention, (q, q, q)),
+                        (workloads.cached_attention, (q, cache, table, lens))):
+            with pytest.raises((TypeError, ValueError)):
+                f(*args, scale=wrong)
+        with pytest.raises((TypeError, ValueError)):
+            workloads.rmsnorm(torch.zeros(2, 64), torch.zeros(64), eps=wrong)
+    with pytest.raises(TypeError):
+        workloads.rmsnorm(torch.zeros(2, 64), torch.zeros(64), eps=None)
+    workloads.rmsnorm(torch.zeros(2, 64), torch.zeros(64), eps=1e39)
+    assert serving._RMSNORM.unpack(launched[0])[12] == float("inf")
