@@ -922,3 +922,59 @@ def test_window_small_weights():
            + n * 2.0 ** -32 * float(v.max()))
     assert bool(((got.double() - want).abs() <= tol).all())
     assert torch.equal(got, got[:1, :1].expand_as(got))
+
+
+def test_ordinary_calls_go_through_cpp(monkeypatch):
+    """The C++ extension takes every operator's ordinary call, and leaves wrong
+    shapes, types, strides and numbers to Python."""
+    from newt_amd import serving
+    fast, results = serving._fast, []
+
+    def recorded(*args):
+        results.append(fast(*args))
+        return results[-1]
+
+    monkeypatch.setattr(serving, "_fast", recorded)
+    bf16 = torch.bfloat16
+    x, w = rnd(7, 512, dtype=bf16, seed=1), rnd(512, dtype=bf16, seed=2)
+    q, k = rnd(2, 4, 5, 64, dtype=bf16, seed=3), rnd(2, 2, 90, 64, dtype=bf16, seed=4)
+    logits, tokens = rnd(3, 3000, dtype=bf16, seed=5), torch.arange(3, device="cuda")
+    cache = W().kv_cache(6, 2, 64, block_size=32)
+    table = torch.arange(6, device="cuda").to(torch.int32).view(2, 3)
+    calls = {"rmsnorm": (x, w, 1e-6, x, -1, None, None, None),
+             "token_logprobs": (logits, tokens, 5, 1.0),
+             "kv_append": (cache, k, k, table, ints(0, 3), ints(90, 80)),
+             "cached_attention": (q, cache, table, ints(90, 83), None, 0, None, None),
+             "window_attention": (q, k, k, 40, 2, 0.125, ints(80, 20), None)}
+    W().rmsnorm(x, w, residual=x)
+    W().rmsnorm(x, w, out_dtype=E4M3, group=64, out=torch.empty_like(x, dtype=E4M3))
+    W().token_logprobs(logits, tokens, top=5, temperature=0.7)
+    W().kv_append(*calls["kv_append"])
+    W().cached_attention(q, cache, table, ints(90, 83), window=30, sinks=2, out=q.clone())
+    W().window_attention(q, k, k)
+    assert len(results) == 6 and all(r is not None for r in results)
+    wrong = {"rmsnorm": {0: (x[0], x.double(), x.t(), x[:, ::2], None), 1: (w[1:], w.half(), None),
+                         2: ("a",), 3: (x[1:], x.float()), 4: (0, -2), 5: (64, 32.0),
+                         6: (x[1:], x.float(), x[:1].expand(7, 512)), 7: (x[1:], x.float())},
+             "token_logprobs": {0: (logits[0], logits.double(), logits[:, ::2], None),
+                                1: (tokens[1:], tokens.int(), None), 2: (65, -1, 2.0),
+                                3: (0.0, -1.0, float("nan"), None)},
+             "kv_append": {0: (cache[:3], tuple(cache[:2]) + (cache[2][:3], cache[3]),
+                               (cache[1], cache[0], *cache[2:]), None),
+                           1: (k[0], k[:, :1], k.half(), None), 2: (k[:, :, 1:], k.half(), None),
+                           3: (table[:1], table.long(), None), 4: (ints(0), tokens[:2], None),
+                           5: (ints(0), tokens[:2])},
+             "cached_attention": {0: (q[0], q[:, :3], q.float(), q.half()[..., ::2], None),
+                                  1: (cache[:3], None), 2: (table[:1], table.long(), None),
+                                  3: (ints(0), tokens[:2], None), 4: (0, 2.0), 5: (-1, 3),
+                                  6: ("a", float("inf")),
+                                  7: (q[:, :1], q.half(), q[:, :1].expand(2, 4, 5, 64))},
+             "window_attention": {0: (q[0], q[:, :3], q.float(), None), 1: (k[:1], k.half(), None),
+                                  2: (k[:, :, 1:], k.half(), None), 3: (0, 2.0), 4: (-1, None),
+                                  5: ("a", float("nan")), 6: (ints(0), tokens[:2]),
+                                  7: (q[:, :1], q.half(), q[:, :1].expand(2, 4, 5, 64))}}
+    for name, args in calls.items():
+        assert fast(name, *args) is not None
+        for i, values in wrong[name].items():
+            for value in values:
+                assert fast(name, *args[:i], value, *args[i + 1:]) is None, (name, i)
