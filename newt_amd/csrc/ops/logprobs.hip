@@ -112,12 +112,16 @@ __device__ __forceinline__ void insert(Entry& e, const Entry& c, int lane) {
   if (lane == place) e = c;
 }
 
-// d = (x - m) c by one fma where the product m c is well inside fp32's range:
-// it is rounded, by the same amount in all that is taken relative to this m, so
-// that the rounding cancels in every result. Rows of nothing but the types'
-// lowest numbers take the longer way.
+// d = (x - m) c by one fma where the product m c is rounded by 2^-5 at most: by
+// the same amount in all that is taken relative to this m, so that the rounding
+// cancels in every result. Larger ones, whose rounding would drown the exponents
+// (tiny temperatures, rows of the types' lowest numbers), take the longer way.
 __device__ __forceinline__ bool near_zero(float m, float c) {
-  return __builtin_fabsf(m * c) < 1e38f;
+  return __builtin_fabsf(m * c) < 1048576.0f;  // 2^20
+}
+// What m c is rounded by in distances to m.
+__device__ __forceinline__ float rounding(float m, float c) {
+  return near_zero(m, c) ? __builtin_fmaf(m, c, -(m * c)) : 0.0f;
 }
 __device__ __forceinline__ float distance(float x, float m, float c) {
   return near_zero(m, c) ? __builtin_fmaf(x, c, -(m * c)) : (x - m) * c;
@@ -130,13 +134,8 @@ struct Sums {
   // The same relative to the maximum `to` >= m.
   __device__ __forceinline__ void rescale(float to, float c) {
     if (!(to > m)) return;
-    float d;
-    {
-      // both products rounded, as those that S and U are relative to: an fma of
-      // one would leave the other's rounding in them, 2^-25 |m c| each time
-#pragma clang fp contract(off)
-      d = near_zero(to, c) ? m * c - to * c : (m - to) * c;
-    }
+    // S and U are relative to the rounded m c, what comes to the rounded `to` c
+    const float d = (m - to) * c + (rounding(to, c) - rounding(m, c));
     const float f = __builtin_amdgcn_exp2f(d);
     if (f == 0.0f && S == S) {
       S = U = 0.0f;

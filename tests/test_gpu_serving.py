@@ -978,3 +978,39 @@ def test_ordinary_calls_go_through_cpp(monkeypatch):
         for i, values in wrong[name].items():
             for value in values:
                 assert fast(name, *args[:i], value, *args[i + 1:]) is None, (name, i)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("V", [4000, 70001])
+@pytest.mark.parametrize("temperature", [1e-6, 3e-9, 1e-20, 2.0 ** -99])
+def test_logprobs_tiny_temperatures(dtype, V, temperature):
+    """Logits over the temperature far above 2^24: a row's largest logits share
+    all of its probability. They are whole numbers, so that fp32 tells them
+    apart at any temperature."""
+    g = torch.Generator(device="cuda").manual_seed(V)
+    x = torch.randint(-40, 40, (6, V), generator=g, device="cuda").to(dtype)
+    x[3:] -= 100
+    tokens = x.float().argmax(-1)
+    check_logprobs(x, tokens, 5, temperature=temperature)
+    logp, entropy, top_logp, _ = W().token_logprobs(x, tokens, top=5, temperature=temperature)
+    n = (x == x.amax(-1, keepdim=True)).sum(-1).double()
+    # what is left of the sum's and the logarithm's own roundings
+    assert bool(((logp.double() + n.log()).abs() <= (V / 64 + 16) * 2.0 ** -24 * 10).all())
+    assert bool(((entropy.double() - n.log()).abs() <= (V / 64 + 16) * 2.0 ** -24 * 10).all())
+    assert torch.equal(logp, top_logp[:, 0])
+
+
+@pytest.mark.parametrize("V", [4000, 70001])
+def test_logprobs_huge_logits(V):
+    """fp32 logits around 1e10, whose steps are 1024, and ones whose maximum
+    grows through all sizes from far below 2^20 to far above it."""
+    g = torch.Generator(device="cuda").manual_seed(V)
+    x = 1024.0 * torch.randint(4, (4, V), generator=g, device="cuda")
+    tokens = torch.full((4,), V // 2, device="cuda")
+    for offset in (1e10, -1e10, 3e13):
+        check_logprobs(x * (offset / 1e10 if offset > 1e12 else 1.0) + offset, tokens, 5)
+    noise = torch.randn(4, V, generator=g, device="cuda")
+    for middle in (2 ** 20 / 1.4426950408889634, -2 ** 20 / 1.4426950408889634):
+        for ramp in (torch.linspace(-20, 20, V, device="cuda"),
+                     torch.linspace(20, -20, V, device="cuda")):
+            check_logprobs(middle + ramp + noise, tokens, 5)
