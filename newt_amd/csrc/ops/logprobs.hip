@@ -127,6 +127,13 @@ __device__ __forceinline__ float distance(float x, float m, float c) {
   return near_zero(m, c) ? __builtin_fmaf(x, c, -(m * c)) : (x - m) * c;
 }
 
+// The log probability but for the sum's share: the distance as a natural
+// logarithm. Logits near the lowest number fp32 holds leave it on the way there.
+__device__ __forceinline__ float natural(float x, float m, float c, float inv_temperature) {
+  const float d = distance(x, m, c);
+  return d == -kInf ? (x - m) * inv_temperature : d * kLn2;
+}
+
 // The sums over what a lane, a wave or a split has seen.
 struct Sums {
   float m, S, U;
@@ -166,14 +173,15 @@ __device__ __forceinline__ void finish(const newt_logprobs_params& p, int64_t ro
     float logp = __builtin_nanf("");
     if (token == -1) logp = 0.0f;
     else if (token >= 0 && token < p.vocab)
-      logp = distance(newt::to_f32(((const T*)p.logits)[row * p.stride + token]), s.m, c) * kLn2 - lse;
+      logp = natural(newt::to_f32(((const T*)p.logits)[row * p.stride + token]), s.m, c,
+                     p.inv_temperature) - lse;
     p.logp[row] = logp;
     p.entropy[row] = lse - kLn2 * (s.U / s.S);
   }
   if (lane < p.top) {
     const bool none = e.id == kNone;
     p.top_logp[row * p.top + lane] =
-        none ? __builtin_nanf("") : distance(e.value, s.m, c) * kLn2 - lse;
+        none ? __builtin_nanf("") : natural(e.value, s.m, c, p.inv_temperature) - lse;
     p.top_ids[row * p.top + lane] = none ? -1 : e.id;
   }
 }

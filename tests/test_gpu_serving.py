@@ -1014,3 +1014,18 @@ def test_logprobs_huge_logits(V):
         for ramp in (torch.linspace(-20, 20, V, device="cuda"),
                      torch.linspace(20, -20, V, device="cuda")):
             check_logprobs(middle + ramp + noise, tokens, 5)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("V", [50, 20001])
+def test_logprobs_of_lowest_values(dtype, V):
+    """Tokens masked with the type's lowest value have log probabilities of that
+    size, not of -inf, as themselves and as alternatives."""
+    x = rnd(4, V, dtype=dtype, seed=V)
+    x[0, 3:] = torch.finfo(dtype).min
+    x[1, ::2] = torch.finfo(dtype).min
+    x[2, :-1] = torch.finfo(dtype).min
+    x[3, 1:] = float("-inf")
+    tokens = ints(V - 1, 0, 0, 1, dtype=torch.int64)
+    check_logprobs(x, tokens, 8)
+    check_logprobs(x, tokens, 8, temperature=2.0)
