@@ -1029,3 +1029,22 @@ def test_logprobs_of_lowest_values(dtype, V):
     tokens = ints(V - 1, 0, 0, 1, dtype=torch.int64)
     check_logprobs(x, tokens, 8)
     check_logprobs(x, tokens, 8, temperature=2.0)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("N", [72, 4097, 40000])
+def test_rmsnorm_in_place(dtype, N):
+    """y over x or over the residual, with and without the sum beside it."""
+    x, r = rnd(5, N, dtype=dtype, seed=N), rnd(5, N, dtype=dtype, seed=N + 1)
+    w = rnd(N, dtype=dtype, seed=N + 2)
+    y, _, h = W().rmsnorm(x, w, residual=r)
+    for i in (0, 1):
+        both = [x.clone(), r.clone()]
+        out, _, hidden = W().rmsnorm(both[0], w, residual=both[1], out=both[i])
+        assert out is both[i] or out.data_ptr() == both[i].data_ptr()
+        assert torch.equal(out, y) and torch.equal(hidden, h)
+        both = [x.clone(), r.clone()]
+        out, _, hidden = W().rmsnorm(both[0], w, residual=both[1], out=both[i], hidden=both[1 - i])
+        assert torch.equal(both[i], y) and torch.equal(both[1 - i], h)
+    y = W().rmsnorm(x, w)[0]
+    assert torch.equal(W().rmsnorm(x, w, out=x)[0], y) and torch.equal(x, y)
