@@ -77,7 +77,8 @@ size_t newt_token_logprobs_workspace(int64_t rows, int64_t vocab, int32_t top, i
 /* The 8-bit cache: `blocks` blocks of `block_size` tokens of kv_heads heads.
  *   k [blocks, kv_heads, block_size, head_dim], v [blocks, kv_heads, head_dim,
  *   block_size] E4M3, k_scale and v_scale [blocks, kv_heads] fp32, all
- *   contiguous; a value is its byte's times its block's and head's scale. */
+ *   contiguous; a value is its byte's times its block's and head's scale, which
+ *   is not negative. */
 typedef struct {
   void* k;
   void* v;
@@ -87,7 +88,8 @@ typedef struct {
   int32_t kv_heads, block_size, head_dim, reserved;
 } newt_kv_cache;
 
-/* Writes count[b] new tokens of each sequence to positions start[b] on. */
+/* Writes count[b] new tokens of each sequence to positions start[b] on. No block
+ * may be written at two places by one call. */
 typedef struct {
   newt_kv_cache cache;
   const void* k;            /* [batch, kv_heads, tokens, head_dim] of dtype */
@@ -106,7 +108,7 @@ int newt_kv_append(const newt_kv_append_params* p, void* stream);
 typedef struct {
   newt_kv_cache cache;
   const void* q;            /* [batch, heads, q_len, head_dim] of dtype */
-  void* out;                /* as q */
+  void* out;                /* as q; rows that overlap, in part too, are refused */
   const int32_t* table;     /* [batch, table_width] block ids */
   const int32_t* lens;      /* [batch] tokens of each sequence, q's among them */
   void* workspace;          /* newt_cached_attention_workspace() bytes, or NULL if that is 0 */

@@ -5,8 +5,8 @@
 // result, or None for anything that is not plainly right: another kind of
 // argument, device, dtype, shape or stride than the kernels take. The Python
 // function then goes through its own checks, which say what is wrong. So this
-// file only has to be strict, and a call costs ~2 us of host time here where
-// the checks and allocations in Python take 5 to 12.
+// file only has to be strict. A call takes 4.4 to 6.0 us of host time with its
+// launch and outputs this way, 10.7 to 13.2 through Python.
 #include <Python.h>
 #include <ATen/ATen.h>
 #include <torch/csrc/autograd/python_variable.h>

@@ -14,10 +14,13 @@
 // e4m3 numbers are exact in bf16 and fp16. The blocks' scales multiply scores
 // and weights in fp32; weights times scales are taken to bf16, whose range
 // holds any scale, and where the queries are fp16 the rest of each weight goes
-// through a second product, for a result as exact as fp16 asks for.
+// through a second product, for a result as exact as fp16 asks for (0.00021 from
+// 64 bits). For bf16 queries a weight rounded by 2^-9 adds no more than the
+// output's own rounding (0.0022 for 0.0016); there the second product would take
+// the batch below from 122.3 to 123.7 us and the single sequence from 14.1 to 14.5.
 // HBM bounds large batches: the visible blocks are read once per KV head. bf16, 64
-// sequences of up to 8192 tokens, 32 heads of 128 over 8: 119.5 us (5.7 TB/s), 5 of
-// them the join. Small ones wait for memory: 1 sequence of 8191 tokens 13.5 us.
+// sequences of up to 8192 tokens, 32 heads of 128 over 8: 122 us (5.6 TB/s), 5 of
+// them the join. Small ones wait for memory: 1 sequence of 8191 tokens 14 us.
 #include "attention.h"
 
 namespace newt_ops {
@@ -72,7 +75,14 @@ constexpr int occupancy(int D, int MT) { return D * MT <= 128 ? 2 : 1; }
 //     end in each unit that a run touches;
 //   - else each takes an even part of one unit, units in as many parts as their
 //     lengths ask for.
-// With `shares` 0 each program takes a unit.
+// With `shares` 0 each program takes a unit. Runs / parts, us, for 8 heads of 128
+// (u: lengths from a quarter on), by the tiles of an even share:
+//   9: 8 sequences of 8192 u 24.4 / 23.6, 2 of 65536 u 26.7 / 24.0;
+//   16: 1 of 65536 33.6 / 34.1, 8 of 8192 30.6 / 35.8;
+//   18: 16 of 8192 u 37.0 / 43.4, 32 of 4096 u 36.5 / 41.3;
+//   32: 8 of 16384 51.0 / 60.7, 16 of 8192 50.8 / 51.2, 32 of 4096 49.6 / 49.6;
+//   38: 16 of 16384 u 62.6 / 89.9; 60: 48 of 8192 u 89.4 / 130.
+// So runs are the better ones from about 12 on; kLong is above that.
 constexpr int kLong = 24;
 
 struct Deal {
@@ -698,7 +708,16 @@ struct Launch {
 };
 
 // The shape of a launch, from sizes that the host knows: the table's width
-// bounds the lengths.
+// bounds the lengths. A program a unit (first) or tiles dealt out by the lengths
+// (second; * what the rule takes), us, 32 heads of 128 over 8, one token:
+//   1 sequence of 256, 512, 768, 1024 tokens: 5.6* 7.9, 7.5* 10.5, 9.4 12.2*, 12.7
+//   12.7*; 24 of them: 6.9* 9.1, 9.7* 12.1, 12.3 14.9*, 14.9 17.4*;
+//   32 of 1024 and 1536: 15.7* 18.3, 20.6 23.1*; 128: 47.8* 52.2, 67.7 72.3*;
+//   64 of any length up to 1024 and 2048: 21.6* 48.8, 34.6 57.7*;
+//   256 of 2048 and of up to 2048: 172 184*, 103 156*;
+//   512 of 2048 and of up to 2048: 339* 365, 194* 265;
+//   1, 8, 64 of 8192: 64 14*, 67 34*, 170 173*; 64 of 2048 to 8192: 137 117*.
+// Dealing out pays for few units and long ones; the rule does it sooner than that.
 Launch launch_of(const newt_cached_attention_params& p) {
   Launch r;
   const int64_t rows = p.q_len * (p.heads / p.cache.kv_heads);

@@ -9,8 +9,8 @@
 // maximum grew, rescales S and U. The list begins with the sorted largest
 // logits of each lane in the first four chunks; after that n logits in no order
 // make about top * ln(n / 2048) insertions. Lists are joined by bitonic merges.
-// bf16 2048 x 100003, two sets in turn: 87 us (4.7 TB/s) without alternatives,
-// 95 with 5, 125 with 20; reading alone would take 58. 1 x 128000: 8 us without,
+// bf16 2048 x 100003, two sets in turn: 89 us (4.6 TB/s) without alternatives,
+// 96 with 5, 125 with 20; reading alone would take 58. 1 x 128000: 8 us without,
 // 15 with 20, of them 5 in the second kernel.
 #include "common.h"
 

@@ -6,9 +6,11 @@
 // HBM bounds it (each input read once, each output written once), so a row is
 // held in registers between the sum of squares and the output, and every
 // access is 16 bytes a lane at whatever alignment the row has. bf16 4096 x 8192
-// with a residual, three sets of inputs in turn: 44 us (6.1 TB/s) to bf16, 41
-// (5.7) to e4m3 with a scale a row, 42 with one for each 128 columns; a copy
-// reaches 5.75 TB/s over 4.3 GB and 7.1 over 268 MB.
+// with a residual, three sets of inputs in turn: 44 us (6.1 TB/s) to bf16, 40
+// (5.8) to e4m3 with a scale a row, 42 (5.6) with one for each 128 columns; a
+// copy reaches 5.77 TB/s over 4.3 GB and 7.1 over 268 MB.
+// Squares are summed in fp32 as they are: a row of numbers around 1e19 has an
+// infinite sum, and its y is 0.
 #include "common.h"
 
 namespace newt_ops {

@@ -12,9 +12,18 @@
 // times an infinity or NaN is NaN, so a program whose accumulators end up not
 // finite runs again and keeps such values from the rows that do not see them;
 // as does one with scores beyond kExact.
-// bf16 4 x 32 x 4096 x 128 in a window of 1024: 313 us, 772 TFLOP/s of visible
+// The weights go to the product in the queries' type, as the matrix unit takes
+// them; their sum is that of the rounded ones, so that values that are all alike
+// come out as they are. That is off by 2^-9 (bf16) or 2^-12 (fp16) of a weight on
+// average, beside the output's own rounding, which is as large: against 64 bits
+// 0.0021 where rounding the output alone gives 0.0016 (fp16 0.00029 and 0.00021).
+// The rest of each weight in a second product, as cached_attention has it for
+// fp16, would make half as many products again of the unit that is busiest here.
+// bf16 4 x 32 x 4096 x 128 in a window of 1024: 317 us, 762 TFLOP/s of visible
 // pairs, MFMA busy 42%. One token of each of 16 sequences over a window of 4096:
-// 52 us (5.1 TB/s), where HBM bounds it.
+// 58 us (4.6 TB/s), where HBM bounds it. 256 head dims do not fit the registers:
+// 192 bytes of scratch a lane (264 where rows are not aligned), 388 TFLOP/s for 2
+// x 16 x 4096 without a window.
 #include "attention.h"
 
 namespace newt_ops {
@@ -365,13 +374,19 @@ bool direct(const newt_window_attention_params& p) {
 }
 
 // Splits of the rows' tiles. Up to 256 programs have a CU each; a program's
-// tile takes about D / 100 us (1.27 for 128 head dims, 0.93 for 64), the kernel
+// tile takes 0.6 + 0.0052 D us (1.27 for 128 head dims, 0.93 for 64), the kernel
 // that joins the splits 3.5 us and what writing and reading the partial results
 // at 2.5 TB/s takes: us for 1, 2, 4, 8, 16, 32 splits of
 //   one token over 8192 keys, 8 KV heads, 4 query heads each: 162 / 86 / 47 /
 //   28 / 18 / 14; 16 sequences, window 4096: 87 / 52 / 49 / 51 / 52 / 63;
 //   128 of 4096: 86 / 52 / 34 / 29 / 29 / 41; 512 of 2048, window 512: 20 / 31;
 //   3 x 16 heads of 64, 333 of 1999, window 500: 17 / 29.
+// The line was drawn through 64 and 128 head dims. Of 256 a tile takes 4.4 us,
+// not 1.9, so that the rule, marked *, does not always find the best there:
+//   16 sequences, 4 KV heads, window 4096: 297 / 159 / 96 / 107* / 126 / 136;
+//   one token over 8192 keys, 8 KV heads: 550 / 281 / 147 / 80 / 48 / 37 (64: 48*);
+//   128 of 4096, 16 heads: 283 / 153 / 86 / 56* / 46 / 70;
+//   512 of 2048, window 512: 58* / 42 / 38 / 60; 4 x 16, 333 of 1999: 66* / 92.
 // From 512 programs of 256 rows on (two for each CU, one after the other), 8
 // waves share each tile: 4 x 32 x 4096 x 128 in a window of 1024 327 -> 315 us.
 Plan plan(const newt_window_attention_params& p) {

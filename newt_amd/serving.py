@@ -163,11 +163,14 @@ def rmsnorm(x, w, eps=1e-6, residual=None, out_dtype=None, group=None, out=None,
         hidden = x + residual              (rounded to x's dtype; None without)
         y = hidden * rsqrt(mean(hidden^2) + eps) * w
 
-    computed in fp32. w [N] is of x's dtype or fp32, residual [M, N] of x's.
+    computed in fp32 (the squares' sum too: rows of numbers around 1e19 give 0).
+    w [N] is of x's dtype or fp32, residual [M, N] of x's.
     `out` is y in x's dtype (scale None), or with out_dtype=float8_e4m3fn y /
     scale in 8 bits, with fp32 scales [M, 1] of whole rows, or [M, N / group] of
     `group` (32, 64, 128, 256) columns each: scale = max(amax |y| / 448, 2^-126),
-    amax over numbers. `hidden` given may be x or residual itself."""
+    NaN not counted; under an infinity all numbers become 0. newt has no product
+    of 8-bit operands: this output is for ones outside of it. `out` and `hidden`
+    given may be x or residual itself, and overlap nothing else."""
     r = _fast("rmsnorm", x, w, eps, residual, -1 if out_dtype is None else
               _DTYPE.get(out_dtype, -2), group, out, hidden)
     if r is not None:
@@ -275,8 +278,8 @@ def token_logprobs(logits, tokens, top=0, temperature=1.0):
 # ---------------------------------------------------------------------------
 class KVCache(NamedTuple):
     """Keys and values in 8 bits (float8_e4m3fn), in blocks of tokens with one
-    fp32 scale for each block and head; an element is its 8-bit number times
-    its scale. A block's values lie transposed."""
+    fp32 scale, not negative, for each block and head; an element is its 8-bit
+    number times its scale. A block's values lie transposed."""
     k: torch.Tensor        # [blocks, kv_heads, block_size, head_dim]
     v: torch.Tensor        # [blocks, kv_heads, head_dim, block_size]
     k_scale: torch.Tensor  # [blocks, kv_heads]
@@ -363,8 +366,8 @@ def kv_append(cache, k, v, block_table, start, count=None):
     scale). Infinities and NaN are kept as NaN and do not count for the scale.
     Positions behind the last new token keep their bytes. Tokens whose
     position lies behind the table, or in a block that is not in the cache,
-    are dropped, and all of a sequence with a negative start. No two sequences
-    of a call may write to one block."""
+    are dropped, and all of a sequence with a negative start. No block may be
+    written at two places by one call, neither of two sequences nor of one."""
     if _fast("kv_append", cache, k, v, block_table, start, count):
         return
     device = _Dev.device()
@@ -468,7 +471,10 @@ def window_attention(q, k, v, window=None, sinks=0, scale=None, q_start=None, ou
     query sees are not read where a whole tile of 64 of them is unseen, and
     never matter: what k and v hold behind the last query's position, or before
     every window, may be anything. Query heads share KV heads as in
-    cached_attention; scale and `out` are as there."""
+    cached_attention; scale and `out` are as there. A weight is rounded to q's
+    dtype before the product with the values; one below 2^-21 (fp16) of its row's
+    largest is off by up to 2^-32 of that. cached_attention rounds fp16 weights
+    to 16 bits, bf16 ones as here."""
     r = _fast("window_attention", q, k, v, window, sinks, scale, q_start, out)
     if r is not None:
         return r
