@@ -316,6 +316,8 @@ struct Wave {
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) seen[mt] = 0xffffu;
     if constexpr (CAREFUL) {
+      // rounded, in no fma with the maximum
+#pragma clang fp contract(off)
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt)
 #pragma unroll

@@ -152,6 +152,8 @@ struct Program {
                                         u32& seen) {
     const int half = (threadIdx.x & 63) >> 5;
     if constexpr (CAREFUL) {
+      // rounded, in no fma with the maximum
+#pragma clang fp contract(off)
       s[0] *= to_log2;
       s[1] *= to_log2;
       to_log2 = 1.0f;
