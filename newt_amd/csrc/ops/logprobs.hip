@@ -131,7 +131,10 @@ __device__ __forceinline__ float distance(float x, float m, float c) {
 // logarithm. Logits near the lowest number fp32 holds leave it on the way there.
 __device__ __forceinline__ float natural(float x, float m, float c, float inv_temperature) {
   const float d = distance(x, m, c);
-  return d == -kInf ? (x - m) * inv_temperature : d * kLn2;
+  if (d != -kInf) return d * kLn2;
+  const float gap = x - m;
+  return gap == -kInf && x > -kInf ? x * inv_temperature - m * inv_temperature
+                                   : gap * inv_temperature;
 }
 
 // The sums over what a lane, a wave or a split has seen.

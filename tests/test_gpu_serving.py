@@ -1048,3 +1048,19 @@ def test_rmsnorm_in_place(dtype, N):
         assert torch.equal(both[i], y) and torch.equal(both[1 - i], h)
     y = W().rmsnorm(x, w)[0]
     assert torch.equal(W().rmsnorm(x, w, out=x)[0], y) and torch.equal(x, y)
+
+
+@pytest.mark.parametrize("V", [50, 20001])
+def test_logprobs_gaps_beyond_fp32(V):
+    """fp32 logits further apart than the largest number, which a temperature
+    brings together again; -inf beside the lowest of them stays -inf."""
+    x = rnd(3, V, seed=V) * 1e38
+    x[0, :5], x[0, 5:9] = 3e38, -3e38
+    x[1] = -3.3e38
+    x[1, 3:8] = float("-inf")
+    x[2, 7] = torch.finfo(torch.float32).max
+    tokens = ints(7, 4, 9, dtype=torch.int64)
+    for temperature in (10.0, 1e20, 2.0 ** 99):
+        check_logprobs(x, tokens, 8, temperature=temperature)
+    got = W().token_logprobs(x, tokens, top=8, temperature=0.5)[0]
+    assert float(got[1]) == float("-inf")
