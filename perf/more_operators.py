@@ -184,7 +184,7 @@ def prepare(case, seed):
         s["bias"] = torch.randn(N, **at).to(t) if case.get("bias") else None
         if own:
             from newt_amd import workloads as W
-            s["laid_out"] = W.q4_weights(q, scales, zeros)
+            s["laid_out"] = W.q4_weights(q, scales, zeros, gated=kind == "gated")
     return s
 
 
