@@ -145,6 +145,80 @@ typedef struct {
 int newt_window_attention(const newt_window_attention_params* p, void* stream);
 size_t newt_window_attention_workspace(const newt_window_attention_params* p);
 
+/* Rotary positions. Pair i (of rot_dim / 2) of a head at position p is turned by
+ * p * turns[i] / 2^64 of a full turn, (a, b) -> amplitude (a cos - b sin, b cos +
+ * a sin); transposed: by the negative angle. Pairs are (i, i + rot_dim / 2), or
+ * (2 i, 2 i + 1) where interleaved. Dimensions from rot_dim on are copied. A
+ * token's position is positions[b][t], or positions[b] + t unless `each`. */
+typedef struct {
+  const void* q;            /* [batch, heads, tokens, head_dim] of dtype */
+  void* q_out;              /* as q (may be q itself) */
+  const void* k;            /* [batch, kv_heads, tokens, head_dim], or NULL with kv_heads 0 */
+  void* k_out;              /* as k (may be k itself) */
+  const uint64_t* turns;    /* [rot_dim / 2] */
+  const int32_t* positions; /* [batch, tokens] where `each`, else [batch] */
+  int64_t batch, heads, kv_heads, tokens, head_dim, rot_dim;
+  int64_t q_stride_b, q_stride_h, q_stride_t;
+  int64_t qo_stride_b, qo_stride_h, qo_stride_t;
+  int64_t k_stride_b, k_stride_h, k_stride_t;
+  int64_t ko_stride_b, ko_stride_h, ko_stride_t;
+  int64_t position_stride_b, position_stride_t;
+  float amplitude;
+  int32_t dtype, interleaved, transposed, each, reserved;
+} newt_rotate_params;
+int newt_rotate(const newt_rotate_params* p, void* stream);
+
+/* Products with 4-bit weights: y[m][n] = sum_k x[m][k] (q[n][k] - z[n][k /
+ * group]) s[n][k / group] + bias[n]; with an `act`, out = act(y of a gate row) *
+ * (y of the row that it gates), without a bias.
+ *   Weights lie in tiles of 16 rows by 128 columns, [tiles, ceil(cols / 128), 64,
+ *   4] 32-bit words: word j of lane l holds row l % 16 of the tile at columns 32 j
+ *   + 8 (l / 16) + i, i = 0..7, of which i even is at bit 2 i, i odd at bit 14 +
+ *   2 i, all rotated left by 3. Scales and zeros are [tiles, groups, 16], groups =
+ *   ceil(cols / 128) * (128 / group). Gated, tiles are a gate's and what it gates
+ *   in turn. What lies behind the last row or column may be any finite number. */
+#define NEWT_ACT_NONE 0
+#define NEWT_ACT_SILU 1 /* v / (1 + e^-v) */
+#define NEWT_ACT_GELU 2 /* v (1 + erf(v / sqrt 2)) / 2 */
+typedef struct {
+  const void* x;            /* [rows, cols] of dtype, F16 or BF16 */
+  const void* q;            /* weights, aligned to 16 bytes */
+  const void* scales;       /* of scale_dtype, F16 or BF16, aligned to 8 bytes */
+  const void* zeros;        /* bytes 0..15, aligned to 4 bytes, or NULL: 8 */
+  const void* bias;         /* [outputs] of dtype, or NULL */
+  void* out;                /* [rows, outputs] of out_dtype: dtype or F32 */
+  int64_t rows, cols, outputs;
+  int64_t x_stride, out_stride;
+  int32_t group;            /* 32, 64 or 128; divides cols */
+  int32_t dtype, scale_dtype, out_dtype, act, reserved;
+} newt_q4_params;
+int newt_q4_matmul(const newt_q4_params* p, void* stream);
+
+/* The next token of each row of logits. A token's weight is e^((logit - the
+ * row's largest) / temperature). Kept are the top_k of the largest logits (0 or
+ * less: all), of these the first, from the largest on, until their weights reach
+ * top_p of the sum (1 or more: all; the first one always), of these the ones of at
+ * least min_p; equal logits go by the lowest id. ids[t] is the first id whose
+ * running sum of kept weights exceeds u[t] times their sum; with a temperature of
+ * 0 that of the largest logit; -1 where logits hold a NaN or +inf or nothing but
+ * -inf, u[t] is NaN, or a row's setting is no number, or its temperature
+ * negative or infinite. */
+typedef struct {
+  const void* logits;         /* [rows, vocab] of dtype */
+  const float* u;             /* [rows], in [0, 1) */
+  int64_t* ids;               /* [rows] */
+  const float* temperature;   /* [rows], or NULL: that of all rows */
+  const int32_t* top_k;       /* [rows], or NULL */
+  const float* top_p;         /* [rows], or NULL */
+  const float* min_p;         /* [rows], or NULL */
+  void* workspace;            /* newt_sample_workspace() bytes, or NULL if that is 0 */
+  int64_t rows, vocab, stride;
+  float temperature_all, top_p_all, min_p_all;
+  int32_t top_k_all, dtype, reserved;
+} newt_sample_params;
+int newt_sample(const newt_sample_params* p, void* stream);
+size_t newt_sample_workspace(int64_t rows, int64_t vocab, int32_t dtype);
+
 #ifdef __cplusplus
 }
 #endif

@@ -335,6 +335,191 @@ PyObject* window_attention(PyObject* const* a, int64_t device, void* stream) {
   return wrap(s.out);
 }
 
+// rotate(q, k, rotary, positions, transposed, q_out, k_out, device, stream)
+PyObject* rotate(PyObject* const* a, int64_t device, void* stream) {
+  const Arg q(a[0], device), k(a[1], device, true), positions(a[3], device),
+      q_given(a[5], device, true), k_given(a[6], device, true);
+  REQUIRE(q.ok && k.ok && positions.ok && q_given.ok && k_given.ok && q->dim() == 4);
+  REQUIRE(PyTuple_Check(a[2]) && PyTuple_GET_SIZE(a[2]) == 3 && PyBool_Check(a[4]));
+  const Arg turns(PyTuple_GET_ITEM(a[2], 0), device);
+  double amplitude;
+  REQUIRE(turns.ok && number(PyTuple_GET_ITEM(a[2], 1), &amplitude) &&
+          PyBool_Check(PyTuple_GET_ITEM(a[2], 2)));
+  const at::ScalarType type = q->scalar_type();
+  REQUIRE(code(type) >= 0 && (!k || (k->dim() == 4 && k->scalar_type() == type)));
+  newt_rotate_params p = {};
+  p.batch = q->size(0);
+  p.heads = q->size(1);
+  p.kv_heads = k ? k->size(1) : 0;
+  p.tokens = q->size(2);
+  p.head_dim = q->size(3);
+  REQUIRE(!k || k.is(type, {p.batch, p.kv_heads, p.tokens, p.head_dim}));
+  REQUIRE(turns->scalar_type() == at::kLong && turns->dim() == 1 && turns->is_contiguous());
+  p.rot_dim = 2 * turns->size(0);
+  REQUIRE(p.rot_dim >= 2 && p.rot_dim <= p.head_dim);
+  const bool each = positions->dim() == 2;
+  REQUIRE(each ? positions.is(at::kInt, {p.batch, p.tokens}) : positions.is(at::kInt, {p.batch}));
+  REQUIRE(!q_given || q_given.is(type, q->sizes()));
+  REQUIRE(k ? !k_given || k_given.is(type, k->sizes()) : !k_given);
+  const at::Tensor q_out = q_given ? *q_given.t : empty(q->sizes(), type, *q.t);
+  at::Tensor k_out;
+  if (k) k_out = k_given ? *k_given.t : empty(k->sizes(), type, *k.t);
+  REQUIRE(q->stride(3) == 1 && q_out.stride(3) == 1);
+  REQUIRE(!k || (k->stride(3) == 1 && k_out.stride(3) == 1));
+  p.q = q.ptr();
+  p.q_out = q_out.data_ptr();
+  p.k = k.ptr();
+  p.k_out = k ? k_out.data_ptr() : nullptr;
+  p.turns = static_cast<const uint64_t*>(turns.ptr());
+  p.positions = static_cast<const int32_t*>(positions.ptr());
+  const auto strides = [](const at::Tensor& t, int64_t& b, int64_t& h, int64_t& i) {
+    b = t.stride(0);
+    h = t.stride(1);
+    i = t.stride(2);
+  };
+  strides(*q.t, p.q_stride_b, p.q_stride_h, p.q_stride_t);
+  strides(q_out, p.qo_stride_b, p.qo_stride_h, p.qo_stride_t);
+  if (k) {
+    strides(*k.t, p.k_stride_b, p.k_stride_h, p.k_stride_t);
+    strides(k_out, p.ko_stride_b, p.ko_stride_h, p.ko_stride_t);
+  }
+  p.position_stride_b = positions->stride(0);
+  p.position_stride_t = each ? positions->stride(1) : 0;
+  p.amplitude = static_cast<float>(amplitude);
+  p.dtype = code(type);
+  p.interleaved = PyTuple_GET_ITEM(a[2], 2) == Py_True;
+  p.transposed = a[4] == Py_True;
+  p.each = each;
+  REQUIRE(newt_rotate(&p, stream) == NEWT_OK);
+  return Py_BuildValue("(NN)", wrap(q_out), wrap(k_out));
+}
+
+// x and laid out weights; the outputs' sizes are left to the caller
+bool q4(PyObject* x_, PyObject* w, int64_t device, bool gated, newt_q4_params* p, Arg* x) {
+  *x = Arg(x_, device);
+  if (!x->ok || !PyTuple_Check(w) || PyTuple_GET_SIZE(w) != 7) return false;
+  const Arg q(PyTuple_GET_ITEM(w, 0), device), scales(PyTuple_GET_ITEM(w, 1), device),
+      zeros(PyTuple_GET_ITEM(w, 2), device, true);
+  int64_t outputs, cols, group;
+  if (!q.ok || !scales.ok || !zeros.ok || !whole(PyTuple_GET_ITEM(w, 3), 0, &outputs) ||
+      !whole(PyTuple_GET_ITEM(w, 4), 1, &cols) || !whole(PyTuple_GET_ITEM(w, 5), 32, &group) ||
+      PyTuple_GET_ITEM(w, 6) != (gated ? Py_True : Py_False))
+    return false;
+  if ((group != 32 && group != 64 && group != 128) || (*x)->dim() != 2) return false;
+  const at::ScalarType type = (*x)->scalar_type(), of_scales = scales->scalar_type();
+  if (type != at::kHalf && type != at::kBFloat16) return false;
+  if (of_scales != at::kHalf && of_scales != at::kBFloat16) return false;
+  if ((*x)->size(1) != cols || (cols > 1 && (*x)->stride(1) != 1)) return false;
+  const int64_t tiles = (outputs + 15) / 16 * (gated ? 2 : 1), blocks = (cols + 127) / 128;
+  const int64_t groups = blocks * (128 / group);
+  if (!q.is(at::kInt, {tiles, blocks, 64, 4}) || !scales.is(of_scales, {tiles, groups, 16}) ||
+      (zeros && !zeros.is(at::kByte, {tiles, groups, 16})))
+    return false;
+  if (!q->is_contiguous() || !scales->is_contiguous() || (zeros && !zeros->is_contiguous()))
+    return false;
+  p->x = x->ptr();
+  p->q = q.ptr();
+  p->scales = scales.ptr();
+  p->zeros = zeros.ptr();
+  p->rows = (*x)->size(0);
+  p->cols = cols;
+  p->outputs = outputs;
+  p->x_stride = (*x)->stride(0);
+  p->group = static_cast<int32_t>(group);
+  p->dtype = code(type);
+  p->scale_dtype = code(of_scales);
+  return true;
+}
+
+PyObject* q4_run(newt_q4_params* p, const Arg& x, const Arg& given, at::ScalarType to, void* stream) {
+  REQUIRE(!given || given.is(to, {p->rows, p->outputs}));
+  const at::Tensor out = given ? *given.t : empty({p->rows, p->outputs}, to, *x.t);
+  REQUIRE(p->outputs <= 1 || out.stride(1) == 1);
+  REQUIRE(p->rows <= 1 || out.stride(0) >= p->outputs);
+  p->out = out.data_ptr();
+  p->out_stride = out.stride(0);
+  p->out_dtype = code(to);
+  REQUIRE(newt_q4_matmul(p, stream) == NEWT_OK);
+  return wrap(out);
+}
+
+// q4_matmul(x, w, bias, out_dtype, out, device, stream); out_dtype as in rmsnorm
+PyObject* q4_matmul(PyObject* const* a, int64_t device, void* stream) {
+  newt_q4_params p = {};
+  Arg x(Py_None, device, true);
+  const Arg bias(a[2], device, true), given(a[4], device, true);
+  REQUIRE(bias.ok && given.ok && q4(a[0], a[1], device, false, &p, &x));
+  REQUIRE(!bias || (bias.is(x->scalar_type(), {p.outputs}) &&
+                    (p.outputs <= 1 || bias->stride(0) == 1)));
+  p.bias = bias.ptr();
+  const long kind = PyLong_AsLong(a[3]);
+  REQUIRE(kind == -1 || kind == p.dtype || kind == NEWT_F32);
+  return q4_run(&p, x, given, kind == NEWT_F32 ? at::kFloat : x->scalar_type(), stream);
+}
+
+// q4_gated(x, w, act, out, device, stream)
+PyObject* q4_gated(PyObject* const* a, int64_t device, void* stream) {
+  newt_q4_params p = {};
+  Arg x(Py_None, device, true);
+  const Arg given(a[3], device, true);
+  REQUIRE(given.ok && PyUnicode_Check(a[2]) && q4(a[0], a[1], device, true, &p, &x));
+  if (!PyUnicode_CompareWithASCIIString(a[2], "silu")) p.act = NEWT_ACT_SILU;
+  else if (!PyUnicode_CompareWithASCIIString(a[2], "gelu")) p.act = NEWT_ACT_GELU;
+  else Py_RETURN_NONE;
+  return q4_run(&p, x, given, x->scalar_type(), stream);
+}
+
+// sample(logits, u, temperature, top_k, top_p, min_p, device, stream)
+PyObject* sample(PyObject* const* a, int64_t device, void* stream) {
+  const Arg logits(a[0], device), u(a[1], device);
+  REQUIRE(logits.ok && u.ok && logits->dim() == 2 && logits->size(1) > 0 &&
+          logits->size(1) < kLimit);
+  newt_sample_params p = {};
+  const int type = code(logits->scalar_type());
+  p.rows = logits->size(0);
+  p.vocab = logits->size(1);
+  const auto per_row = [&](const Arg& t, at::ScalarType of) {
+    return t.ok && t.is(of, {p.rows}) && (p.rows <= 1 || t->stride(0) == 1);
+  };
+  REQUIRE(type >= 0 && per_row(u, at::kFloat) && (p.vocab == 1 || logits->stride(1) == 1));
+  const auto setting = [&](PyObject* o, const float** rows, float* all) {
+    double v;
+    if (number(o, &v)) {
+      *all = static_cast<float>(v);
+      return true;
+    }
+    if (!THPVariable_Check(o)) return false;
+    const Arg t(o, device);
+    if (!per_row(t, at::kFloat)) return false;
+    *rows = static_cast<const float*>(t.ptr());
+    return true;
+  };
+  REQUIRE(setting(a[2], &p.temperature, &p.temperature_all) &&
+          setting(a[4], &p.top_p, &p.top_p_all) && setting(a[5], &p.min_p, &p.min_p_all));
+  int64_t top_k;
+  if (whole(a[3], 0, &top_k)) {
+    p.top_k_all = static_cast<int32_t>(top_k);
+  } else {
+    REQUIRE(THPVariable_Check(a[3]));
+    const Arg t(a[3], device);
+    REQUIRE(per_row(t, at::kInt));
+    p.top_k = static_cast<const int32_t*>(t.ptr());
+  }
+  const at::Tensor ids = empty({p.rows}, at::kLong, *logits.t);
+  at::Tensor workspace;
+  if (const size_t need = newt_sample_workspace(p.rows, p.vocab, type)) {
+    workspace = empty({static_cast<int64_t>(need)}, at::kByte, *logits.t);
+    p.workspace = workspace.data_ptr();
+  }
+  p.logits = logits.ptr();
+  p.u = static_cast<const float*>(u.ptr());
+  p.ids = static_cast<int64_t*>(ids.data_ptr());
+  p.stride = logits->stride(0);
+  p.dtype = type;
+  REQUIRE(newt_sample(&p, stream) == NEWT_OK);
+  return wrap(ids);
+}
+
 // The last two arguments are the current device and its stream. What torch
 // throws (out of memory) becomes a Python exception: no C++ one leaves here.
 template <PyObject* (*F)(PyObject* const*, int64_t, void*), int ARGS>
@@ -356,7 +541,9 @@ PyObject* entry(PyObject*, PyObject* const* a, Py_ssize_t n) {
   {#name, reinterpret_cast<PyCFunction>(entry<name, args>), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {ENTRY(rmsnorm, 8),          ENTRY(token_logprobs, 4),
                          ENTRY(kv_append, 6),        ENTRY(cached_attention, 8),
-                         ENTRY(window_attention, 8), {nullptr, nullptr, 0, nullptr}};
+                         ENTRY(window_attention, 8), ENTRY(rotate, 7),
+                         ENTRY(q4_matmul, 5),        ENTRY(q4_gated, 4),
+                         ENTRY(sample, 6),           {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_newt_ops",
                       "Ordinary calls of newt_amd.serving's operators.", -1, methods,

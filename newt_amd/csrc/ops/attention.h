@@ -7,8 +7,6 @@
 // a program share each key and value tile and a single token still fills G
 // rows.
 #pragma once
-#include <utility>
-
 #include "common.h"
 
 namespace newt_ops {
@@ -161,27 +159,6 @@ join_splits_kernel(const void* workspace, void* out, Rows o, int64_t units, int 
   const u32 head = sequence_head % kv_heads, b = sequence_head / kv_heads;
   T* to = (T*)out + o.at(b, head * group + r % group, r / group) + d;
   newt::store_vec<T, 4>(to, t, newt::any_align());
-}
-
-// Whether rows of `dim` numbers in three dimensions share memory, which several
-// programs would write at once: a dimension, from the smallest stride on, has to
-// step over all that those before it reach. Slices, permutations and the like of
-// a tensor without overlaps do.
-inline bool rows_overlap(int dim, int64_t n0, int64_t s0, int64_t n1, int64_t s1, int64_t n2,
-                         int64_t s2) {
-  struct { int64_t n, stride; } d[3] = {{n0, s0}, {n1, s1}, {n2, s2}};
-  for (auto& e : d) e.stride = e.stride < 0 ? -e.stride : e.stride;
-  const auto order = [&](int i, int j) { if (d[j].stride < d[i].stride) std::swap(d[i], d[j]); };
-  order(0, 1);
-  order(1, 2);
-  order(0, 1);
-  double reach = dim;  // what strides of any size cannot exceed
-  for (const auto& e : d) {
-    if (e.n <= 1) continue;
-    if ((double)e.stride < reach) return true;
-    reach += (double)(e.n - 1) * (double)e.stride;
-  }
-  return false;
 }
 
 // What both operators refuse of their queries, outputs and scale; null: nothing.

@@ -6,6 +6,7 @@
 #include <hip/hip_runtime.h>
 
 #include <type_traits>
+#include <utility>
 
 #include "../../../include/newt_ops.h"
 #include "newt_gfx950.h"
@@ -34,6 +35,27 @@ int run(const char* what, void (*kernel)(P...), int64_t grid, int block, unsigne
 
 // What is wrong with a cache's description, or null.
 const char* cache_wrong(const newt_kv_cache& c);
+
+// Whether rows of `dim` numbers in three dimensions share memory, which several
+// programs would write at once: a dimension, from the smallest stride on, has to
+// step over all that those before it reach. Slices, permutations and the like of
+// a tensor without overlaps do.
+inline bool rows_overlap(int dim, int64_t n0, int64_t s0, int64_t n1, int64_t s1, int64_t n2,
+                         int64_t s2) {
+  struct { int64_t n, stride; } d[3] = {{n0, s0}, {n1, s1}, {n2, s2}};
+  for (auto& e : d) e.stride = e.stride < 0 ? -e.stride : e.stride;
+  const auto order = [&](int i, int j) { if (d[j].stride < d[i].stride) std::swap(d[i], d[j]); };
+  order(0, 1);
+  order(1, 2);
+  order(0, 1);
+  double reach = dim;  // what strides of any size cannot exceed
+  for (const auto& e : d) {
+    if (e.n <= 1) continue;
+    if ((double)e.stride < reach) return true;
+    reach += (double)(e.n - 1) * (double)e.stride;
+  }
+  return false;
+}
 
 // ---------------------------------------------------------------------------
 // workgroup reductions: each wave's partial through LDS, read back by all.

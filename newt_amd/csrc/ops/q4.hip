@@ -1,0 +1,251 @@
+// Products with 4-bit weights and a scale for each group of columns:
+//   y[m][n] = sum_g s[n][g] (sum_k x[m][k] q[n][k] - z[n][g] sum_k x[m][k])
+// and, for a gated feed-forward block, act(y of the gate) * (y of the rest).
+// For few rows the weights' bytes bound it: each is read once, 16 bytes a lane
+// in the order in which the matrix unit takes it, and no number of it goes
+// through LDS. A weight becomes a 16-bit number without a conversion: its 4 bits
+// are put below the point of a number in [1, 2), (16 + q) / 16, exactly. The
+// products' sums then hold (16 + z) / 16 times the sum of x too much, which comes
+// from one more product, of x and ones, for all rows of weights that a wave has:
+//   sum_k x (q - z) = 16 (sum_k x (16 + q) / 16 - (16 + z) / 16 sum_k x)
+// A wave takes NT tiles of 16 weight rows, MT tiles of 16 rows of x and every
+// WAVES-th block of 128 columns; the waves' sums are joined in LDS.
+#include "common.h"
+
+namespace newt_ops {
+namespace {
+
+template <typename T> struct frag;
+template <> struct frag<bf16> { typedef bf16x8 type; };
+template <> struct frag<f16> { typedef f16x8 type; };
+
+// 8 weights to (16 + q) / 16
+template <typename T>
+__device__ __forceinline__ typename frag<T>::type widen(u32 w) {
+  u32x4 r;
+  if constexpr (__is_same(T, bf16)) {  // the 4 upper of 7 bits
+    const u32 mask = 0x00780078, one = 0x3f803f80;
+    r[0] = (w & mask) | one;
+    r[1] = ((w >> 4) & mask) | one;
+    r[2] = ((w >> 8) & mask) | one;
+    r[3] = (__builtin_amdgcn_alignbit(w, w, 12) & mask) | one;
+  } else {  // of 10 bits
+    const u32 mask = 0x03c003c0, one = 0x3c003c00;
+    r[0] = ((w << 3) & mask) | one;
+    r[1] = ((w >> 1) & mask) | one;
+    r[2] = ((w >> 5) & mask) | one;
+    r[3] = (__builtin_amdgcn_alignbit(w, w, 9) & mask) | one;
+  }
+  return __builtin_bit_cast(typename frag<T>::type, r);
+}
+
+__device__ __forceinline__ float activate(float v, int act) {
+  if (act == NEWT_ACT_SILU) return v / (1.0f + __builtin_expf(-v));
+  return 0.5f * v * (1.0f + erff(v * 0.70710678f));
+}
+
+template <typename T, int NT, int MT, int WAVES, int GROUP, bool GATED>
+__global__ void __launch_bounds__(64 * WAVES)
+q4_kernel(newt_q4_params p, int n_blocks) {
+  typedef typename frag<T>::type TX;
+  constexpr int STEPS = GROUP / 32, PER = 128 / GROUP;  // of a group, groups of a block
+  constexpr int SIZE = NT * MT * 256;                   // sums of a wave
+  __shared__ __attribute__((aligned(16))) float sums[WAVES * SIZE];
+  const int lane = threadIdx.x & 63, wave = wave_id(), part = lane >> 4, col = lane & 15;
+  const int n_block = blockIdx.x % n_blocks, m_block = blockIdx.x / n_blocks;
+  const int blocks = (int)((p.cols + 127) / 128), groups = blocks * PER;
+  const int64_t tiles = (p.outputs + 15) / 16 * (GATED ? 2 : 1);
+  const int64_t tile = (int64_t)n_block * NT;
+
+  const u32x4* q[NT];
+  int64_t at[NT];  // of scales and zeros
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const int64_t t = tile + n < tiles ? tile + n : tiles - 1;
+    q[n] = (const u32x4*)p.q + t * blocks * 64 + lane;
+    at[n] = t * groups * 16 + 4 * part;
+  }
+  const T* x[MT];
+  bool in[MT];
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+    const int64_t row = ((int64_t)m_block * MT + m) * 16 + col;
+    in[m] = row < p.rows;
+    x[m] = (const T*)p.x + (in[m] ? row : 0) * p.x_stride + 8 * part;
+  }
+  TX ones;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) ones[i] = (T)1.0f;
+  f32x4 acc[NT][MT];
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int m = 0; m < MT; ++m) acc[n][m] = (f32x4)(0.0f);
+
+  for (int b = wave; b < blocks; b += WAVES) {
+    u32x4 w[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) w[n] = q[n][(int64_t)b * 64];
+    TX v[MT][4];
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        T t[8] = {};
+        if (in[m] && b * 128 + 32 * j < p.cols)
+          newt::load_vec<T, 8>(x[m] + b * 128 + 32 * j, t, newt::any_align());
+        v[m][j] = __builtin_bit_cast(TX, newt::pack8(t[0], t[1], t[2], t[3], t[4], t[5], t[6], t[7]));
+      }
+#pragma unroll
+    for (int g = 0; g < PER; ++g) {
+      f32x4 all[MT];
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        all[m] = (f32x4)(0.0f);
+#pragma unroll
+        for (int j = 0; j < STEPS; ++j) all[m] = newt::mfma_16x16x32(ones, v[m][g * STEPS + j], all[m]);
+      }
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const int64_t s = at[n] + (int64_t)(b * PER + g) * 16;
+        float scale[4], zero[4];
+        if (p.scale_dtype == NEWT_F16) {
+          f16 t[4];
+          newt::load_vec<f16, 4>((const f16*)p.scales + s, t);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) scale[i] = newt::to_f32(t[i]);
+        } else {
+          bf16 t[4];
+          newt::load_vec<bf16, 4>((const bf16*)p.scales + s, t);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) scale[i] = newt::to_f32(t[i]);
+        }
+        u32 z = 0x08080808u;
+        if (p.zeros) z = *(const u32*)((const unsigned char*)p.zeros + s);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) zero[i] = -1.0f - 0.0625f * (float)((z >> (8 * i)) & 255);
+        TX a[STEPS];
+#pragma unroll
+        for (int j = 0; j < STEPS; ++j) a[j] = widen<T>(w[n][g * STEPS + j]);
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          f32x4 part_sum = (f32x4)(0.0f);
+#pragma unroll
+          for (int j = 0; j < STEPS; ++j)
+            part_sum = newt::mfma_16x16x32(a[j], v[m][g * STEPS + j], part_sum);
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            acc[n][m][i] = __builtin_fmaf(__builtin_fmaf(all[m][i], zero[i], part_sum[i]), scale[i],
+                                          acc[n][m][i]);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+      *(f32x4*)(sums + wave * SIZE + ((n * MT + m) * 64 + lane) * 4) = acc[n][m];
+  __syncthreads();
+  // 4 neighbouring outputs of a row of x at a time
+  constexpr int OUT = GATED ? NT / 2 : NT;
+  const auto joined = [&](int n, int m, int l) {
+    f32x4 t = (f32x4)(0.0f);
+#pragma unroll
+    for (int i = 0; i < WAVES; ++i) t += *(const f32x4*)(sums + i * SIZE + ((n * MT + m) * 64 + l) * 4);
+    return t * 16.0f;
+  };
+  for (int e = threadIdx.x; e < OUT * MT * 64; e += 64 * WAVES) {
+    const int l = e & 63, m = e / 64 % MT, n = e / 64 / MT;
+    const int64_t row = ((int64_t)m_block * MT + m) * 16 + (l & 15);
+    const int64_t first = ((int64_t)n_block * OUT + n) * 16 + 4 * (l >> 4);
+    if (row >= p.rows || first >= p.outputs) continue;
+    f32x4 y;
+    if constexpr (GATED) {
+      const f32x4 gate = joined(2 * n, m, l), up = joined(2 * n + 1, m, l);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) y[i] = activate(gate[i], p.act) * up[i];
+    } else {
+      y = joined(n, m, l);
+    }
+    const int count = p.outputs - first < 4 ? (int)(p.outputs - first) : 4;
+    if (!GATED && p.bias)
+      for (int i = 0; i < count; ++i) y[i] += newt::to_f32(((const T*)p.bias)[first + i]);
+    if (p.out_dtype == NEWT_F32) {
+      float* out = (float*)p.out + row * p.out_stride + first;
+      const float t[4] = {y[0], y[1], y[2], y[3]};
+      if (count == 4) newt::store_vec<float, 4>(out, t, newt::any_align());
+      else for (int i = 0; i < count; ++i) out[i] = y[i];
+    } else {
+      T* out = (T*)p.out + row * p.out_stride + first;
+      const T t[4] = {(T)y[0], (T)y[1], (T)y[2], (T)y[3]};
+      if (count == 4) newt::store_vec<T, 4>(out, t, newt::any_align());
+      else for (int i = 0; i < count; ++i) out[i] = (T)y[i];
+    }
+  }
+}
+
+template <typename T, int GROUP, bool GATED>
+int launch(const newt_q4_params& p, hipStream_t stream) {
+  const int64_t tiles = (p.outputs + 15) / 16 * (GATED ? 2 : 1);
+  const auto go = [&](auto nt, auto mt, auto waves) {
+    constexpr int NT = decltype(nt)::value, MT = decltype(mt)::value, WAVES = decltype(waves)::value;
+    const int64_t n_blocks = (tiles + NT - 1) / NT, m_blocks = (p.rows + 16 * MT - 1) / (16 * MT);
+    if (n_blocks * m_blocks > 0x7fffffff)
+      return fail(NEWT_ERR_INVALID, "newt_q4_matmul: too many rows");
+    return run("newt_q4_matmul", q4_kernel<T, NT, MT, WAVES, GROUP, GATED>, n_blocks * m_blocks,
+               64 * WAVES, 0, stream, p, (int)n_blocks);
+  };
+#define NEWT_TILE(NT, MT, WAVES)                                                       \
+  go(std::integral_constant<int, NT>(), std::integral_constant<int, MT>(),             \
+     std::integral_constant<int, WAVES>())
+  if (p.rows <= 16) return NEWT_TILE(2, 1, 8);
+  return NEWT_TILE(4, 4, 2);
+#undef NEWT_TILE
+}
+
+template <typename T, bool GATED>
+int by_group(const newt_q4_params& p, hipStream_t stream) {
+  switch (p.group) {
+    case 32: return launch<T, 32, GATED>(p, stream);
+    case 64: return launch<T, 64, GATED>(p, stream);
+    default: return launch<T, 128, GATED>(p, stream);
+  }
+}
+
+template <typename T>
+int by_act(const newt_q4_params& p, hipStream_t stream) {
+  return p.act == NEWT_ACT_NONE ? by_group<T, false>(p, stream) : by_group<T, true>(p, stream);
+}
+
+const char* wrong(const newt_q4_params& p) {
+  if (p.rows < 0 || p.outputs < 0 || p.cols <= 0) return "bad size";
+  if (p.rows >= 1 << 30 || p.outputs >= 1 << 30 || p.cols >= 1 << 30) return "sizes stay below 2^30";
+  if (p.group != 32 && p.group != 64 && p.group != 128) return "groups are of 32, 64 or 128 columns";
+  if (p.cols % p.group) return "columns have to be whole groups";
+  if (p.act != NEWT_ACT_NONE && p.act != NEWT_ACT_SILU && p.act != NEWT_ACT_GELU)
+    return "unknown activation";
+  if (p.act != NEWT_ACT_NONE && p.bias) return "a gated product has no bias";
+  if (p.dtype != NEWT_F16 && p.dtype != NEWT_BF16) return "x is fp16 or bf16";
+  if (p.scale_dtype != NEWT_F16 && p.scale_dtype != NEWT_BF16) return "scales are fp16 or bf16";
+  if (p.out_dtype != p.dtype && p.out_dtype != NEWT_F32) return "out is of x's type or fp32";
+  if (p.rows > 1 && p.out_stride < p.outputs) return "rows of out overlap";
+  return nullptr;
+}
+
+}  // namespace
+}  // namespace newt_ops
+
+extern "C" int newt_q4_matmul(const newt_q4_params* params, void* stream) {
+  using namespace newt_ops;
+  if (!params) return fail(NEWT_ERR_INVALID, "newt_q4_matmul: null params");
+  const newt_q4_params& p = *params;
+  if (const char* w = wrong(p)) return fail(NEWT_ERR_INVALID, "newt_q4_matmul: %s", w);
+  if (p.rows == 0 || p.outputs == 0) return NEWT_OK;
+  if (!p.x || !p.q || !p.scales || !p.out)
+    return fail(NEWT_ERR_INVALID, "newt_q4_matmul: null tensor");
+  if (((uintptr_t)p.q & 15) | ((uintptr_t)p.scales & 7) | ((uintptr_t)p.zeros & 3))
+    return fail(NEWT_ERR_INVALID, "newt_q4_matmul: weights are not aligned");
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  return p.dtype == NEWT_F16 ? by_act<f16>(p, s) : by_act<bf16>(p, s);
+}

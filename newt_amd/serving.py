@@ -2,8 +2,9 @@
 
 They stand beside the kernels of `newt_amd.workloads`, which re-exports them:
 `rmsnorm` beside `layernorm`, `window_attention` and `cached_attention` beside
-`attention`, `token_logprobs` beside `softmax`. All are forward only, as the
-others are. The kernels are in csrc/ops, behind the C ABI of
+`attention`, `token_logprobs` and `sample` beside `softmax`, `q4_matmul` and
+`q4_gated` beside `matmul`, `rotate` in front of `kv_append`. All are forward
+only, as the others are (`rotate` transposed is its own gradient). The kernels are in csrc/ops, behind the C ABI of
 include/newt_ops.h; they are compiled ahead of time, so a first call costs no
 compilation.
 
@@ -16,12 +17,18 @@ range) before anything is launched.
 One step of a decoder layer over the 8-bit cache:
 
     x, _, hidden = rmsnorm(x, w_norm, residual=hidden)
-    q, k, v = ...                      # matmul(x, ...), rotated
+    q, k, v = ...                      # slices of q4_matmul(x, w_qkv)
+    q, k = rotate(q, k, positions_of, lens - k.shape[2])
     kv_append(cache, k, v, block_table, lens - k.shape[2])
     o = cached_attention(q, cache, block_table, lens)
+    x, _, hidden = rmsnorm(q4_matmul(o, w_out), w_norm2, residual=hidden)
+    x = q4_matmul(q4_gated(x, w_gate_up), w_down)
+
+and after the last one ids = sample(q4_matmul(x, w_vocab), u, top_p=0.9).
 """
 
 import ctypes
+import decimal
 import functools
 import math
 import os
@@ -47,6 +54,9 @@ _CACHE = "4Qq4i"
 _APPEND = struct.Struct("=" + _CACHE + "5Q10q2i")
 _CACHED = struct.Struct("=" + _CACHE + "5Q12qf3i")
 _WINDOW = struct.Struct("=6Q17qf5i")
+_ROTATE = struct.Struct("=6Q20qf5i")
+_Q4 = struct.Struct("=6Q5q6i")
+_SAMPLE = struct.Struct("=8Q3q3f3i")
 
 
 @functools.cache
@@ -59,7 +69,7 @@ def lib():
             f"`python -m newt_amd.build`")
     L = ctypes.CDLL(LIB_PATH)
     for name in ("newt_rmsnorm", "newt_token_logprobs", "newt_kv_append", "newt_cached_attention",
-                 "newt_window_attention"):
+                 "newt_window_attention", "newt_rotate", "newt_q4_matmul", "newt_sample"):
         f = getattr(L, name)
         f.restype, f.argtypes = ctypes.c_int, [ctypes.c_char_p, ctypes.c_void_p]
     for name in ("newt_cached_attention_workspace", "newt_window_attention_workspace"):
@@ -68,6 +78,8 @@ def lib():
     L.newt_token_logprobs_workspace.restype = ctypes.c_size_t
     L.newt_token_logprobs_workspace.argtypes = [ctypes.c_int64, ctypes.c_int64, ctypes.c_int32,
                                                 ctypes.c_int32]
+    L.newt_sample_workspace.restype = ctypes.c_size_t
+    L.newt_sample_workspace.argtypes = [ctypes.c_int64, ctypes.c_int64, ctypes.c_int32]
     L.newt_ops_last_error.restype = ctypes.c_char_p
     if L.newt_ops_abi_version() != 1:
         raise RuntimeError("newt: libnewt_ops.so ABI mismatch; rebuild it")
@@ -510,3 +522,353 @@ def window_attention(q, k, v, window=None, sinks=0, scale=None, q_start=None, ou
         params = _WINDOW.pack(*pointers, workspace.data_ptr(), *rest)
     _call(L.newt_window_attention, "window_attention", params, device)
     return out
+
+
+# ---------------------------------------------------------------------------
+# rotary positions
+# ---------------------------------------------------------------------------
+class Rotary(NamedTuple):
+    """How pairs of a head turn with the position, made by `rotary`."""
+    turns: torch.Tensor  # [dim / 2] int64: 2^64 of a full turn a position
+    amplitude: float
+    interleaved: bool
+
+
+_PI = decimal.Decimal("3.14159265358979323846264338327950288419716939937510")
+
+
+def rotary(dim, base=10000.0, factor=1.0, ramp=None, amplitude=1.0, interleaved=False,
+           frequencies=None, device=None):
+    """The Rotary of heads whose first `dim` dimensions turn: pair i by base^(-2 i /
+    dim) radians a position, or by frequencies[i]. Pairs are (i, i + dim / 2), or
+    (2 i, 2 i + 1) where interleaved.
+
+    For contexts longer than a model was trained on, frequencies are divided by
+    `factor`; with ramp=(original, low, high) only those that turn less than `low`
+    times over `original` positions, not those that turn at least `high` times,
+    and in between a share that falls evenly with the number of turns. The turned
+    dimensions come out `amplitude` times as large."""
+    _whole("rotary", "dim", dim, 2)
+    if dim % 2:
+        raise ValueError(f"rotary: dim={dim} is odd")
+    if not isinstance(interleaved, bool):
+        raise TypeError("rotary: interleaved must be a bool")
+    for name, value in (("base", base), ("factor", factor)):
+        if not 0.0 < value < math.inf:
+            raise ValueError(f"rotary: {name}={value} has to be positive and finite")
+    amplitude = _fp32(amplitude)
+    if not math.isfinite(amplitude):
+        raise ValueError("rotary: amplitude has to be finite")
+    if ramp is not None:
+        original, low, high = ramp
+        if not (0.0 < original < math.inf and 0.0 <= low < high < math.inf):
+            raise ValueError(f"rotary: ramp={ramp} is not (original, low, high), low < high")
+    number = decimal.Decimal
+    # a fraction of a turn to 64 bits, whatever its size, needs more than fp64
+    with decimal.localcontext(decimal.Context(prec=60)):
+        if frequencies is None:
+            frequencies = [number(base) ** (number(-2 * i) / dim) for i in range(dim // 2)]
+        else:
+            frequencies = [float(f) for f in frequencies]
+            if len(frequencies) != dim // 2 or not all(math.isfinite(f) for f in frequencies):
+                raise ValueError(f"rotary: {dim // 2} finite frequencies are needed")
+        turns = []
+        for f in frequencies:
+            f = number(f) / (2 * _PI)
+            share = number(0)  # of the frequency as it is
+            if ramp is not None:
+                share = (abs(f) * number(original) - number(low)) / (number(high) - number(low))
+                share = min(max(share, number(0)), number(1))
+            f = f * share + f / number(factor) * (1 - share)
+            t = int((f * 2 ** 64).to_integral_value()) % 2 ** 64
+            turns.append(t - 2 ** 64 if t >= 2 ** 63 else t)
+    device = torch.device("cuda", _Dev.device()) if device is None else device
+    return Rotary(torch.tensor(turns, dtype=torch.int64, device=device), amplitude, interleaved)
+
+
+def rotate(q, k, rotary, positions, transposed=False, q_out=None, k_out=None):
+    """(q_out, k_out): q [B, H, S, head_dim] and k [B, kv_heads, S, head_dim], fp32,
+    fp16 or bf16 (any strides but along head_dim), turned as `rotary` says by
+    their tokens' positions; k may be None. positions are int32, [B, S], or [B]: the
+    first token's, the others follow it. They may be any, negative ones too: the
+    angle is right to 2^-30 of a radian everywhere.
+
+    (a, b) -> amplitude (a cos - b sin, b cos + a sin) in fp32, rounded once;
+    dimensions from the rotary's on are copied. Transposed, the angle's sign is
+    changed: the map that takes the outputs' gradients to the inputs'. Outputs
+    given may be q and k themselves, and overlap nothing else."""
+    r = _fast("rotate", q, k, rotary, positions, transposed, q_out, k_out)
+    if r is not None:
+        return r
+    device = _Dev.device()
+    if not isinstance(rotary, (tuple, list)) or len(rotary) != 3:
+        raise TypeError("rotate: rotary must be a Rotary")
+    turns, amplitude, interleaved = rotary
+    _tensors("rotate", device, {"k": k, "q_out": q_out, "k_out": k_out}, q=q, turns=turns,
+             positions=positions)
+    if q.dim() != 4:
+        raise ValueError(f"rotate: q has shape {tuple(q.shape)}, not [B, H, S, head_dim]")
+    if q.dtype not in _DTYPE or q.dtype == E4M3:
+        raise TypeError(f"rotate: q is {q.dtype}")
+    B, H, S, D = q.shape
+    KV = 0
+    if k is not None:
+        if k.dim() != 4:
+            raise ValueError(f"rotate: k has shape {tuple(k.shape)}, not [B, kv_heads, S, head_dim]")
+        KV = k.shape[1]
+        _shape("rotate", "k", k, (B, KV, S, D), q.dtype)
+    elif k_out is not None:
+        raise ValueError("rotate: k_out is an output of k")
+    if turns.dim() != 1 or turns.dtype != torch.int64 or not turns.is_contiguous():
+        raise TypeError("rotate: rotary must be a Rotary")
+    rot = 2 * turns.shape[0]
+    if not 2 <= rot <= D:
+        raise ValueError(f"rotate: a rotary of {rot} dimensions for heads of {D}")
+    if positions.dtype != torch.int32:
+        raise TypeError(f"rotate: positions are {positions.dtype}, not int32")
+    if positions.shape != (B,) and positions.shape != (B, S):
+        raise ValueError(f"rotate: positions have shape {tuple(positions.shape)}, not {(B,)} or "
+                         f"{(B, S)}")
+    each = positions.dim() == 2
+    outs = []
+    for name, x, out in (("q_out", q, q_out), ("k_out", k, k_out)):
+        if x is not None and out is None:
+            out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        elif x is not None:
+            _shape("rotate", name, out, x.shape, x.dtype)
+        outs.append(out)
+    if any(t is not None and t.stride(3) != 1 and D > 1 for t in (q, k, *outs)):
+        raise ValueError("rotate: tensors need unit stride along head_dim")
+    strides = [s for t in (q, outs[0], k, outs[1]) for s in ((0, 0, 0) if t is None
+                                                           else t.stride()[:3])]
+    _call(lib().newt_rotate, "rotate", _ROTATE.pack(
+        q.data_ptr(), outs[0].data_ptr(), _ptr(k), _ptr(outs[1]), turns.data_ptr(),
+        positions.data_ptr(), B, H, KV, S, D, rot, *strides, positions.stride(0),
+        positions.stride(1) if each else 0, _fp32(amplitude), _DTYPE[q.dtype], bool(interleaved),
+        bool(transposed), each, 0), device)
+    return tuple(outs)
+
+
+# ---------------------------------------------------------------------------
+# products with 4-bit weights
+# ---------------------------------------------------------------------------
+class Q4Weights(NamedTuple):
+    """4-bit weights laid out for the kernels by `q4_weights`."""
+    q: torch.Tensor       # [tiles, ceil(cols / 128), 64, 4] int32
+    scales: torch.Tensor  # [tiles, groups, 16]
+    zeros: torch.Tensor   # as scales, uint8, or None
+    outputs: int          # rows of weights; of a gated pair those of one
+    cols: int
+    group: int
+    gated: bool
+
+
+def q4_weights(q, scales, zeros=None, gated=False):
+    """Weights [N, K] of 4 bits, laid out once for q4_matmul or, gated, for q4_gated:
+    (number - zero) * scale. q [N, K / 2] uint8 holds two neighbouring columns'
+    numbers a byte, the first one's in the lower half. scales [N, K / group] fp16
+    or bf16 and zeros, uint8 as scales (8 without), are for groups of 32, 64 or 128
+    columns. Of gated weights the first N / 2 rows are the gate's."""
+    for name, t in (("q", q), ("scales", scales)) + ((("zeros", zeros),) if zeros is not None else ()):
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"q4_weights: {name} must be a tensor")
+        if t.dim() != 2:
+            raise ValueError(f"q4_weights: {name} has shape {tuple(t.shape)}, not two dimensions")
+        if t.device != q.device:
+            raise TypeError(f"q4_weights: {name} is not on q's device")
+    if not isinstance(gated, bool):
+        raise TypeError("q4_weights: gated must be a bool")
+    if q.dtype != torch.uint8:
+        raise TypeError(f"q4_weights: q is {q.dtype}, not uint8")
+    if scales.dtype != torch.float16 and scales.dtype != torch.bfloat16:
+        raise TypeError(f"q4_weights: scales are {scales.dtype}, not float16 or bfloat16")
+    N, K = q.shape[0], 2 * q.shape[1]
+    groups = scales.shape[1]
+    if scales.shape[0] != N or groups == 0 or K % groups or K // groups not in (32, 64, 128):
+        raise ValueError(f"q4_weights: scales of shape {tuple(scales.shape)} are not those of [{N}, "
+                         f"{K}] in groups of 32, 64 or 128 columns")
+    group = K // groups
+    if zeros is not None:
+        _shape("q4_weights", "zeros", zeros, scales.shape, torch.uint8)
+    if gated and N % 2:
+        raise ValueError(f"q4_weights: {N} rows are not a gate's and what it gates")
+    if N >= 2 ** 30 or K >= 2 ** 30:
+        raise ValueError("q4_weights: sizes stay below 2^30")
+    halves = 2 if gated else 1
+    outputs, blocks = N // halves, -(-K // 128)
+    tiles = -(-outputs // 16)
+
+    def tiled(t, cols, fill):
+        """[halves * tiles, 16, cols], the halves' tiles in turn, `fill` around."""
+        r = t.new_full((halves, tiles * 16, cols), fill)
+        r[:, :outputs, :t.shape[1]] = t.view(halves, outputs, -1)
+        return r.view(halves, tiles, 16, cols).transpose(0, 1).reshape(halves * tiles, 16, cols)
+
+    words = torch.empty(halves * tiles, blocks, 64, 4, dtype=torch.int32, device=q.device)
+    packed = tiled(q.contiguous(), blocks * 64, 0x88)
+    step = max(1, (1 << 26) // (blocks * 1024))  # tiles at a time
+    for i in range(0, len(words), step):
+        # [tiles, row, block, j, part, pair] -> [tiles, block, part, row, j, pair]
+        b = packed[i:i + step].view(-1, 16, blocks, 4, 4, 4).permute(0, 2, 4, 1, 3, 5).int()
+        w = torch.zeros(b.shape[:-1], dtype=torch.int32, device=q.device)
+        for pair in range(4):
+            w |= (b[..., pair] & 15) << (4 * pair) | (b[..., pair] >> 4) << (16 + 4 * pair)
+        w = w << 3 | (w >> 29) & 7
+        words[i:i + step] = w.view(-1, blocks, 64, 4)
+    per = blocks * (128 // group)
+    laid_out = [None if t is None else tiled(t.contiguous(), per, fill).transpose(1, 2).contiguous()
+                for t, fill in ((scales, 0.0), (zeros, 8))]
+    return Q4Weights(words, *laid_out, outputs, K, group, gated)
+
+
+def _q4(what, x, w, gated, optional):
+    """Checked sizes, x's type and the weights' packed fields."""
+    if not isinstance(w, Q4Weights):
+        raise TypeError(f"{what}: w must be Q4Weights")
+    device = _Dev.device()
+    _tensors(what, device, {"zeros": w.zeros, **optional}, x=x, q=w.q, scales=w.scales)
+    if x.dim() != 2:
+        raise ValueError(f"{what}: x has shape {tuple(x.shape)}, not [M, K]")
+    if x.dtype != torch.float16 and x.dtype != torch.bfloat16:
+        raise TypeError(f"{what}: x is {x.dtype}, not float16 or bfloat16")
+    if w.gated != gated:
+        raise ValueError(f"{what}: weights are {'' if w.gated else 'not '}laid out gated")
+    M, K = x.shape
+    if K != w.cols:
+        raise ValueError(f"{what}: x has {K} columns, the weights {w.cols}")
+    if K > 1 and x.stride(1) != 1:
+        raise ValueError(f"{what}: rows of x need unit stride")
+    if w.group not in (32, 64, 128):
+        raise ValueError(f"{what}: no groups of {w.group} columns")
+    tiles, blocks = -(-w.outputs // 16) * (2 if gated else 1), -(-K // 128)
+    _shape(what, "q", w.q, (tiles, blocks, 64, 4), torch.int32)
+    _shape(what, "scales", w.scales, (tiles, blocks * (128 // w.group), 16))
+    if w.scales.dtype != torch.float16 and w.scales.dtype != torch.bfloat16:
+        raise TypeError(f"{what}: scales are {w.scales.dtype}, not float16 or bfloat16")
+    if w.zeros is not None:
+        _shape(what, "zeros", w.zeros, w.scales.shape, torch.uint8)
+    if not all(t is None or t.is_contiguous() for t in w[:3]):
+        raise ValueError(f"{what}: weights have to be contiguous")
+    return device, M
+
+
+def _q4_call(what, x, w, bias, out, act, device):
+    M, N = x.shape[0], w.outputs
+    if N > 1 and out.stride(1) != 1:
+        raise ValueError(f"{what}: rows of out need unit stride")
+    if M > 1 and out.stride(0) < N:
+        raise ValueError(f"{what}: rows of out overlap")
+    _call(lib().newt_q4_matmul, what, _Q4.pack(
+        x.data_ptr(), w.q.data_ptr(), w.scales.data_ptr(), _ptr(w.zeros), _ptr(bias),
+        out.data_ptr(), M, w.cols, N, x.stride(0), out.stride(0), w.group, _DTYPE[x.dtype],
+        _DTYPE[w.scales.dtype], _DTYPE[out.dtype], act, 0), device)
+    return out
+
+
+def q4_matmul(x, w, bias=None, out_dtype=None, out=None):
+    """x [M, K] fp16 or bf16, rows of any stride, times the transposed 4-bit
+    weights (q4_weights): [M, N] of x's dtype or, with out_dtype=float32, fp32. bias
+    [N] is of x's dtype. Products are summed in fp32 and multiplied there by their
+    group's scale; the result is rounded once. For few rows the weights are read
+    once; for many, matmul over weights of 16 bits is faster. A row of x that holds
+    an infinity or NaN gives no numbers."""
+    r = _fast("q4_matmul", x, w, bias, -1 if out_dtype is None else _DTYPE.get(out_dtype, -2), out)
+    if r is not None:
+        return r
+    device, M = _q4("q4_matmul", x, w, False, {"bias": bias, "out": out})
+    N = w.outputs
+    if bias is not None:
+        _shape("q4_matmul", "bias", bias, (N,), x.dtype)
+        if N > 1 and bias.stride(0) != 1:
+            raise ValueError("q4_matmul: bias needs unit stride")
+    out_dtype = x.dtype if out_dtype is None else out_dtype
+    if out_dtype != x.dtype and out_dtype != torch.float32:
+        raise TypeError(f"q4_matmul: no {out_dtype} output of {x.dtype}")
+    if out is None:
+        out = torch.empty((M, N), dtype=out_dtype, device=x.device)
+    else:
+        _shape("q4_matmul", "out", out, (M, N), out_dtype)
+    return _q4_call("q4_matmul", x, w, bias, out, 0, device)
+
+
+_ACTS = {"silu": 1, "gelu": 2}
+
+
+def q4_gated(x, w, act="silu", out=None):
+    """act(x Wg) * (x Wu) [M, F] in x's dtype, the first half of a gated feed-forward
+    block: x [M, K] fp16 or bf16, w of q4_weights(..., gated=True) with the 2 F rows
+    of Wg and Wu transposed. act is silu, v / (1 + e^-v), or gelu, v (1 + erf(v / sqrt
+    2)) / 2. Both products stay in fp32 until the result is rounded; x as in
+    q4_matmul."""
+    r = _fast("q4_gated", x, w, act, out)
+    if r is not None:
+        return r
+    device, M = _q4("q4_gated", x, w, True, {"out": out})
+    if act not in _ACTS:
+        raise ValueError(f"q4_gated: act={act!r} is not one of {tuple(_ACTS)}")
+    if out is None:
+        out = torch.empty((M, w.outputs), dtype=x.dtype, device=x.device)
+    else:
+        _shape("q4_gated", "out", out, (M, w.outputs), x.dtype)
+    return _q4_call("q4_gated", x, w, None, out, _ACTS[act], device)
+
+
+# ---------------------------------------------------------------------------
+# the next token
+# ---------------------------------------------------------------------------
+def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """ids [T] int64: of each row of logits [T, V] fp32, fp16 or bf16 (rows of any
+    stride) a token, chosen by u [T] fp32, random numbers in [0, 1) that the caller
+    draws.
+
+    A token's weight is e^((logit - largest) / temperature). Kept are the top_k
+    largest (0: all); of these the first, from the largest on, until they have
+    top_p of the weight that top_k leaves (1: all; the first one always); of these
+    the ones of weight min_p or more. Equal logits go by the lowest id. The choice
+    is the first id, in the vocabulary's order, whose running sum of kept weights
+    exceeds u times their sum; with a temperature of 0 the largest logit's. Weights
+    below 2^-46 (for more than 2^17 tokens 2^(bits of V - 63)) count as 0.
+
+    temperature, top_p and min_p are numbers, taken as fp32, or fp32 [T], top_k an
+    int or int32 [T]: settings of each row's own. -1 stands for no token: a row
+    that holds a NaN or +inf or nothing but -inf, or whose u or setting is NaN, or
+    its temperature negative or infinite."""
+    r = _fast("sample", logits, u, temperature, top_k, top_p, min_p)
+    if r is not None:
+        return r
+    device = _Dev.device()
+    settings = {"temperature": temperature, "top_k": top_k, "top_p": top_p, "min_p": min_p}
+    rows = {name: v for name, v in settings.items() if isinstance(v, torch.Tensor)}
+    _tensors("sample", device, logits=logits, u=u, **rows)
+    if logits.dim() != 2 or not 0 < logits.shape[1] < 2 ** 30:
+        raise ValueError(f"sample: logits have shape {tuple(logits.shape)}, not [T, V]")
+    if logits.dtype not in _DTYPE or logits.dtype == E4M3:
+        raise TypeError(f"sample: logits are {logits.dtype}")
+    T, V = logits.shape
+    _shape("sample", "u", u, (T,), torch.float32)
+    for name, v in rows.items():
+        _shape("sample", name, v, (T,), torch.int32 if name == "top_k" else torch.float32)
+    if T > 1 and any(t.stride(0) != 1 for t in (u, *rows.values())):
+        raise ValueError("sample: u and the rows' settings need unit stride")
+    if V > 1 and logits.stride(1) != 1:
+        raise ValueError("sample: rows of logits need unit stride")
+    if "top_k" not in rows:
+        _whole("sample", "top_k", top_k, 0)
+    for name, most in (("temperature", math.inf), ("top_p", math.inf), ("min_p", 1.0)):
+        if name not in rows:
+            if isinstance(settings[name], bool) or not isinstance(settings[name], (int, float)):
+                raise TypeError(f"sample: {name} must be a number or a tensor")
+            v = settings[name] = _fp32(settings[name])
+            if not 0.0 <= v <= most or (name == "temperature" and v == math.inf):
+                raise ValueError(f"sample: {name}={v} is out of range")
+    ids = torch.empty(T, dtype=torch.int64, device=logits.device)
+    L = lib()
+    code = _DTYPE[logits.dtype]
+    need = L.newt_sample_workspace(T, V, code)
+    workspace = torch.empty(need, dtype=torch.uint8, device=logits.device) if need else None
+    scalar = {name: 0 if name in rows else v for name, v in settings.items()}
+    _call(L.newt_sample, "sample", _SAMPLE.pack(
+        logits.data_ptr(), u.data_ptr(), ids.data_ptr(), *(_ptr(rows.get(n)) for n in settings),
+        _ptr(workspace), T, V, logits.stride(0), scalar["temperature"], scalar["top_p"],
+        scalar["min_p"], scalar["top_k"], code, 0), device)
+    return ids

@@ -33,8 +33,9 @@ Everything above is compiled by newt_amd's compiler to HIP for gfx950.
 
 Beside them stand the operators of a decoder's serving step, written by hand
 in HIP (newt_amd/serving.py): rmsnorm with the residual's addition and an 8-bit
-output, window_attention, the 8-bit cache with kv_append and cached_attention,
-and token_logprobs.
+output, q4_matmul and q4_gated over 4-bit weights, rotate for rotary positions,
+window_attention, the 8-bit cache with kv_append and cached_attention,
+token_logprobs and sample.
 """
 
 import functools
@@ -44,7 +45,8 @@ import torch
 import newt_amd as newt
 import newt_amd.language as nl
 
-from .serving import (KVCache, cached_attention, kv_append, kv_cache, rmsnorm,  # noqa: F401
+from .serving import (KVCache, Q4Weights, Rotary, cached_attention, kv_append,  # noqa: F401
+                      kv_cache, q4_gated, q4_matmul, q4_weights, rmsnorm, rotary, rotate, sample,
                       token_logprobs, window_attention)
 
 
