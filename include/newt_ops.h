@@ -183,16 +183,18 @@ int newt_rotate(const newt_rotate_params* p, void* stream);
 typedef struct {
   const void* x;            /* [rows, cols] of dtype, F16 or BF16 */
   const void* q;            /* weights, aligned to 16 bytes */
-  const void* scales;       /* of scale_dtype, F16 or BF16, aligned to 8 bytes */
-  const void* zeros;        /* bytes 0..15, aligned to 4 bytes, or NULL: 8 */
+  const void* scales;       /* of scale_dtype, F16 or BF16, aligned to 16 bytes */
+  const void* zeros;        /* bytes 0..15, aligned to 16 bytes, or NULL: 8 */
   const void* bias;         /* [outputs] of dtype, or NULL */
   void* out;                /* [rows, outputs] of out_dtype: dtype or F32 */
+  void* workspace;          /* newt_q4_matmul_workspace() bytes, or NULL if that is 0 */
   int64_t rows, cols, outputs;
   int64_t x_stride, out_stride;
   int32_t group;            /* 32, 64 or 128; divides cols */
   int32_t dtype, scale_dtype, out_dtype, act, reserved;
 } newt_q4_params;
 int newt_q4_matmul(const newt_q4_params* p, void* stream);
+size_t newt_q4_matmul_workspace(const newt_q4_params* p);
 
 /* The next token of each row of logits. A token's weight is e^((logit - the
  * row's largest) / temperature). Kept are the top_k of the largest logits (0 or

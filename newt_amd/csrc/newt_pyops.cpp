@@ -439,6 +439,11 @@ PyObject* q4_run(newt_q4_params* p, const Arg& x, const Arg& given, at::ScalarTy
   p->out = out.data_ptr();
   p->out_stride = out.stride(0);
   p->out_dtype = code(to);
+  at::Tensor workspace;
+  if (const size_t need = newt_q4_matmul_workspace(p)) {
+    workspace = empty({static_cast<int64_t>(need)}, at::kByte, *x.t);
+    p->workspace = workspace.data_ptr();
+  }
   REQUIRE(newt_q4_matmul(p, stream) == NEWT_OK);
   return wrap(out);
 }

@@ -80,13 +80,6 @@ struct Rows {
   }
 };
 
-// Workgroups go round the 8 dies of the chip, each with an L2 of its own; this
-// gives each die a run of neighbouring programs, which share keys and values.
-__device__ __forceinline__ int by_die(int i, int n) {
-  const int die = i & 7, each = n >> 3, more = n & 7;
-  return die * each + (die < more ? die : more) + (i >> 3);
-}
-
 // Partial results of `splits` programs for `rows` rows each: accumulators
 // [unit, split, row, D], then maxima and sums [unit, split, row] each.
 struct Parts {

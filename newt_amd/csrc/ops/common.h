@@ -81,6 +81,13 @@ __device__ __forceinline__ int wave_id() {
   return __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
 }
 
+// Workgroups go round the 8 dies of the chip, each with an L2 of its own; this
+// gives each die a run of neighbouring programs, which share keys and values.
+__device__ __forceinline__ int by_die(int i, int n) {
+  const int die = i & 7, each = n >> 3, more = n & 7;
+  return die * each + (die < more ? die : more) + (i >> 3);
+}
+
 // Four floats to four e4m3 bytes, rounded to nearest even by the hardware.
 __device__ __forceinline__ u32 to_e4m3x4(float a, float b, float c, float d) {
   int w = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);

@@ -1,0 +1,63 @@
+// What the products with 4-bit weights share: from a word of weights to an operand
+// of the matrix unit, and from sums to outputs.
+#pragma once
+#include "common.h"
+
+namespace newt_ops {
+
+template <typename T> struct frag;
+template <> struct frag<bf16> { typedef bf16x8 type; };
+template <> struct frag<f16> { typedef f16x8 type; };
+
+// 8 weights to (16 + q) / 16: the 4 bits go below the point of a number in [1, 2)
+template <typename T>
+__device__ __forceinline__ typename frag<T>::type widen(u32 w) {
+  u32x4 r;
+  if constexpr (__is_same(T, bf16)) {  // the 4 upper of 7 bits
+    const u32 mask = 0x00780078, one = 0x3f803f80;
+    r[0] = (w & mask) | one;
+    r[1] = ((w >> 4) & mask) | one;
+    r[2] = ((w >> 8) & mask) | one;
+    r[3] = (__builtin_amdgcn_alignbit(w, w, 12) & mask) | one;
+  } else {  // of 10 bits
+    const u32 mask = 0x03c003c0, one = 0x3c003c00;
+    r[0] = ((w << 3) & mask) | one;
+    r[1] = ((w >> 1) & mask) | one;
+    r[2] = ((w >> 5) & mask) | one;
+    r[3] = (__builtin_amdgcn_alignbit(w, w, 9) & mask) | one;
+  }
+  return __builtin_bit_cast(typename frag<T>::type, r);
+}
+
+__device__ __forceinline__ float activate(float v, int act) {
+  if (act == NEWT_ACT_SILU) return v / (1.0f + __builtin_expf(-v));
+  return 0.5f * v * (1.0f + erff(v * 0.70710678f));
+}
+
+// 4 neighbouring outputs of a row from `first` on.
+template <typename T>
+__device__ __forceinline__ void store4(const newt_q4_params& p, int64_t row, int64_t first, f32x4 y) {
+  const int count = p.outputs - first < 4 ? (int)(p.outputs - first) : 4;
+  if (p.bias) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i < count) y[i] += newt::to_f32(((const T*)p.bias)[first + i]);
+  }
+  if (p.out_dtype == NEWT_F32) {
+    float* out = (float*)p.out + row * p.out_stride + first;
+    const float t[4] = {y[0], y[1], y[2], y[3]};
+    if (count == 4) newt::store_vec<float, 4>(out, t, newt::any_align());
+    else for (int i = 0; i < count; ++i) out[i] = t[i];
+  } else {
+    T* out = (T*)p.out + row * p.out_stride + first;
+    const T t[4] = {(T)y[0], (T)y[1], (T)y[2], (T)y[3]};
+    if (count == 4) newt::store_vec<T, 4>(out, t, newt::any_align());
+    else for (int i = 0; i < count; ++i) out[i] = t[i];
+  }
+}
+
+// q4_many.hip: products with many rows of x.
+size_t q4_many_workspace(const newt_q4_params& p);
+int q4_many(const newt_q4_params& p, hipStream_t stream);
+
+}  // namespace newt_ops

@@ -10,39 +10,10 @@
 //   sum_k x (q - z) = 16 (sum_k x (16 + q) / 16 - (16 + z) / 16 sum_k x)
 // A wave takes NT tiles of 16 weight rows, MT tiles of 16 rows of x and every
 // WAVES-th block of 128 columns; the waves' sums are joined in LDS.
-#include "common.h"
+#include "q4.h"
 
 namespace newt_ops {
 namespace {
-
-template <typename T> struct frag;
-template <> struct frag<bf16> { typedef bf16x8 type; };
-template <> struct frag<f16> { typedef f16x8 type; };
-
-// 8 weights to (16 + q) / 16
-template <typename T>
-__device__ __forceinline__ typename frag<T>::type widen(u32 w) {
-  u32x4 r;
-  if constexpr (__is_same(T, bf16)) {  // the 4 upper of 7 bits
-    const u32 mask = 0x00780078, one = 0x3f803f80;
-    r[0] = (w & mask) | one;
-    r[1] = ((w >> 4) & mask) | one;
-    r[2] = ((w >> 8) & mask) | one;
-    r[3] = (__builtin_amdgcn_alignbit(w, w, 12) & mask) | one;
-  } else {  // of 10 bits
-    const u32 mask = 0x03c003c0, one = 0x3c003c00;
-    r[0] = ((w << 3) & mask) | one;
-    r[1] = ((w >> 1) & mask) | one;
-    r[2] = ((w >> 5) & mask) | one;
-    r[3] = (__builtin_amdgcn_alignbit(w, w, 9) & mask) | one;
-  }
-  return __builtin_bit_cast(typename frag<T>::type, r);
-}
-
-__device__ __forceinline__ float activate(float v, int act) {
-  if (act == NEWT_ACT_SILU) return v / (1.0f + __builtin_expf(-v));
-  return 0.5f * v * (1.0f + erff(v * 0.70710678f));
-}
 
 template <typename T, int NT, int MT, int WAVES, int GROUP, bool GATED>
 __global__ void __launch_bounds__(64 * WAVES)
@@ -168,20 +139,7 @@ q4_kernel(newt_q4_params p, int n_blocks) {
     } else {
       y = joined(n, m, l);
     }
-    const int count = p.outputs - first < 4 ? (int)(p.outputs - first) : 4;
-    if (!GATED && p.bias)
-      for (int i = 0; i < count; ++i) y[i] += newt::to_f32(((const T*)p.bias)[first + i]);
-    if (p.out_dtype == NEWT_F32) {
-      float* out = (float*)p.out + row * p.out_stride + first;
-      const float t[4] = {y[0], y[1], y[2], y[3]};
-      if (count == 4) newt::store_vec<float, 4>(out, t, newt::any_align());
-      else for (int i = 0; i < count; ++i) out[i] = y[i];
-    } else {
-      T* out = (T*)p.out + row * p.out_stride + first;
-      const T t[4] = {(T)y[0], (T)y[1], (T)y[2], (T)y[3]};
-      if (count == 4) newt::store_vec<T, 4>(out, t, newt::any_align());
-      else for (int i = 0; i < count; ++i) out[i] = (T)y[i];
-    }
+    store4<T>(p, row, first, y);
   }
 }
 
@@ -200,7 +158,9 @@ int launch(const newt_q4_params& p, hipStream_t stream) {
   go(std::integral_constant<int, NT>(), std::integral_constant<int, MT>(),             \
      std::integral_constant<int, WAVES>())
   if (p.rows <= 16) return NEWT_TILE(2, 1, 8);
-  return NEWT_TILE(4, 4, 2);
+  if (p.rows <= 32) return NEWT_TILE(2, 2, 8);
+  if (p.rows <= 48) return NEWT_TILE(2, 3, 8);
+  return NEWT_TILE(2, 4, 8);
 #undef NEWT_TILE
 }
 
@@ -217,6 +177,8 @@ template <typename T>
 int by_act(const newt_q4_params& p, hipStream_t stream) {
   return p.act == NEWT_ACT_NONE ? by_group<T, false>(p, stream) : by_group<T, true>(p, stream);
 }
+
+constexpr int64_t kFewRows = 64;
 
 const char* wrong(const newt_q4_params& p) {
   if (p.rows < 0 || p.outputs < 0 || p.cols <= 0) return "bad size";
@@ -236,6 +198,12 @@ const char* wrong(const newt_q4_params& p) {
 }  // namespace
 }  // namespace newt_ops
 
+extern "C" size_t newt_q4_matmul_workspace(const newt_q4_params* p) {
+  using namespace newt_ops;
+  if (!p || wrong(*p) || p->rows <= kFewRows || p->outputs == 0) return 0;
+  return q4_many_workspace(*p);
+}
+
 extern "C" int newt_q4_matmul(const newt_q4_params* params, void* stream) {
   using namespace newt_ops;
   if (!params) return fail(NEWT_ERR_INVALID, "newt_q4_matmul: null params");
@@ -244,8 +212,9 @@ extern "C" int newt_q4_matmul(const newt_q4_params* params, void* stream) {
   if (p.rows == 0 || p.outputs == 0) return NEWT_OK;
   if (!p.x || !p.q || !p.scales || !p.out)
     return fail(NEWT_ERR_INVALID, "newt_q4_matmul: null tensor");
-  if (((uintptr_t)p.q & 15) | ((uintptr_t)p.scales & 7) | ((uintptr_t)p.zeros & 3))
+  if (((uintptr_t)p.q | (uintptr_t)p.scales | (uintptr_t)p.zeros) & 15)
     return fail(NEWT_ERR_INVALID, "newt_q4_matmul: weights are not aligned");
   hipStream_t s = static_cast<hipStream_t>(stream);
+  if (p.rows > kFewRows) return q4_many(p, s);
   return p.dtype == NEWT_F16 ? by_act<f16>(p, s) : by_act<bf16>(p, s);
 }

@@ -55,7 +55,7 @@ _APPEND = struct.Struct("=" + _CACHE + "5Q10q2i")
 _CACHED = struct.Struct("=" + _CACHE + "5Q12qf3i")
 _WINDOW = struct.Struct("=6Q17qf5i")
 _ROTATE = struct.Struct("=6Q20qf5i")
-_Q4 = struct.Struct("=6Q5q6i")
+_Q4 = struct.Struct("=7Q5q6i")
 _SAMPLE = struct.Struct("=8Q3q3f3i")
 
 
@@ -72,7 +72,8 @@ def lib():
                  "newt_window_attention", "newt_rotate", "newt_q4_matmul", "newt_sample"):
         f = getattr(L, name)
         f.restype, f.argtypes = ctypes.c_int, [ctypes.c_char_p, ctypes.c_void_p]
-    for name in ("newt_cached_attention_workspace", "newt_window_attention_workspace"):
+    for name in ("newt_cached_attention_workspace", "newt_window_attention_workspace",
+                 "newt_q4_matmul_workspace"):
         f = getattr(L, name)
         f.restype, f.argtypes = ctypes.c_size_t, [ctypes.c_char_p]
     L.newt_token_logprobs_workspace.restype = ctypes.c_size_t
@@ -567,7 +568,9 @@ def rotary(dim, base=10000.0, factor=1.0, ramp=None, amplitude=1.0, interleaved=
     # a fraction of a turn to 64 bits, whatever its size, needs more than fp64
     with decimal.localcontext(decimal.Context(prec=60)):
         if frequencies is None:
-            frequencies = [number(base) ** (number(-2 * i) / dim) for i in range(dim // 2)]
+            step, frequencies = number(base) ** (number(-2) / dim), [number(1)]
+            while len(frequencies) < dim // 2:
+                frequencies.append(frequencies[-1] * step)
         else:
             frequencies = [float(f) for f in frequencies]
             if len(frequencies) != dim // 2 or not all(math.isfinite(f) for f in frequencies):
@@ -758,10 +761,17 @@ def _q4_call(what, x, w, bias, out, act, device):
         raise ValueError(f"{what}: rows of out need unit stride")
     if M > 1 and out.stride(0) < N:
         raise ValueError(f"{what}: rows of out overlap")
-    _call(lib().newt_q4_matmul, what, _Q4.pack(
-        x.data_ptr(), w.q.data_ptr(), w.scales.data_ptr(), _ptr(w.zeros), _ptr(bias),
-        out.data_ptr(), M, w.cols, N, x.stride(0), out.stride(0), w.group, _DTYPE[x.dtype],
-        _DTYPE[w.scales.dtype], _DTYPE[out.dtype], act, 0), device)
+    L = lib()
+    pointers = (x.data_ptr(), w.q.data_ptr(), w.scales.data_ptr(), _ptr(w.zeros), _ptr(bias),
+                out.data_ptr())
+    rest = (M, w.cols, N, x.stride(0), out.stride(0), w.group, _DTYPE[x.dtype],
+            _DTYPE[w.scales.dtype], _DTYPE[out.dtype], act, 0)
+    params = _Q4.pack(*pointers, 0, *rest)
+    need = L.newt_q4_matmul_workspace(params)
+    if need:
+        workspace = torch.empty(need, dtype=torch.uint8, device=x.device)
+        params = _Q4.pack(*pointers, workspace.data_ptr(), *rest)
+    _call(L.newt_q4_matmul, what, params, device)
     return out
 
 
