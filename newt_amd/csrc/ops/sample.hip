@@ -39,13 +39,6 @@ __device__ __forceinline__ u64 place_of(float x, u32 id) {
   return ((u64)~key_of(x) << 32) | id;
 }
 
-template <typename V>
-__device__ __forceinline__ V wave_sum(V v) {
-#pragma unroll
-  for (int m = 1; m < 64; m <<= 1) v += __shfl_xor(v, m);
-  return v;
-}
-
 // The sum over this lane and those below it.
 template <typename V>
 __device__ __forceinline__ V wave_scan(V v, int lane) {
@@ -148,16 +141,40 @@ struct Row {
   }
   __device__ __forceinline__ u64 weight(float f) const { return weight(point(f)); }
 
-  // f(number, id) for each of the row, in no order
-  template <typename F>
-  __device__ __forceinline__ void each(F f) const {
-    for (int c = wave; c < chunks; c += kWaves) {
+  // f(number, id) for each of the row, in no order, and done(chunk) behind each
+  // chunk: a wave loads four chunks, then works on them.
+  template <typename F, typename D>
+  __device__ __forceinline__ void each(F f, D done) const {
+    constexpr int AHEAD = 4;
+    const int whole = vocab / CHUNK;
+    for (int c = wave; c < whole; c += kWaves * AHEAD) {
+      T t[AHEAD][V];
+#pragma unroll
+      for (int a = 0; a < AHEAD; ++a) {
+        const int at = c + a * kWaves < whole ? c + a * kWaves : whole - 1;
+        newt::load_vec<T, V>(x + (int64_t)at * CHUNK + lane * V, t[a], newt::any_align());
+      }
+#pragma unroll
+      for (int a = 0; a < AHEAD; ++a) {
+        if (c + a * kWaves >= whole) break;
+        const int64_t i = (int64_t)(c + a * kWaves) * CHUNK + lane * V;
+#pragma unroll
+        for (int j = 0; j < V; ++j) f(newt::to_f32(t[a][j]), i + j);
+        done(c + a * kWaves);
+      }
+    }
+    if (whole < chunks && whole % kWaves == wave) {
       float v[V];
-      const int64_t i = (int64_t)c * CHUNK + lane * V;
+      const int64_t i = (int64_t)whole * CHUNK + lane * V;
       load(i, v);
 #pragma unroll
       for (int j = 0; j < V; ++j) f(v[j], i + j);
+      done(whole);
     }
+  }
+  template <typename F>
+  __device__ __forceinline__ void each(F f) const {
+    each(f, [](int) {});
   }
 
   __device__ __forceinline__ void clear() const {
@@ -210,7 +227,7 @@ struct Row {
 
   // The mass of all bins.
   __device__ __forceinline__ u64 total() const {
-    const u64 m = wave_sum(s.mass[2 * threadIdx.x] + s.mass[2 * threadIdx.x + 1]);
+    const u64 m = newt::lane_reduce<newt::Sum, 63>(s.mass[2 * threadIdx.x] + s.mass[2 * threadIdx.x + 1]);
     if (lane == 0) s.part[wave] = m;
     __syncthreads();
     u64 sum = 0;
@@ -273,20 +290,15 @@ struct Row {
   template <typename F>
   __device__ __forceinline__ void segments(F f) const {
     const int per = (chunks + kBins - 1) / kBins;
-    const int count = (chunks + per - 1) / per;
-    for (int g = wave; g < count; g += kWaves) {
-      u64 sum = 0;
-      for (int c = g * per; c < chunks && c < (g + 1) * per; ++c) {
-        float v[V];
-        const int64_t i = (int64_t)c * CHUNK + lane * V;
-        load(i, v);
-#pragma unroll
-        for (int j = 0; j < V; ++j) sum += f(v[j], i + j);
-      }
-      sum = wave_sum(sum);
-      if (lane == 0) s.mass[g] = sum;
-    }
-    for (int g = count + threadIdx.x; g < kBins; g += kThreads) s.mass[g] = 0;
+    for (int g = threadIdx.x; g < kBins; g += kThreads) s.mass[g] = 0;
+    __syncthreads();
+    u64 sum = 0;
+    each([&](float v, int64_t i) { sum += f(v, i); }, [&](int c) {
+      sum = newt::lane_reduce<newt::Sum, 63>(sum);
+      if (per == 1) s.mass[c] = sum;
+      else if (lane == 0) atomicAdd(&s.mass[c / per], sum);
+      sum = 0;
+    });
     __syncthreads();
   }
   __device__ __forceinline__ int segment_of(int64_t id) const {
