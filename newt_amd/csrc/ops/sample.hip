@@ -20,6 +20,7 @@ namespace {
 constexpr int kThreads = 1024, kWaves = kThreads / 64;
 constexpr int kBins = 2048;
 constexpr int kList = 4096;
+constexpr int kMostParts = 64;
 constexpr float kInf = __builtin_inff();
 constexpr u32 kNone = 0xffffffffu;
 
@@ -54,18 +55,42 @@ struct Shared {
   double table[kBins];  // 2^shift e^(-i / 64)
   u64 mass[kBins];      // a histogram's masses, a search's segments
   u32 count[kBins];
-  u64 list[kList];
+  u64 list[kList];      // places of tokens
+  u64 some[kList];      // those of one bin
   u64 part[kWaves];
   u32 part_count[kWaves];
   float top[kWaves];
   int bad[kWaves];
-  u32 listed;
+  u32 listed, picked, first;
   u64 last;
+  double edge;  // the table's entry of the bin at the end
   // what a search found
   u64 before;
   u32 before_count, place, place_count;
   u64 place_mass;
 };
+
+// A row's settings.
+struct Settings {
+  float temperature, top_p, min_p, u;
+  u32 top_k;
+  bool bad, greedy, by_count, by_mass;
+  __device__ __forceinline__ Settings(const newt_sample_params& p, int64_t r)
+      : temperature(p.temperature ? p.temperature[r] : p.temperature_all),
+        top_p(p.top_p ? p.top_p[r] : p.top_p_all),
+        min_p(p.min_p ? p.min_p[r] : p.min_p_all), u(p.u[r]) {
+    const int k = p.top_k ? p.top_k[r] : p.top_k_all;
+    top_k = (u32)k;
+    bad = !(temperature >= 0.0f && temperature < kInf) | (u != u) | (top_p != top_p) |
+          (min_p != min_p);
+    greedy = (temperature == 0.0f) | (k == 1);
+    by_count = (k > 0) & (k < p.vocab);
+    by_mass = top_p < 1.0f;
+  }
+};
+
+// What is read of a row behind the histogram, and how the kept ones are found.
+enum Mode { kSums, kListed, kSlow };
 
 template <typename T>
 struct Row {
@@ -73,11 +98,23 @@ struct Row {
   static constexpr int CHUNK = 64 * V;  // of a wave
   const T* x;
   int vocab, chunks, shift;
+  int from, to;  // the chunks that are this program's
   int lane, wave;
   Shared& s;
-  float top;   // the largest logit
-  double by;   // 64 / T
-  u64 least;   // the smallest weight that min_p keeps
+  float top;     // the largest logit
+  double by;     // 64 / T
+  double reach;  // 64 ln(1 / min_p): of (max - x) 64 / T
+
+  __device__ __forceinline__ Row(const newt_sample_params& p, Shared& s_, int64_t r, int shift_)
+      : x((const T*)p.logits + r * p.stride), vocab((int)p.vocab),
+        chunks((int)((p.vocab + CHUNK - 1) / CHUNK)), shift(shift_), from(0), to(chunks),
+        lane(threadIdx.x & 63), wave(wave_id()), s(s_) {}
+  __device__ __forceinline__ void set(const Settings& o, float top_) {
+    top = top_;
+    by = 64.0 / (double)o.temperature;
+    // 2^-46 less of a weight, as little as it is rounded by, still reaches min_p
+    reach = o.min_p > 0.0f ? 0x1p-40 - 64.0 * log((double)__builtin_fminf(o.min_p, 1.0f)) : 1e300;
+  }
 
   // V numbers from i on, -inf behind the row's end
   __device__ __forceinline__ void load(int64_t i, float* f) const {
@@ -121,23 +158,26 @@ struct Row {
   struct Point {
     double rest;
     int bin;
+    __device__ __forceinline__ bool within(double reach) const { return rest + bin <= reach; }
   };
   __device__ __forceinline__ Point point(float f) const {
     const double t = __builtin_fmin(((double)top - (double)f) * by, (double)(kBins - 1));
     const double whole = t + 6755399441055744.0;  // 1.5 2^52: the low bits are the bin
     return {t - (whole - 6755399441055744.0), (int)__builtin_bit_cast(u64, whole)};
   }
-  // The weight as a whole number: e^(-rest / 64), whose first term left out is
-  // (1 / 128)^6 / 6!, 2^-51, times the table's, rounded by 2^52 more.
+  // e^(-rest / 64), off by 2^-45 of it, times the table's entry, rounded to a whole
+  // number by 2^52 more: its low 52 bits.
+  __device__ __forceinline__ static u64 weight_bits(double rest, double entry) {
+    double e = 2.483531912468741e-09;
+    e = __builtin_fma(e, rest, -6.357848178607495e-07);
+    e = __builtin_fma(e, rest, 1.2207031249984305e-04);
+    e = __builtin_fma(e, rest, -0.015624999999939368);
+    e = __builtin_fma(e, rest, 1.0);
+    return __builtin_bit_cast(u64, __builtin_fma(e, entry, 4503599627370496.0));
+  }
+  static constexpr u64 kWhole = 0x4330000000000000ull;  // the bits of 2^52
   __device__ __forceinline__ u64 weight(const Point& a) const {
-    double e = -7.76102145512898763e-12;  // -1 / 64^5 / 5!
-    e = __builtin_fma(e, a.rest, 2.48352686564127604e-9);
-    e = __builtin_fma(e, a.rest, -6.35782877604166667e-7);
-    e = __builtin_fma(e, a.rest, 1.220703125e-4);
-    e = __builtin_fma(e, a.rest, -0.015625);
-    e = __builtin_fma(e, a.rest, 1.0);
-    const double whole = __builtin_fma(e, s.table[a.bin], 4503599627370496.0);
-    return __builtin_bit_cast(u64, whole) & 0xfffffffffffffull;
+    return weight_bits(a.rest, s.table[a.bin]) & 0xfffffffffffffull;
   }
   __device__ __forceinline__ u64 weight(float f) const { return weight(point(f)); }
 
@@ -146,8 +186,8 @@ struct Row {
   template <typename F, typename D>
   __device__ __forceinline__ void each(F f, D done) const {
     constexpr int AHEAD = 4;
-    const int whole = vocab / CHUNK;
-    for (int c = wave; c < whole; c += kWaves * AHEAD) {
+    const int whole = to < vocab / CHUNK ? to : vocab / CHUNK;
+    for (int c = from + wave; c < whole; c += kWaves * AHEAD) {
       T t[AHEAD][V];
 #pragma unroll
       for (int a = 0; a < AHEAD; ++a) {
@@ -163,7 +203,7 @@ struct Row {
         done(c + a * kWaves);
       }
     }
-    if (whole < chunks && whole % kWaves == wave) {
+    if (from <= whole && whole < to && wave == kWaves - 1) {
       float v[V];
       const int64_t i = (int64_t)whole * CHUNK + lane * V;
       load(i, v);
@@ -253,36 +293,81 @@ struct Row {
       }
     __syncthreads();
   }
-  // Rounds the list up to a power of two with entries behind all others.
-  __device__ __forceinline__ int fill_up(int n) const {
-    int size = 64;
+  // The first n of `some` in rising order: by counting for few, else bitonic.
+  __device__ __forceinline__ void order(int n) const {
+    if (n <= 256) {
+      const int i = threadIdx.x;
+      u64 own = 0;
+      int rank = 0;
+      if (i < n) {
+        own = s.some[i];
+        for (int j = 0; j < n; ++j) rank += s.some[j] < own;
+      }
+      __syncthreads();
+      if (i < n) s.some[rank] = own;
+      __syncthreads();
+      return;
+    }
+    int size = 512;
     while (size < n) size <<= 1;
-    for (int i = n + threadIdx.x; i < size; i += kThreads) s.list[i] = ~0ull;
-    return size;
-  }
-  // Sums of w over the list's entries before this thread's first, 4 neighbouring
-  // ones a thread.
-  __device__ __forceinline__ u64 scan(const u64 (&w)[4], u64* sum) const {
-    const u64 own = w[0] + w[1] + w[2] + w[3];
-    u64 m = wave_scan(own, lane);
-    if (lane == 63) s.part[wave] = m;
+    for (int i = n + threadIdx.x; i < size; i += kThreads) s.some[i] = ~0ull;
+    for (int k = 2; k <= size; k <<= 1)
+      for (int j = k >> 1; j > 0; j >>= 1) {
+        __syncthreads();
+        for (int i = threadIdx.x; i < size / 2; i += kThreads) {
+          const int a = 2 * i - (i & (j - 1)), b = a + j;
+          const u64 u = s.some[a], v = s.some[b];
+          if ((u > v) == ((a & k) == 0)) {
+            s.some[a] = v;
+            s.some[b] = u;
+          }
+        }
+      }
     __syncthreads();
-    u64 all = 0;
-#pragma unroll
-    for (int i = 0; i < kWaves; ++i) {
-      if (i == wave) m += all;
-      all += s.part[i];
+  }
+  __device__ __forceinline__ static float logit_of(u64 place) {
+    return of_key(~(u32)(place >> 32));
+  }
+  __device__ __forceinline__ void append(u64 place) const {
+    const u32 i = atomicAdd(&s.listed, 1u);
+    if (i < kList) s.list[i] = place;
+  }
+  // Moves the list's entries for which f(place) holds to `some`, and counts them.
+  template <typename F>
+  __device__ __forceinline__ int take(int n, F f) const {
+    if (threadIdx.x == 0) s.picked = 0;
+    __syncthreads();
+    for (int i = threadIdx.x; i < n; i += kThreads) {
+      const u64 place = s.list[i];
+      if (f(place)) s.some[atomicAdd(&s.picked, 1u)] = place;
     }
     __syncthreads();
-    *sum = all;
-    return m - own;
+    return (int)s.picked;
   }
-  __device__ __forceinline__ void append(u64 entry) const {
-    const u32 i = atomicAdd(&s.listed, 1u);
-    if (i < kList) s.list[i] = entry;
-  }
-  __device__ __forceinline__ u64 listed_weight(int i, int n) const {
-    return i < n ? weight(of_key(~(u32)(s.list[i] >> 32))) : 0;
+  // The last of `some`, n in order, before which less than the target lies, with
+  // `before` in front of them all: 0 for none. All have the table entry `entry`.
+  __device__ __forceinline__ u64 last_by_mass(int n, u64 before, double target,
+                                              double entry) const {
+    if (threadIdx.x == 0) s.last = 0;
+    const int i = 4 * threadIdx.x;
+    u64 w[4], own = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      w[j] = i + j < n ? weight_bits(point(logit_of(s.some[i + j])).rest, entry) - kWhole : 0;
+      own += w[j];
+    }
+    u64 run = wave_scan(own, lane);
+    if (lane == 63) s.part[wave] = run;
+    __syncthreads();
+    run += before - own;
+    for (int a = 0; a < wave; ++a) run += s.part[a];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (i + j < n && (double)run < target) atomicMax(&s.last, s.some[i + j]);
+      run += w[j];
+    }
+    __syncthreads();
+    return s.last;
   }
 
   // The sums of f(number, id), in segments of consecutive chunks that `find`
@@ -449,216 +534,442 @@ struct Row {
     }
   }
 
-  __device__ __forceinline__ u64 kept_weight(float f, int64_t i, u64 cut) const {
-    if (place_of(f, (u32)i) > cut) return 0;
-    const u64 w = weight(f);
-    return w >= least ? w : 0;
-  }
   // A number below `sum`, u of it.
   __device__ __forceinline__ static u64 share(float u, u64 sum) {
     const u64 r = (u64)((double)__builtin_fmaxf(u, 0.0f) * (double)sum);
     return r < sum ? r : sum - 1;
   }
 
-  // The choice among tokens up to the place `cut`, whose weights the segments
-  // hold. One wave's lanes return it.
-  __device__ __forceinline__ int choose(float u, u64 cut) const {
-    const u64 sum = total();
-    if (wave != 0) return 0;
-    return find(share(u, sum), [&](float f, int64_t i) { return kept_weight(f, i, cut); });
+  // The steps, each of all threads of a program, with a barrier at their ends.
+
+  // The largest logit, and whether one is a NaN.
+  __device__ __forceinline__ float largest(bool& bad) const {
+    float most = -kInf;
+    bool nan = false;
+    each([&](float f, int64_t) {
+      most = __builtin_fmaxf(most, f);
+      nan |= f != f;
+    });
+    most = newt::lane_reduce<newt::Max, 63>(most);
+    nan = __ballot(nan) != 0;
+    if (lane == 0) {
+      s.top[wave] = most;
+      s.bad[wave] = nan;
+    }
+    if (threadIdx.x == 0) {
+      s.listed = 0;
+      s.first = 0xffffffffu;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      most = __builtin_fmaxf(most, s.top[w]);
+      nan |= s.bad[w] != 0;
+    }
+    bad = nan;
+    return most;
   }
 
-  // The choice where the list holds all tokens that top_k may keep.
-  __device__ __forceinline__ int choose_listed(int n, u32 k, float top_p, float u) const {
-    const int size = fill_up(n);
-    sort(size);
-    const int i = 4 * threadIdx.x;
-    u64 w[4], of_k[4], sum, mass;
-    u32 id[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      w[j] = listed_weight(i + j, n);
-      of_k[j] = i + j < k ? w[j] : 0;
-      id[j] = i + j < n ? (u32)s.list[i + j] : 0;
-    }
-    u64 before = scan(of_k, &mass);
-    const double target = (double)top_p * (double)mass;
-    u64 entry[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const bool stays = (i + j < k) & ((i + j == 0) | (top_p >= 1.0f) | ((double)before < target)) &
-                         (w[j] >= least);
-      before += of_k[j];
-      // by id, with what finds the weight again
-      entry[j] = stays && i + j < n ? ((u64)id[j] << 32) | (u32)(s.list[i + j] >> 32) : ~0ull;
+  // Bins' counts, for top_k, or masses, for top_p alone.
+  __device__ __forceinline__ void histogram(const Settings& o) const {
+    clear();
+    if (o.by_count) {
+      each([&](float f, int64_t) {
+        const int b = point(f).bin;
+        if (b < kBins - 1) atomicAdd(&s.count[b], 1u);
+      });
+    } else {
+      each([&](float f, int64_t) {
+        const Point a = point(f);
+        if (a.bin < kBins - 1) atomicAdd(&s.mass[a.bin], weight(a));
+      });
     }
     __syncthreads();
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (i + j < size) s.list[i + j] = entry[j];
-    sort(size);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const u64 e = i + j < size ? s.list[i + j] : ~0ull;
-      w[j] = e != ~0ull ? weight(of_key(~(u32)e)) : 0;
+  }
+
+  // What the histogram says of the end of what is kept.
+  struct End {
+    Mode mode;
+    int bin;           // with the last one that top_k and top_p keep (kBins: no such bin)
+    int edge;          // kSums: bins before it are kept, those behind it not
+    u64 before;
+    u32 before_count;
+    double target;     // the mass at which top_p ends
+  };
+  __device__ __forceinline__ End end(const Settings& o) const {
+    End e = {kSums, kBins, kBins, 0, 0, 0.0};
+    if (o.by_count | o.by_mass) {
+      // at least the first token
+      if (!o.by_count)
+        e.target = __builtin_fmax((double)o.top_p * (double)total(), 0x1p-60);
+      pick(!o.by_count, o.top_k, 0, e.target);
+      if (s.place != kNone) {
+        e.bin = s.place;
+        e.before = s.before;
+        e.before_count = s.before_count;
+        const u32 upto = s.before_count + s.place_count;
+        if (o.by_count && upto <= kList) e.mode = kListed;
+        else if (o.by_count && (o.by_mass || s.place_count > kList)) e.mode = kSlow;
+      } else if (o.by_count && o.by_mass) {
+        e.mode = kSlow;
+      }
+      __syncthreads();
     }
-    u64 run = scan(w, &sum);
-    const u64 r = share(u, sum);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if (run <= r && run + w[j] > r) s.place = (u32)(s.list[i + j] >> 32);
-      run += w[j];
+    // bins fall with the logit: what lies before the bin of `reach` is within it
+    const int of_min = reach < kBins - 1.5 ? (int)__builtin_rint(reach) : kBins;
+    e.edge = e.bin < of_min ? e.bin : of_min;
+    return e;
+  }
+
+  // Segments' sums of what is certainly kept, and the list of what may be.
+  __device__ __forceinline__ void sums(const End& e) const {
+    // weights from the edge on come out as 0
+    if (threadIdx.x == 0 && e.edge < kBins) s.edge = s.table[e.edge];
+    __syncthreads();
+    for (int i = e.edge + threadIdx.x; i < kBins; i += kThreads) s.table[i] = 0.0;
+    for (int g = threadIdx.x; g < kBins; g += kThreads) s.mass[g] = 0;
+    __syncthreads();
+    const int per = (chunks + kBins - 1) / kBins;
+    u64 sum = 0;
+    each([&](float f, int64_t i) {
+      const Point a = point(f);
+      sum += weight_bits(a.rest, s.table[a.bin]);
+      if (a.bin == e.edge) append(place_of(f, (u32)i));
+    }, [&](int c) {
+      sum = newt::lane_reduce<newt::Sum, 63>(sum - V * kWhole);
+      if (per == 1) s.mass[c] = sum;
+      else if (lane == 0) atomicAdd(&s.mass[c / per], sum);
+      sum = 0;
+    });
+    __syncthreads();
+  }
+  // The list of all that top_k may keep.
+  __device__ __forceinline__ void candidates(const End& e) const {
+    each([&](float f, int64_t i) {
+      if (point(f).bin <= e.bin) append(place_of(f, (u32)i));
+    });
+    __syncthreads();
+  }
+  // The first id of the largest logit.
+  __device__ __forceinline__ void first() const {
+    each([&](float f, int64_t i) {
+      if (f == top) atomicMin(&s.first, (u32)i);
+    });
+    __syncthreads();
+  }
+
+  // The choice among what the segments hold, of the bins before `edge` and of places
+  // up to `cut`.
+  __device__ __forceinline__ int choose(float u, int edge, u64 cut) const {
+    const u64 sum = total();
+    if (wave != 0) return 0;
+    return find(share(u, sum), [&](float f, int64_t i) -> u64 {
+      const Point a = point(f);
+      if (a.bin < edge) return weight(a);
+      if (place_of(f, (u32)i) > cut) return 0;
+      return weight_bits(a.rest, s.edge) - kWhole;
+    });
+  }
+
+  // The choice after `sums`, whose list holds the edge's bin.
+  __device__ __forceinline__ int choose_by_sums(const Settings& o, const End& e) const {
+    const int n = (int)s.listed;
+    u64 cut = 0;
+    if (n) {
+      const int m = take(n, [&](u64 place) { return point(logit_of(place)).within(reach); });
+      if (m) {
+        // places beyond those of top_k and top_p, if their bin is the edge
+        cut = ~0ull;
+        if (e.bin == e.edge) {
+          order(m);
+          cut = o.by_count ? ((u64)m < o.top_k - e.before_count ? ~0ull
+                                                                : s.some[o.top_k - e.before_count - 1])
+                           : last_by_mass(m, e.before, e.target, s.edge);
+        }
+        if (threadIdx.x == 0) s.last = 0;
+        __syncthreads();
+        for (int i = threadIdx.x; i < m; i += kThreads) {
+          const u64 place = s.some[i];
+          if (place > cut) continue;
+          atomicAdd(&s.mass[segment_of((u32)place)],
+                    weight_bits(point(logit_of(place)).rest, s.edge) - kWhole);
+          atomicMax(&s.last, place);
+        }
+        __syncthreads();
+        cut = s.last;
+      }
+    }
+    return choose(o.u, e.edge, cut);
+  }
+
+  // The choice after `candidates`.
+  __device__ __forceinline__ int choose_listed(const Settings& o, const End& e) const {
+    const int n = (int)s.listed;
+    const auto bin_of = [&](u64 place) { return point(logit_of(place)).bin; };
+    order(take(n, [&](u64 place) { return bin_of(place) == e.bin; }));
+    u64 cut = s.some[o.top_k - e.before_count - 1];
+    __syncthreads();
+    clear();
+    if (o.by_mass) {
+      for (int i = threadIdx.x; i < n; i += kThreads) {
+        const u64 place = s.list[i];
+        const Point a = point(logit_of(place));
+        if (place <= cut) atomicAdd(&s.mass[a.bin], weight(a));
+      }
+      __syncthreads();
+      const double target = __builtin_fmax((double)o.top_p * (double)total(), 0x1p-60);
+      pick(true, 0, 0, target);
+      const u32 bin = s.place;
+      const u64 before = s.before;
+      if (bin != kNone) {
+        const int m =
+            take(n, [&](u64 place) { return (place <= cut) & ((u32)bin_of(place) == bin); });
+        order(m);
+        const u64 by_p = last_by_mass(m, before, target, s.table[bin]);
+        cut = by_p < cut ? by_p : cut;
+      }
+      __syncthreads();
+      clear();
+    }
+    for (int i = threadIdx.x; i < n; i += kThreads) {
+      const u64 place = s.list[i];
+      const Point a = point(logit_of(place));
+      if (place <= cut && a.within(reach)) atomicAdd(&s.mass[segment_of((u32)place)], weight(a));
     }
     __syncthreads();
-    return (int)s.place;
+    const u64 sum = total();
+    if (wave != 0) return 0;
+    return find(share(o.u, sum), [&](float f, int64_t i) -> u64 {
+      if (place_of(f, (u32)i) > cut) return 0;
+      const Point a = point(f);
+      return a.within(reach) ? weight(a) : 0;
+    });
+  }
+
+  // The choice where a bin holds more than a list. The table is whole.
+  __device__ __forceinline__ int choose_slowly(const Settings& o) const {
+    u64 cut = ~0ull;
+    if (o.by_count) cut = last(false, o.top_k, 0.0);
+    if (o.by_mass) {
+      segments([&](float f, int64_t i) {
+        return place_of(f, (u32)i) <= cut ? weight(f) : (u64)0;
+      });
+      const u64 by_p = last(true, 0, __builtin_fmax((double)o.top_p * (double)total(), 0x1p-60));
+      cut = by_p < cut ? by_p : cut;
+    }
+    const auto kept = [&](float f, int64_t i) -> u64 {
+      const Point a = point(f);
+      return place_of(f, (u32)i) <= cut && a.within(reach) ? weight(a) : 0;
+    };
+    segments(kept);
+    const u64 sum = total();
+    return wave == 0 ? find(share(o.u, sum), kept) : 0;
   }
 };
 
+// A row in one program.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) sample_kernel(newt_sample_params p, int shift) {
   __shared__ Shared s;
   const int64_t r = blockIdx.x;
-  const int lane = threadIdx.x & 63, wave = wave_id();
-  Row<T> row{(const T*)p.logits + r * p.stride, (int)p.vocab, 0, shift, lane, wave, s, 0, 0, 0};
-  row.chunks = (int)((p.vocab + Row<T>::CHUNK - 1) / Row<T>::CHUNK);
-  const float temperature = p.temperature ? p.temperature[r] : p.temperature_all;
-  const float top_p = p.top_p ? p.top_p[r] : p.top_p_all;
-  const float min_p = p.min_p ? p.min_p[r] : p.min_p_all;
-  const int top_k = p.top_k ? p.top_k[r] : p.top_k_all;
-  const float u = p.u[r];
-
-  float top = -kInf;
-  int bad = 0;
-  row.each([&](float f, int64_t) {
-    top = __builtin_fmaxf(top, f);
-    bad |= f != f;
-  });
-  top = newt::lane_reduce<newt::Max, 63>(top);
-  bad = __ballot(bad) != 0;
-  if (lane == 0) {
-    s.top[wave] = top;
-    s.bad[wave] = bad;
-  }
-  if (threadIdx.x == 0) s.listed = s.last = 0;
+  Row<T> row(p, s, r, shift);
+  const Settings o(p, r);
   row.fill_table();
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) {
-    top = __builtin_fmaxf(top, s.top[w]);
-    bad |= s.bad[w];
-  }
-  bad |= !(__builtin_fabsf(top) < kInf) | !(temperature >= 0.0f && temperature < kInf) |
-         (u != u) | (top_p != top_p) | (min_p != min_p);
-  if (bad) {
-    if (threadIdx.x == 0) p.ids[r] = -1;
-    return;
-  }
-  row.top = top;
-  if (temperature == 0.0f || top_k == 1) {
-    const auto is_top = [&](float f, int64_t) { return (u64)(f == top); };
-    row.segments(is_top);
-    if (wave == 0) {
-      const int id = row.find(0, is_top);
-      if (lane == 0) p.ids[r] = id;
-    }
-    return;
-  }
-  row.by = 64.0 / (double)temperature;
-  // the largest weight is 2^shift
-  row.least = (u64)__builtin_ceil(
-      __builtin_fmin(__builtin_fmax((double)min_p, 0.0), 1.0) * __builtin_ldexp(1.0, shift));
-
-  const bool by_count = top_k > 0 && top_k < p.vocab, by_mass = top_p < 1.0f;
-  u64 cut = ~0ull;
-  if (!by_count && !by_mass) {
-    row.segments([&](float f, int64_t i) { return row.kept_weight(f, i, cut); });
-    const int id = row.choose(u, cut);
-    if (threadIdx.x == 0) p.ids[r] = id;
-    return;
-  }
-  row.clear();
-  if (by_count) {
-    row.each([&](float f, int64_t) {
-      const int b = row.point(f).bin;
-      if (b < kBins - 1) atomicAdd(&s.count[b], 1u);
-    });
-  } else {
-    row.each([&](float f, int64_t) {
-      const auto a = row.point(f);
-      if (a.bin < kBins - 1) atomicAdd(&s.mass[a.bin], row.weight(a));
-    });
-  }
-  __syncthreads();
-  // at least the first token
-  const double target = by_count ? 0.0
-      : __builtin_fmax((double)top_p * (double)row.total(), 0x1p-60);
-  row.pick(!by_count, (u64)top_k, 0, target);
-  int bin = s.place == kNone ? kBins : (int)s.place;
-  const u64 before = s.before;
-  const u32 before_count = s.before_count, of_bin = s.place_count;
-  if (by_count && bin < kBins && before_count + of_bin <= kList) {
-    row.each([&](float f, int64_t i) {
-      if (row.point(f).bin <= bin) row.append(place_of(f, (u32)i));
-    });
-    __syncthreads();
-    const int id = row.choose_listed((int)s.listed, (u32)top_k, top_p, u);
-    if (threadIdx.x == 0) p.ids[r] = id;
-    return;
-  }
-  bool listed = !(by_count && by_mass) && !(by_count && of_bin > kList);
-  if (listed) {
-    // what lies before the bin counts at once, what is in it when it is in order
-    __syncthreads();
-    row.segments([&](float f, int64_t i) -> u64 {
-      const auto a = row.point(f);
-      if (a.bin < bin) {
-        const u64 w = row.weight(a);
-        return w >= row.least ? w : 0;
-      }
-      if (a.bin == bin) row.append(place_of(f, (u32)i));
-      return 0;
-    });
-    listed = s.listed <= kList;
-  }
-  if (listed) {
-    const int n = (int)s.listed;
-    if (n) {
-      row.sort(row.fill_up(n));
-      const int i = 4 * threadIdx.x;
-      u64 w[4], sum;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) w[j] = row.listed_weight(i + j, n);
-      u64 run = before + row.scan(w, &sum);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if (i + j < n && (by_count ? before_count + i + j < (u32)top_k : (double)run < target)) {
-          const u64 entry = s.list[i + j];
-          if (w[j] >= row.least) atomicAdd(&s.mass[row.segment_of((u32)entry)], w[j]);
-          atomicMax(&s.last, entry);
+  bool bad;
+  const float top = row.largest(bad);
+  int id = -1;
+  if (!(bad | o.bad) && __builtin_fabsf(top) < kInf) {
+    row.set(o, top);
+    if (o.greedy) {
+      row.first();
+      id = (int)s.first;
+    } else {
+      if (o.by_count | o.by_mass) row.histogram(o);
+      const auto e = row.end(o);
+      if (e.mode == kListed) {
+        row.candidates(e);
+        id = row.choose_listed(o, e);
+      } else {
+        if (e.mode == kSums) row.sums(e);
+        if (e.mode == kSlow || s.listed > kList) {
+          __syncthreads();
+          row.fill_table();
+          __syncthreads();
+          id = row.choose_slowly(o);
+        } else {
+          id = row.choose_by_sums(o, e);
         }
-        run += w[j];
+      }
+    }
+  }
+  if (threadIdx.x == 0) p.ids[r] = id;
+}
+
+// A row in several programs: the same steps, a launch each, whose results meet in
+// the workspace.
+struct Joint {
+  float top[kMostParts];
+  int bad[kMostParts];
+  u32 listed, first;
+  u64 bins[kBins];  // masses or counts
+  u64 segments[kBins];
+  u64 list[kList];
+};
+
+template <typename T>
+struct Part {
+  Joint& j;
+  Row<T> row;
+  Settings o;
+  int parts, part;
+  __device__ __forceinline__ Part(const newt_sample_params& p, Shared& s, int64_t r, int parts_,
+                                  int part_, int shift)
+      : j(((Joint*)p.workspace)[r]), row(p, s, r, shift), o(p, r), parts(parts_), part(part_) {}
+  // this program's chunks, whole segments
+  __device__ __forceinline__ void own() {
+    const int per = (row.chunks + kBins - 1) / kBins;
+    const int each = ((row.chunks + parts - 1) / parts + per - 1) / per * per;
+    row.from = part * each < row.chunks ? part * each : row.chunks;
+    row.to = row.from + each < row.chunks ? row.from + each : row.chunks;
+  }
+  // Sets the row's largest logit; false where there is nothing to choose.
+  __device__ __forceinline__ bool top() {
+    float most = -kInf;
+    bool bad = o.bad;
+    for (int i = 0; i < parts; ++i) {
+      most = __builtin_fmaxf(most, j.top[i]);
+      bad |= j.bad[i] != 0;
+    }
+    if (bad || !(__builtin_fabsf(most) < kInf)) return false;
+    row.set(o, most);
+    return true;
+  }
+  __device__ __forceinline__ typename Row<T>::End end() {
+    if (o.by_count | o.by_mass) {
+      for (int i = threadIdx.x; i < kBins; i += kThreads) {
+        row.s.mass[i] = o.by_count ? 0 : j.bins[i];
+        row.s.count[i] = o.by_count ? (u32)j.bins[i] : 0;
       }
       __syncthreads();
-      cut = s.last;
     }
-  } else {
-    __syncthreads();
-    if (by_count) cut = row.last(false, (u32)top_k, 0.0);
-    if (by_mass) {
-      double mass_target = target;
-      if (by_count) {
-        row.segments([&](float f, int64_t i) {
-          return place_of(f, (u32)i) <= cut ? row.weight(f) : (u64)0;
-        });
-        mass_target = __builtin_fmax((double)top_p * (double)row.total(), 0x1p-60);
-      }
-      const u64 by_p = row.last(true, 0, mass_target);
-      cut = by_p < cut ? by_p : cut;
-    }
-    row.segments([&](float f, int64_t i) { return row.kept_weight(f, i, cut); });
+    return row.end(o);
   }
-  const int id = row.choose(u, cut);
+};
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads) part_top_kernel(newt_sample_params p, int parts,
+                                                            int shift) {
+  __shared__ Shared s;
+  Part<T> a(p, s, blockIdx.x / parts, parts, blockIdx.x % parts, shift);
+  a.own();
+  bool bad;
+  const float top = a.row.largest(bad);
+  for (int i = a.part * kThreads + threadIdx.x; i < kBins; i += parts * kThreads) a.j.bins[i] = 0;
+  if (threadIdx.x == 0) {
+    a.j.top[a.part] = top;
+    a.j.bad[a.part] = bad;
+    if (a.part == 0) {
+      a.j.listed = 0;
+      a.j.first = 0xffffffffu;
+    }
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads) part_histogram_kernel(newt_sample_params p, int parts,
+                                                                  int shift) {
+  __shared__ Shared s;
+  Part<T> a(p, s, blockIdx.x / parts, parts, blockIdx.x % parts, shift);
+  a.own();
+  if (a.o.greedy || !(a.o.by_count | a.o.by_mass) || !a.top()) return;
+  a.row.fill_table();
+  a.row.histogram(a.o);
+  for (int i = threadIdx.x; i < kBins; i += kThreads) {
+    const u64 v = a.o.by_count ? s.count[i] : s.mass[i];
+    if (v) atomicAdd(&a.j.bins[i], v);
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads) part_sums_kernel(newt_sample_params p, int parts,
+                                                             int shift) {
+  __shared__ Shared s;
+  Part<T> a(p, s, blockIdx.x / parts, parts, blockIdx.x % parts, shift);
+  a.own();
+  if (!a.top()) return;
+  if (threadIdx.x == 0) {
+    s.listed = 0;
+    s.first = 0xffffffffu;
+  }
+  a.row.fill_table();
+  __syncthreads();
+  if (a.o.greedy) {
+    a.row.first();
+    if (threadIdx.x == 0) atomicMin(&a.j.first, s.first);
+    return;
+  }
+  const auto e = a.end();
+  if (e.mode == kSlow) return;
+  if (e.mode == kListed) {
+    a.row.candidates(e);
+  } else {
+    a.row.sums(e);
+    const int per = (a.row.chunks + kBins - 1) / kBins;
+    for (int g = a.row.from / per + threadIdx.x; g * per < a.row.to; g += kThreads)
+      a.j.segments[g] = s.mass[g];
+  }
+  if (threadIdx.x == 0) s.place = atomicAdd(&a.j.listed, s.listed);
+  __syncthreads();
+  const u32 n = s.listed < kList ? s.listed : kList;
+  for (u32 i = threadIdx.x; i < n; i += kThreads)
+    if (s.place + i < kList) a.j.list[s.place + i] = s.list[i];
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads) part_choose_kernel(newt_sample_params p, int parts,
+                                                               int shift) {
+  __shared__ Shared s;
+  const int64_t r = blockIdx.x;
+  Part<T> a(p, s, r, parts, 0, shift);
+  int id = -1;
+  if (a.top()) {
+    if (a.o.greedy) {
+      id = (int)a.j.first;
+    } else {
+      a.row.fill_table();
+      __syncthreads();
+      const auto e = a.end();
+      const u32 n = a.j.listed;
+      if (e.mode == kSlow || n > kList) {
+        id = a.row.choose_slowly(a.o);
+      } else {
+        for (u32 i = threadIdx.x; i < n; i += kThreads) s.list[i] = a.j.list[i];
+        if (threadIdx.x == 0) {
+          s.listed = n;
+          if (e.edge < kBins) s.edge = s.table[e.edge];
+        }
+        if (e.mode == kSums) {
+          const int per = (a.row.chunks + kBins - 1) / kBins;
+          for (int g = threadIdx.x; g < kBins; g += kThreads)
+            s.mass[g] = g * per < a.row.chunks ? a.j.segments[g] : 0;
+        }
+        __syncthreads();
+        id = e.mode == kListed ? a.row.choose_listed(a.o, e) : a.row.choose_by_sums(a.o, e);
+      }
+    }
+  }
   if (threadIdx.x == 0) p.ids[r] = id;
+}
+
+// How many programs share a row: enough to fill the chip, each with work for its
+// waves.
+int parts_of(int64_t rows, int64_t vocab, int dtype) {
+  const int64_t chunk = dtype == NEWT_F32 ? 256 : 512;
+  int64_t n = rows ? 256 / rows : 1;
+  const int64_t most = (vocab + chunk * kWaves - 1) / (chunk * kWaves);
+  n = n < most ? n : most;
+  n = n < kMostParts ? n : kMostParts;
+  return n < 2 ? 1 : (int)n;
 }
 
 // A weight's bits behind the point: sums of `vocab` of them stay below 2^63.
@@ -666,6 +977,26 @@ int weight_bits(int64_t vocab) {
   int bits = 0;
   while (vocab >> bits) ++bits;
   return 62 - bits < 45 ? 62 - bits : 45;
+}
+
+template <typename T>
+int launch(const newt_sample_params& p, int shift, hipStream_t stream) {
+  const char* const what = "newt_sample";
+  const int parts = parts_of(p.rows, p.vocab, p.dtype);
+  if (parts == 1) return run(what, sample_kernel<T>, p.rows, kThreads, 0, stream, p, shift);
+  if (!p.workspace || ((uintptr_t)p.workspace & 7))
+    return fail(NEWT_ERR_INVALID, "newt_sample: null or unaligned workspace");
+  int status = run(what, part_top_kernel<T>, p.rows * parts, kThreads, 0, stream, p, parts, shift);
+  // settings of the rows' own are on the GPU: a row may need the histogram
+  const bool none = !p.top_k && !p.top_p && !(p.top_k_all > 0 && p.top_k_all < p.vocab) &&
+                    p.top_p_all >= 1.0f;
+  if (status == NEWT_OK && !none)
+    status = run(what, part_histogram_kernel<T>, p.rows * parts, kThreads, 0, stream, p, parts, shift);
+  if (status == NEWT_OK)
+    status = run(what, part_sums_kernel<T>, p.rows * parts, kThreads, 0, stream, p, parts, shift);
+  if (status == NEWT_OK)
+    status = run(what, part_choose_kernel<T>, p.rows, kThreads, 0, stream, p, parts, shift);
+  return status;
 }
 
 const char* wrong(const newt_sample_params& p) {
@@ -682,7 +1013,11 @@ const char* wrong(const newt_sample_params& p) {
 }  // namespace
 }  // namespace newt_ops
 
-extern "C" size_t newt_sample_workspace(int64_t, int64_t, int32_t) { return 0; }
+extern "C" size_t newt_sample_workspace(int64_t rows, int64_t vocab, int32_t dtype) {
+  using namespace newt_ops;
+  if (rows <= 0 || vocab <= 0 || parts_of(rows, vocab, dtype) == 1) return 0;
+  return (size_t)rows * sizeof(Joint);
+}
 
 extern "C" int newt_sample(const newt_sample_params* params, void* stream) {
   using namespace newt_ops;
@@ -693,12 +1028,9 @@ extern "C" int newt_sample(const newt_sample_params* params, void* stream) {
   if (!p.logits || !p.u || !p.ids) return fail(NEWT_ERR_INVALID, "newt_sample: null tensor");
   hipStream_t s = static_cast<hipStream_t>(stream);
   const int shift = weight_bits(p.vocab);
-  const auto go = [&](auto kernel) {
-    return run("newt_sample", kernel, p.rows, kThreads, 0, s, p, shift);
-  };
   switch (p.dtype) {
-    case NEWT_F32: return go(sample_kernel<float>);
-    case NEWT_F16: return go(sample_kernel<f16>);
-    default: return go(sample_kernel<bf16>);
+    case NEWT_F32: return launch<float>(p, shift, s);
+    case NEWT_F16: return launch<f16>(p, shift, s);
+    default: return launch<bf16>(p, shift, s);
   }
 }

@@ -345,10 +345,10 @@ def test_sample_settings_of_rows():
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
-def test_sample_ties(dtype):
+@pytest.mark.parametrize("V", [4003, 30011])
+def test_sample_ties(dtype, V):
     """Equal logits: the lowest ids stay, in counts that top_k and top_p cut."""
-    V = 4003
-    x = torch.full((8, V), 1.5, dtype=dtype, device="cuda")
+    x = torch.full((8, V), 1.5, dtype=dtype, device="cuda")  # ties beyond any list
     x[1, ::2] = -0.0
     x[1, 1::2] = 0.0
     x[2, 100:] = 0.5
@@ -365,15 +365,15 @@ def test_sample_ties(dtype):
             check_sample(x, u, **settings)
 
 
-def test_sample_masked_and_bad_rows():
-    V = 3000
+@pytest.mark.parametrize("V", [3000, 50000])
+def test_sample_masked_and_bad_rows(V):
     x = rnd(12, V, seed=3, scale=2.0)
     x[0] = -INF
     x[1, 5] = NAN
-    x[2, 2999] = INF
+    x[2, V - 1] = INF
     x[3] = -INF
     x[3, 1234] = -7.0
-    x[4, :2990] = -INF
+    x[4, :V - 10] = -INF
     x[5, 1:] = torch.finfo(F32).min
     x[6] = torch.finfo(F32).min
     x[7] = torch.linspace(-3e38, 3e38, V)
@@ -383,13 +383,33 @@ def test_sample_masked_and_bad_rows():
     for settings in ({}, {"top_k": 20}, {"top_p": 0.9}, {"min_p": 0.1}, {"temperature": 0.0},
                      {"temperature": 1e-30, "top_k": 3}, {"temperature": 1e30, "top_p": 0.5}):
         got = check_sample(x, u, **settings)
-        assert got[0] == got[1] == got[2] == got[9] == -1 and got[3] == 1234 and got[4] >= 2990
+        assert got[0] == got[1] == got[2] == got[9] == -1 and got[3] == 1234 and got[4] >= V - 10
     bad = {"temperature": [NAN, -1.0, INF, 1.0], "top_p": [1.0, 1.0, 1.0, NAN]}
     settings = {k: torch.tensor(v, device="cuda") for k, v in bad.items()}
     assert W().sample(x[8:9].expand(4, V), u[:4], **settings).tolist() == [-1] * 4
     edge = torch.tensor([NAN, -0.5, 1.0, 7.0], device="cuda")
     got = W().sample(torch.zeros(4, V, device="cuda"), edge)
     assert got.tolist() == [-1, 0, V - 1, V - 1]
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("T", [2, 150])
+def test_sample_narrow_and_wide_rows(dtype, T):
+    """Logits that all lie in a few bins of the histogram, or far apart, in rows of
+    one program and of several: each way in which the end is found."""
+    V = 20001
+    x = rnd(T, V, dtype=dtype, seed=9)
+    for scale, temperature in ((0.01, 1.0), (1.0, 40.0), (1.0, 1.0), (4.0, 0.2), (200.0, 1.0)):
+        y = x * scale
+        for settings in ({"top_k": 3000}, {"top_k": 6000}, {"top_k": 19999}, {"top_p": 0.3},
+                         {"top_p": 0.999}, {"top_k": 6000, "top_p": 0.5}, {"min_p": 0.3},
+                         {"top_k": 2000, "top_p": 0.9, "min_p": 0.2},
+                         {"top_p": 0.9, "min_p": 0.001}, {"min_p": 1e-13}):
+            got = W().sample(y, uniform(T, 3), temperature=temperature, **settings).tolist()
+            for r in range(0, T, 75):
+                row = {k: v if k == "top_k" else torch.tensor(v, dtype=F32).item()
+                       for k, v in {"temperature": temperature, **settings}.items()}
+                assert got[r] == orc.sample(y[r], uniform(T, 3)[r].item(), **row), (r, scale, row)
 
 
 def test_sample_strides():
