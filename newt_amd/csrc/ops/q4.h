@@ -9,25 +9,36 @@ template <typename T> struct frag;
 template <> struct frag<bf16> { typedef bf16x8 type; };
 template <> struct frag<f16> { typedef f16x8 type; };
 
-// 8 weights to (16 + q) / 16: the 4 bits go below the point of a number in [1, 2)
+// 8 weights to (16 + q) / 16: the 4 bits go below the point of a number in [1, 2),
+// by one shift and one v_and_or_b32 for two of them. That instruction takes one
+// constant from a scalar register and none from the code, so both are kept from
+// the compiler, which would rather use two instructions with constants in them.
 template <typename T>
-__device__ __forceinline__ typename frag<T>::type widen(u32 w) {
-  u32x4 r;
-  if constexpr (__is_same(T, bf16)) {  // the 4 upper of 7 bits
-    const u32 mask = 0x00780078, one = 0x3f803f80;
-    r[0] = (w & mask) | one;
-    r[1] = ((w >> 4) & mask) | one;
-    r[2] = ((w >> 8) & mask) | one;
-    r[3] = (__builtin_amdgcn_alignbit(w, w, 12) & mask) | one;
-  } else {  // of 10 bits
-    const u32 mask = 0x03c003c0, one = 0x3c003c00;
-    r[0] = ((w << 3) & mask) | one;
-    r[1] = ((w >> 1) & mask) | one;
-    r[2] = ((w >> 5) & mask) | one;
-    r[3] = (__builtin_amdgcn_alignbit(w, w, 9) & mask) | one;
+struct Widen {
+  u32 mask, one;
+  __device__ __forceinline__ Widen() {
+    constexpr bool B = __is_same(T, bf16);  // the upper 4 of 7 bits, or of 10
+    mask = B ? 0x00780078u : 0x03c003c0u;
+    one = B ? 0x3f803f80u : 0x3c003c00u;
+    asm("" : "+s"(mask));
+    asm("" : "+v"(one));
   }
-  return __builtin_bit_cast(typename frag<T>::type, r);
-}
+  __device__ __forceinline__ typename frag<T>::type operator()(u32 w) const {
+    u32x4 r;
+    if constexpr (__is_same(T, bf16)) {
+      r[0] = (w & mask) | one;
+      r[1] = ((w >> 4) & mask) | one;
+      r[2] = ((w >> 8) & mask) | one;
+      r[3] = (__builtin_amdgcn_alignbit(w, w, 12) & mask) | one;
+    } else {
+      r[0] = ((w << 3) & mask) | one;
+      r[1] = ((w >> 1) & mask) | one;
+      r[2] = ((w >> 5) & mask) | one;
+      r[3] = (__builtin_amdgcn_alignbit(w, w, 9) & mask) | one;
+    }
+    return __builtin_bit_cast(typename frag<T>::type, r);
+  }
+};
 
 __device__ __forceinline__ float activate(float v, int act) {
   if (act == NEWT_ACT_SILU) return v / (1.0f + __builtin_expf(-v));

@@ -44,6 +44,7 @@ q4_kernel(newt_q4_params p, int n_blocks) {
     in[m] = row < p.rows;
     x[m] = (const T*)p.x + (in[m] ? row : 0) * p.x_stride + 8 * part;
   }
+  const Widen<T> widen;
   TX ones;
 #pragma unroll
   for (int i = 0; i < 8; ++i) ones[i] = (T)1.0f;
@@ -97,7 +98,7 @@ q4_kernel(newt_q4_params p, int n_blocks) {
         for (int i = 0; i < 4; ++i) zero[i] = -1.0f - 0.0625f * (float)((z >> (8 * i)) & 255);
         TX a[STEPS];
 #pragma unroll
-        for (int j = 0; j < STEPS; ++j) a[j] = widen<T>(w[n][g * STEPS + j]);
+        for (int j = 0; j < STEPS; ++j) a[j] = widen(w[n][g * STEPS + j]);
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
           f32x4 part_sum = (f32x4)(0.0f);

@@ -22,14 +22,16 @@ __global__ void __launch_bounds__(256, 2)
 q4_many_kernel(newt_q4_params p, int m_blocks, int n_blocks, int per) {
   typedef typename frag<T>::type TX;
   constexpr int PER = kBlock / GROUP, STEPS = GROUP / 16;
-  __shared__ __attribute__((aligned(16))) T even[kRows * kBlock];
-  __shared__ __attribute__((aligned(16))) T odd[kRows * kBlock];
-  __shared__ __attribute__((aligned(16))) bf16x4 sums[PER * kRows];
-  // a block's scales and zeros, [tile][group][16]
-  constexpr int SCALES = kTiles * PER * 2, ZEROS = kTiles * PER;  // pieces of 16 bytes
-  constexpr int LEVELS = (SCALES + ZEROS + 63) / 64 * 64 * 16;
-  __shared__ __attribute__((aligned(16))) unsigned char levels_even[LEVELS];
-  __shared__ __attribute__((aligned(16))) unsigned char levels_odd[LEVELS];
+  // three stages of x, [row][column], and of each wave's scales and zeros, [tile]
+  // [group][16]
+  constexpr int SCALES = 4 * PER * 2, ZEROS = 4 * PER;  // pieces of 16 bytes
+  __shared__ __attribute__((aligned(16))) T x0[kRows * kBlock];
+  __shared__ __attribute__((aligned(16))) T x1[kRows * kBlock];
+  __shared__ __attribute__((aligned(16))) T x2[kRows * kBlock];
+  __shared__ __attribute__((aligned(16))) unsigned char levels0[4 * 2048];
+  __shared__ __attribute__((aligned(16))) unsigned char levels1[4 * 2048];
+  __shared__ __attribute__((aligned(16))) unsigned char levels2[4 * 2048];
+  __shared__ __attribute__((aligned(16))) bf16x4 sums[2][PER * kRows];
   const int lane = threadIdx.x & 63, wave = wave_id(), half = lane >> 5;
   const int program = by_die(blockIdx.x, gridDim.x);
   const int split = program / (m_blocks * n_blocks), unit = program % (m_blocks * n_blocks);
@@ -44,42 +46,42 @@ q4_many_kernel(newt_q4_params p, int m_blocks, int n_blocks, int per) {
 
   // a lane's row of the two times 32 that its wave has
   const auto at = [&](int t) { return (int64_t)(t < tiles ? t : tiles - 1); };
-  const u32x4* q[2];
+  const char* const q = (const char*)p.q + at(tile) * blocks * 1024;
+  u32 q_at[2];  // fewer than 2^19 blocks
 #pragma unroll
   for (int f = 0; f < 2; ++f)
-    q[f] = (const u32x4*)p.q + at(tile + 2 * f + ((lane >> 4) & 1)) * blocks * 64 + 16 * half +
-           (lane & 15);
-  // the piece of a block's scales or zeros that a thread stages
-  const int piece = threadIdx.x;
-  const unsigned char* level = nullptr;
-  int level_step = 0;
-  if (piece < SCALES) {
-    level = (const unsigned char*)p.scales +
-            (at(n_block * kTiles + piece / (2 * PER)) * groups * 2 + piece % (2 * PER)) * 16;
-    level_step = 2 * PER * 16;
-  } else if (piece < SCALES + ZEROS && p.zeros) {
-    const int i = piece - SCALES;
-    level = (const unsigned char*)p.zeros +
-            (at(n_block * kTiles + i / PER) * groups + i % PER) * 16;
-    level_step = PER * 16;
-  }
+    q_at[f] = (u32)(at(tile + 2 * f + ((lane >> 4) & 1)) - at(tile)) * (u32)blocks * 1024 +
+              (16 * half + (lane & 15)) * 16;
+  // the pieces of its wave's scales and zeros that a lane stages
+  const char* const levels_of[2] = {
+      (const char*)p.scales + at(tile) * groups * 32,
+      (const char*)(p.zeros ? p.zeros : p.scales) + at(tile) * groups * 16};
+  const auto level_at = [&](int per) {  // pieces of a tile in a block
+    return (u32)(at(tile + lane / per % 4) - at(tile)) * (u32)(blocks * per) * 16 + lane % per * 16;
+  };
+  const u32 scale_at = level_at(2 * PER), zero_at = level_at(PER);
 
+  int row0, k0;
+  newt::lds_tile_slot<T, kBlock>(threadIdx.x, row0, k0);
+  const u32 x_at = (u32)(row0 * (int)p.x_stride + k0) * 2;
   const auto stage = [&](int b, T* to_lds, unsigned char* levels) {
-    if (level) newt::lds_dma16(level + (int64_t)b * level_step, levels + 64 * wave * 16);
+    newt::lds_dma16_masked(levels_of[0] + (int64_t)b * (2 * PER * 16), scale_at, lane < SCALES,
+                           levels + 2048 * wave);
+    newt::lds_dma16_masked(levels_of[1] + (int64_t)b * (PER * 16), zero_at, lane < ZEROS,
+                           levels + 2048 * wave + 1024);
     const T* base = (const T*)p.x + m0 * p.x_stride + b * kBlock;
     const int cols = (int)(p.cols - (int64_t)b * kBlock);
 #pragma unroll
-    for (int c = 0; c < kRows * kBlock / 8 / 256; ++c) {
-      const int first = c * 256 + 64 * wave;
-      int row, k;
-      newt::lds_tile_slot<T, kBlock>(first + lane, row, k);
-      const bool in = (row < rows) & (k < cols);
+    for (int c = 0; c < kRows / 16; ++c) {
+      // 16 rows on, a lane's place in them is the same
+      const bool in = (row0 < rows - 16 * c) & (k0 < cols);
       if constexpr (DIRECT) {
-        newt::lds_dma16_masked(base, (u32)(row * (int)p.x_stride + k) * 2, in, to_lds + first * 8);
+        newt::lds_dma16_masked(base + 16 * c * p.x_stride, x_at, in,
+                               to_lds + (c * 256 + 64 * wave) * 8);
       } else {
         T t[8] = {};
-        if (in) newt::load_vec<T, 8>(base + row * p.x_stride + k, t, newt::any_align());
-        newt::store_vec<T, 8>(to_lds + (first + lane) * 8, t);
+        if (in) newt::load_vec<T, 8>(base + (row0 + 16 * c) * p.x_stride + k0, t, newt::any_align());
+        newt::store_vec<T, 8>(to_lds + (c * 256 + threadIdx.x) * 8, t);
       }
     }
   };
@@ -89,44 +91,51 @@ q4_many_kernel(newt_q4_params p, int m_blocks, int n_blocks, int per) {
   for (int f = 0; f < 2; ++f)
 #pragma unroll
     for (int m = 0; m < 2; ++m) acc[f][m] = (f32x16)(0.0f);
+  const Widen<T> widen;
   TX ones;
 #pragma unroll
   for (int i = 0; i < 8; ++i) ones[i] = (T)1.0f;
 
-  const auto load = [&](int b, u32x4 (&w)[2][2]) {
+  // A block's x, scales, zeros and weights.
+  const auto load = [&](int b, u32x4 (&w)[2][2], T* to_lds, unsigned char* levels) {
+    b = b < to ? b : to - 1;
+    stage(b, to_lds, levels);
 #pragma unroll
     for (int f = 0; f < 2; ++f)
 #pragma unroll
-      for (int i = 0; i < 2; ++i) w[f][i] = q[f][(int64_t)b * 64 + 32 * i];
+      for (int i = 0; i < 2; ++i)
+        w[f][i] = *(const u32x4*)(q + (int64_t)b * 1024 + q_at[f] + 512 * i);
   };
 
-  // One block, while the next one is on its way.
-  const auto step = [&](int b, const T* now, T* next, const unsigned char* levels,
-                        unsigned char* next_levels, u32x4 (&v)[2][2], u32x4 (&w)[2][2]) {
-    newt::wait_vmcnt<0>();
-    __syncthreads();
-    if (b + 1 < to) {
-      stage(b + 1, next, next_levels);
-      load(b + 1, w);
-    }
+  // The sums of 16 rows of a block, in three parts.
+  const auto add_up = [&](const T* x_lds, bf16x4* to_sums) {
     f32x4 all = (f32x4)(0.0f);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const TX x = __builtin_bit_cast(TX, newt::lds_frag_k<T, kBlock, 16>(now, 16 * wave, 32 * j, lane));
+      const TX x = __builtin_bit_cast(TX, newt::lds_frag_k<T, kBlock, 16>(x_lds, 16 * wave, 32 * j, lane));
       all = newt::mfma_16x16x32(ones, x, all);
       if ((j + 1) % (GROUP / 32) == 0) {
         const bf16 hi = (bf16)all[0];
         const float rest = all[0] - (float)hi;
         const bf16 mid = (bf16)rest;
         if (lane < 16)
-          sums[j / (GROUP / 32) * kRows + 16 * wave + lane] =
+          to_sums[j / (GROUP / 32) * kRows + 16 * wave + lane] =
               bf16x4{hi, mid, (bf16)(rest - (float)mid), (bf16)0.0f};
         all = (f32x4)(0.0f);
       }
     }
-    // the sums are there; what is on its way to the other stage need not be
+  };
+
+  // One block, while the one after the next is on its way: the next one is there,
+  // and its sums come one block ahead, so that they need no barrier of their own.
+  const auto step = [&](int b, const T* now, const unsigned char* levels, u32x4 (&v)[2][2],
+                        const T* after, T* next, unsigned char* next_levels, u32x4 (&w)[2][2],
+                        const bf16x4* own_sums, bf16x4* next_sums) {
+    newt::wait_vmcnt<0>();
     __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
     newt::barrier_nofence();
+    load(b + 2, w, next, next_levels);
+    add_up(after, next_sums);
     // not unrolled: groups side by side would not fit the registers
 #pragma unroll 1
     for (int g = 0; g < PER; ++g) {
@@ -135,49 +144,63 @@ q4_many_kernel(newt_q4_params p, int m_blocks, int n_blocks, int per) {
       for (int f = 0; f < 2; ++f)
 #pragma unroll
         for (int m = 0; m < 2; ++m) part[f][m] = (f32x16)(0.0f);
-#pragma unroll
-      for (int i = 0; i < STEPS; ++i) {
-        const int st = g * STEPS + i;
-        TX x[2];
+      // a step's operands are made while the one before it is multiplied
+      TX x[2][2], a[2][2];
+      const auto operands = [&](int i) {
 #pragma unroll
         for (int m = 0; m < 2; ++m)
-          x[m] = __builtin_bit_cast(TX, newt::lds_frag_k<T, kBlock, 32>(now, 32 * m, 16 * st, lane));
+          x[i & 1][m] = __builtin_bit_cast(
+              TX, newt::lds_frag_k<T, kBlock, 32>(now, 32 * m, 16 * (g * STEPS + i), lane));
 #pragma unroll
-        for (int f = 0; f < 2; ++f) {
-          const TX a = widen<T>(v[f][i & 1][i / 2]);
+        for (int f = 0; f < 2; ++f) a[i & 1][f] = widen(v[f][i & 1][i / 2]);
+      };
+      operands(0);
 #pragma unroll
-          for (int m = 0; m < 2; ++m) part[f][m] = newt::mfma_32x32x16(a, x[m], part[f][m]);
+      for (int i = 0; i < STEPS; ++i) {
+        if (i + 1 < STEPS) operands(i + 1);
+#pragma unroll
+        for (int f = 0; f < 2; ++f)
+#pragma unroll
+          for (int m = 0; m < 2; ++m)
+            part[f][m] = newt::mfma_32x32x16(a[i & 1][f], x[i & 1][m], part[f][m]);
+        __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);  // LDS reads
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // a product
+          __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);  // vector instructions
         }
       }
-      bf16x8 x[2];
+      bf16x8 less_x[2];
 #pragma unroll
       for (int m = 0; m < 2; ++m) {
-        const bf16x4 t = sums[g * kRows + 32 * m + (lane & 31)];
+        const bf16x4 t = own_sums[g * kRows + 32 * m + (lane & 31)];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[m][i] = i < 3 && half == 0 ? t[i] : (bf16)0.0f;
+        for (int i = 0; i < 8; ++i) less_x[m][i] = i < 3 && half == 0 ? t[i] : (bf16)0.0f;
       }
 #pragma unroll
       for (int f = 0; f < 2; ++f) {
         // the lane's own row's zero, and the scales of the rows whose sums it has
-        const int own = 4 * wave + 2 * f;
+        const int own = 2 * f;
         const u32 zero =
-            p.zeros ? levels[SCALES * 16 + ((own + ((lane >> 4) & 1)) * PER + g) * 16 + (lane & 15)] : 8;
+            p.zeros ? levels[2048 * wave + 1024 +
+                             ((own + ((lane >> 4) & 1)) * PER + g) * 16 + (lane & 15)]
+                    : 8;
         float scale[16];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           S t[4];
           newt::load_vec<S, 4>(
-              (const S*)levels + ((own + i / 2) * PER + g) * 16 + 8 * (i & 1) + 4 * half, t);
+              (const S*)(levels + 2048 * wave) + ((own + i / 2) * PER + g) * 16 + 8 * (i & 1) + 4 * half, t);
 #pragma unroll
           for (int j = 0; j < 4; ++j) scale[4 * i + j] = newt::to_f32(t[j]);
         }
         const bf16 less = (bf16)(-1.0f - 0.0625f * (float)zero);
-        bf16x8 a;
+        bf16x8 less_a;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) a[i] = i < 3 ? less : (bf16)0.0f;
+        for (int i = 0; i < 8; ++i) less_a[i] = i < 3 ? less : (bf16)0.0f;
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
-          part[f][m] = newt::mfma_32x32x16(a, x[m], part[f][m]);
+          part[f][m] = newt::mfma_32x32x16(less_a, less_x[m], part[f][m]);
 #pragma unroll
           for (int e = 0; e < 16; ++e)
             acc[f][m][e] = __builtin_fmaf(part[f][m][e], scale[e], acc[f][m][e]);
@@ -193,15 +216,25 @@ q4_many_kernel(newt_q4_params p, int m_blocks, int n_blocks, int per) {
       }
     }
   };
-  u32x4 v[2][2], w[2][2];
-  if (from < to) {
-    stage(from, even, levels_even);
-    load(from, v);
+  u32x4 w0[2][2], w1[2][2], w2[2][2];
+  load(from, w0, x0, levels0);
+  load(from + 1, w1, x1, levels1);
+  newt::wait_vmcnt<0>();
+  __syncthreads();
+  add_up(x0, sums[0]);
+  for (int b = from; b < to; b += 6) {
+#define NEWT_STEP(i, X, AFTER, NEXT, S)                                                        \
+  if (b + i < to)                                                                              \
+  step(b + i, x##X, levels##X, w##X, x##AFTER, x##NEXT, levels##NEXT, w##NEXT, sums[S], sums[1 - S])
+    NEWT_STEP(0, 0, 1, 2, 0);
+    NEWT_STEP(1, 1, 2, 0, 1);
+    NEWT_STEP(2, 2, 0, 1, 0);
+    NEWT_STEP(3, 0, 1, 2, 1);
+    NEWT_STEP(4, 1, 2, 0, 0);
+    NEWT_STEP(5, 2, 0, 1, 1);
+#undef NEWT_STEP
   }
-  for (int b = from; b < to; b += 2) {
-    step(b, even, odd, levels_even, levels_odd, v, w);
-    if (b + 1 < to) step(b + 1, odd, even, levels_odd, levels_even, w, v);
-  }
+  newt::wait_vmcnt<0>();
 
   const bool whole = per >= blocks;
 #pragma unroll
@@ -290,6 +323,7 @@ template <typename T, typename S, int GROUP>
 int launch(const newt_q4_params& p, hipStream_t stream) {
   const Plan r(p);
   const int64_t grid = r.m_blocks * r.n_blocks * r.splits;
+  if (p.cols >= 1 << 25) return fail(NEWT_ERR_INVALID, "newt_q4_matmul: too many columns");
   if (grid > 0x7fffffff) return fail(NEWT_ERR_INVALID, "newt_q4_matmul: too many rows");
   if (r.splits > 1 && !p.workspace)
     return fail(NEWT_ERR_INVALID, "newt_q4_matmul: null workspace");
