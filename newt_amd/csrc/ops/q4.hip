@@ -36,13 +36,13 @@ q4_kernel(newt_q4_params p, int n_blocks) {
     q[n] = (const u32x4*)p.q + t * blocks * 64 + lane;
     at[n] = t * groups * 16 + 4 * part;
   }
+  // Rows of x behind the last one are that one again, and columns behind the last
+  // one the first ones: their sums are not stored, their scales are 0.
   const T* x[MT];
-  bool in[MT];
 #pragma unroll
   for (int m = 0; m < MT; ++m) {
     const int64_t row = ((int64_t)m_block * MT + m) * 16 + col;
-    in[m] = row < p.rows;
-    x[m] = (const T*)p.x + (in[m] ? row : 0) * p.x_stride + 8 * part;
+    x[m] = (const T*)p.x + (row < p.rows ? row : p.rows - 1) * p.x_stride + 8 * part;
   }
   const Widen<T> widen;
   TX ones;
@@ -56,16 +56,26 @@ q4_kernel(newt_q4_params p, int n_blocks) {
 
   for (int b = wave; b < blocks; b += WAVES) {
     u32x4 w[NT];
+    u32x2 s[PER][NT];
+    u32 z[PER][NT];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) w[n] = q[n][(int64_t)b * 64];
+    for (int n = 0; n < NT; ++n) {
+      w[n] = q[n][(int64_t)b * 64];
+#pragma unroll
+      for (int g = 0; g < PER; ++g) {
+        const int64_t i = at[n] + (int64_t)(b * PER + g) * 16;
+        s[g][n] = *(const u32x2*)((const unsigned short*)p.scales + i);
+        z[g][n] = p.zeros ? *(const u32*)((const unsigned char*)p.zeros + i) : 0x08080808u;
+      }
+    }
     TX v[MT][4];
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        T t[8] = {};
-        if (in[m] && b * 128 + 32 * j < p.cols)
-          newt::load_vec<T, 8>(x[m] + b * 128 + 32 * j, t, newt::any_align());
+        const int k = b * 128 + 32 * j < (int)p.cols ? b * 128 + 32 * j : 0;
+        T t[8];
+        newt::load_vec<T, 8>(x[m] + k, t, newt::any_align());
         v[m][j] = __builtin_bit_cast(TX, newt::pack8(t[0], t[1], t[2], t[3], t[4], t[5], t[6], t[7]));
       }
 #pragma unroll
@@ -75,39 +85,31 @@ q4_kernel(newt_q4_params p, int n_blocks) {
       for (int m = 0; m < MT; ++m) {
         all[m] = (f32x4)(0.0f);
 #pragma unroll
-        for (int j = 0; j < STEPS; ++j) all[m] = newt::mfma_16x16x32(ones, v[m][g * STEPS + j], all[m]);
+        for (int j = 0; j < STEPS; ++j)
+          all[m] = newt::mfma_16x16x32(ones, v[m][g * STEPS + j], all[m]);
       }
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        const int64_t s = at[n] + (int64_t)(b * PER + g) * 16;
-        float scale[4], zero[4];
-        if (p.scale_dtype == NEWT_F16) {
-          f16 t[4];
-          newt::load_vec<f16, 4>((const f16*)p.scales + s, t);
+        f32x4 part_sum[MT];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) scale[i] = newt::to_f32(t[i]);
-        } else {
-          bf16 t[4];
-          newt::load_vec<bf16, 4>((const bf16*)p.scales + s, t);
+        for (int m = 0; m < MT; ++m) part_sum[m] = (f32x4)(0.0f);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) scale[i] = newt::to_f32(t[i]);
+        for (int j = 0; j < STEPS; ++j) {
+          const TX a = widen(w[n][g * STEPS + j]);
+#pragma unroll
+          for (int m = 0; m < MT; ++m)
+            part_sum[m] = newt::mfma_16x16x32(a, v[m][g * STEPS + j], part_sum[m]);
         }
-        u32 z = 0x08080808u;
-        if (p.zeros) z = *(const u32*)((const unsigned char*)p.zeros + s);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) zero[i] = -1.0f - 0.0625f * (float)((z >> (8 * i)) & 255);
-        TX a[STEPS];
+        for (int i = 0; i < 4; ++i) {
+          const u32 bits = s[g][n][i / 2] >> (16 * (i & 1));
+          const float scale = p.scale_dtype == NEWT_F16
+                                  ? newt::to_f32(__builtin_bit_cast(f16, (unsigned short)bits))
+                                  : newt::bits_f32(bits << 16);
+          const float zero = -1.0f - 0.0625f * (float)((z[g][n] >> (8 * i)) & 255);
 #pragma unroll
-        for (int j = 0; j < STEPS; ++j) a[j] = widen(w[n][g * STEPS + j]);
-#pragma unroll
-        for (int m = 0; m < MT; ++m) {
-          f32x4 part_sum = (f32x4)(0.0f);
-#pragma unroll
-          for (int j = 0; j < STEPS; ++j)
-            part_sum = newt::mfma_16x16x32(a[j], v[m][g * STEPS + j], part_sum);
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            acc[n][m][i] = __builtin_fmaf(__builtin_fmaf(all[m][i], zero[i], part_sum[i]), scale[i],
+          for (int m = 0; m < MT; ++m)
+            acc[n][m][i] = __builtin_fmaf(__builtin_fmaf(all[m][i], zero, part_sum[m][i]), scale,
                                           acc[n][m][i]);
         }
       }
@@ -155,13 +157,28 @@ int launch(const newt_q4_params& p, hipStream_t stream) {
     return run("newt_q4_matmul", q4_kernel<T, NT, MT, WAVES, GROUP, GATED>, n_blocks * m_blocks,
                64 * WAVES, 0, stream, p, (int)n_blocks);
   };
-#define NEWT_TILE(NT, MT, WAVES)                                                       \
-  go(std::integral_constant<int, NT>(), std::integral_constant<int, MT>(),             \
+#define NEWT_TILE(NT, MT, WAVES)                                           \
+  go(std::integral_constant<int, NT>(), std::integral_constant<int, MT>(), \
      std::integral_constant<int, WAVES>())
-  if (p.rows <= 16) return NEWT_TILE(2, 1, 8);
-  if (p.rows <= 32) return NEWT_TILE(2, 2, 8);
-  if (p.rows <= 48) return NEWT_TILE(2, 3, 8);
-  return NEWT_TILE(2, 4, 8);
+  // Wide programs read x less often, narrow ones of many waves have more of the
+  // weights on their way where there are few: us of (NT, WAVES) for bf16, groups of 128,
+  //   1 x 16384 x 2048: (1, 16) 9.7, (2, 16) 13.3, (2, 8) 15.3, (4, 8) 24;
+  //   1 x 4096 x 6144: (1, 16) 6.7, (2, 8) 6.3, (4, 8) 8.7; 16 rows 11.2 / 7.9 / 9.8;
+  //   gated 1 x 4096 x 2 x 12288: (2, 8) 11.9, (4, 8) 13.5, (4, 4) 15.3;
+  //   16 x 4096 x 28672: (2, 8) 22, (4, 4) 17; 4 x 4096 x 128000: 62, 57;
+  //   gated 32 x 2048 x 2 x 5504 fp16, groups of 64: (2, 8) 12.3, (4, 4) 12.2, (4, 8) 9.7;
+  //   of 48 rows: 17.5, 15.4, 11.6.
+  // Two blocks at a time take as long as one or longer: waves, not the loads of a
+  // wave, hide the memory's latency (6.3 and 6.3, 13.5 and 11.9, 63.7 and 62.4 us).
+  if (p.rows <= 16) {
+    if constexpr (!GATED)
+      if (tiles <= 128) return NEWT_TILE(1, 1, 16);
+    if (tiles > 2048 || (tiles > 1024 && p.rows > 4)) return NEWT_TILE(4, 1, 4);
+    return NEWT_TILE(2, 1, 8);
+  }
+  if constexpr (GROUP > 32)  // whose scales would not fit the registers
+    if (tiles >= 512) return p.rows <= 32 ? NEWT_TILE(4, 2, 8) : NEWT_TILE(4, 3, 8);
+  return p.rows <= 32 ? NEWT_TILE(2, 2, 8) : NEWT_TILE(2, 3, 8);
 #undef NEWT_TILE
 }
 
@@ -179,7 +196,10 @@ int by_act(const newt_q4_params& p, hipStream_t stream) {
   return p.act == NEWT_ACT_NONE ? by_group<T, false>(p, stream) : by_group<T, true>(p, stream);
 }
 
-constexpr int64_t kFewRows = 64;
+// more take the tiles of q4_many.hip: us for 64 rows, gated, 4096 x 2 x 12288 bf16 44
+// here, 32 there; 2048 x 2 x 5504 fp16, groups of 64, 17 and 22; 48 rows of the first
+// 31 and 31, of the second 11.6 and 19.7
+constexpr int64_t kFewRows = 48;
 
 const char* wrong(const newt_q4_params& p) {
   if (p.rows < 0 || p.outputs < 0 || p.cols <= 0) return "bad size";

@@ -304,11 +304,15 @@ struct Plan {
     m_blocks = (p.rows + kRows - 1) / kRows;
     n_blocks = (tiles + kTiles - 1) / kTiles;
     const int64_t units = m_blocks * n_blocks;
-    const double each = 2.0 * p.rows * tiles * 16 * 4 / 4e6;  // us for a split's sums
+    // us for a block of one program on a CU, and of two side by side, by the group
+    const double one = p.group == 128 ? 1.2 : p.group == 64 ? 1.9 : 3.0;
+    const double two = p.group == 128 ? 2.2 : p.group == 64 ? 2.7 : 3.9;
+    const double each = 2.0 * p.rows * tiles * 16 * 4 / 4e6;  // for a split's sums
     double least = 1e30;
     for (int64_t n = 1; n <= 32 && n <= blocks; ++n) {
       const int64_t some = (blocks + n - 1) / n, parts = (blocks + some - 1) / some;
-      const double cost = (double)((units * parts + 255) / 256) * (double)(some + 1) * 0.6 +
+      const int64_t rounds = units * parts / 512, rest = units * parts % 512;
+      const double cost = (rounds * two + (rest > 256 ? two : rest ? one : 0.0)) * (some + 2) +
                           (parts > 1 ? 4.0 + each * parts : 0.0);
       if (cost < least) {
         least = cost;
