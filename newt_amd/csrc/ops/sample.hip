@@ -822,6 +822,14 @@ struct Part {
   Row<T> row;
   Settings o;
   int parts, part;
+  u64 bins[2], segments[2];  // read before what says whether they are needed
+  __device__ __forceinline__ void preload() {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      bins[i] = j.bins[2 * threadIdx.x + i];
+      segments[i] = j.segments[2 * threadIdx.x + i];
+    }
+  }
   __device__ __forceinline__ Part(const newt_sample_params& p, Shared& s, int64_t r, int parts_,
                                   int part_, int shift)
       : j(((Joint*)p.workspace)[r]), row(p, s, r, shift), o(p, r), parts(parts_), part(part_) {}
@@ -846,9 +854,10 @@ struct Part {
   }
   __device__ __forceinline__ typename Row<T>::End end() {
     if (o.by_count | o.by_mass) {
-      for (int i = threadIdx.x; i < kBins; i += kThreads) {
-        row.s.mass[i] = o.by_count ? 0 : j.bins[i];
-        row.s.count[i] = o.by_count ? (u32)j.bins[i] : 0;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        row.s.mass[2 * threadIdx.x + i] = o.by_count ? 0 : bins[i];
+        row.s.count[2 * threadIdx.x + i] = o.by_count ? (u32)bins[i] : 0;
       }
       __syncthreads();
     }
@@ -896,6 +905,7 @@ __global__ void __launch_bounds__(kThreads) part_sums_kernel(newt_sample_params 
   __shared__ Shared s;
   Part<T> a(p, s, blockIdx.x / parts, parts, blockIdx.x % parts, shift);
   a.own();
+  a.preload();
   if (!a.top()) return;
   if (threadIdx.x == 0) {
     s.listed = 0;
@@ -931,6 +941,11 @@ __global__ void __launch_bounds__(kThreads) part_choose_kernel(newt_sample_param
   __shared__ Shared s;
   const int64_t r = blockIdx.x;
   Part<T> a(p, s, r, parts, 0, shift);
+  a.preload();
+  const u32 n = a.j.listed;
+#pragma unroll
+  for (int i = 0; i < kList / kThreads; ++i)
+    s.list[i * kThreads + threadIdx.x] = a.j.list[i * kThreads + threadIdx.x];
   int id = -1;
   if (a.top()) {
     if (a.o.greedy) {
@@ -939,19 +954,20 @@ __global__ void __launch_bounds__(kThreads) part_choose_kernel(newt_sample_param
       a.row.fill_table();
       __syncthreads();
       const auto e = a.end();
-      const u32 n = a.j.listed;
       if (e.mode == kSlow || n > kList) {
         id = a.row.choose_slowly(a.o);
       } else {
-        for (u32 i = threadIdx.x; i < n; i += kThreads) s.list[i] = a.j.list[i];
         if (threadIdx.x == 0) {
           s.listed = n;
           if (e.edge < kBins) s.edge = s.table[e.edge];
         }
         if (e.mode == kSums) {
           const int per = (a.row.chunks + kBins - 1) / kBins;
-          for (int g = threadIdx.x; g < kBins; g += kThreads)
-            s.mass[g] = g * per < a.row.chunks ? a.j.segments[g] : 0;
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int g = 2 * threadIdx.x + i;
+            s.mass[g] = g * per < a.row.chunks ? a.segments[i] : 0;
+          }
         }
         __syncthreads();
         id = e.mode == kListed ? a.row.choose_listed(a.o, e) : a.row.choose_by_sums(a.o, e);
@@ -961,11 +977,15 @@ __global__ void __launch_bounds__(kThreads) part_choose_kernel(newt_sample_param
   if (threadIdx.x == 0) p.ids[r] = id;
 }
 
-// How many programs share a row: enough to fill the chip, each with work for its
-// waves.
+// How many programs share a row: one where there are rows for half the chip, or
+// where rows are so short that four launches cost more than they save; else enough
+// to fill the chip, each with work for its waves. us in one and in several:
+//   1 x 128000 bf16: no filter 28 / 17, top_p 56 / 37, all three 35 / 34;
+//   16 x 128000, settings of each row's own: 74 / 53; 64 x 128000, top_p 69 / 55;
+//   64 x 32000 fp32, settings of each row's own: 28 / 37; 16 x 32000 bf16 28 / 36.
 int parts_of(int64_t rows, int64_t vocab, int dtype) {
   const int64_t chunk = dtype == NEWT_F32 ? 256 : 512;
-  int64_t n = rows ? 256 / rows : 1;
+  int64_t n = rows && vocab >= 65536 ? 256 / rows : 1;
   const int64_t most = (vocab + chunk * kWaves - 1) / (chunk * kWaves);
   n = n < most ? n : most;
   n = n < kMostParts ? n : kMostParts;
