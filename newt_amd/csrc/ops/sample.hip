@@ -40,14 +40,26 @@ __device__ __forceinline__ u64 place_of(float x, u32 id) {
   return ((u64)~key_of(x) << 32) | id;
 }
 
-// The sum over this lane and those below it.
-template <typename V>
-__device__ __forceinline__ V wave_scan(V v, int lane) {
-#pragma unroll
-  for (int m = 1; m < 64; m <<= 1) {
-    const V o = __shfl_up(v, m);
-    if (lane >= m) v += o;
+// v of the lane that a DPP control names, 0 where there is none.
+template <int CTRL, int ROWS, typename V>
+__device__ __forceinline__ V lane_from(V v) {
+  if constexpr (sizeof(V) == 4) {
+    return (V)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, false);
+  } else {
+    const u32 lo = lane_from<CTRL, ROWS>((u32)v), hi = lane_from<CTRL, ROWS>((u32)(v >> 32));
+    return ((V)hi << 32) | lo;
   }
+}
+
+// The sum over this lane and those below it: in rows of 16 lanes, then row by row.
+template <typename V>
+__device__ __forceinline__ V wave_scan(V v) {
+  v += lane_from<0x111, 0xF>(v);  // row_shr:1
+  v += lane_from<0x112, 0xF>(v);
+  v += lane_from<0x114, 0xF>(v);
+  v += lane_from<0x118, 0xF>(v);
+  v += lane_from<0x142, 0xA>(v);  // row_bcast:15, to rows 1 and 3
+  v += lane_from<0x143, 0xC>(v);  // row_bcast:31, to rows 2 and 3
   return v;
 }
 
@@ -55,8 +67,8 @@ struct Shared {
   double table[kBins];  // 2^shift e^(-i / 64)
   u64 mass[kBins];      // a histogram's masses, a search's segments
   u32 count[kBins];
-  u64 list[kList];      // places of tokens
-  u64 some[kList];      // those of one bin
+  __attribute__((aligned(16))) u64 list[kList];  // places of tokens
+  __attribute__((aligned(16))) u64 some[kList];  // those of one bin
   u64 part[kWaves];
   u32 part_count[kWaves];
   float top[kWaves];
@@ -232,17 +244,18 @@ struct Row {
     const int i = threadIdx.x * 2;
     const u64 m0 = s.mass[i], m1 = s.mass[i + 1];
     const u32 c0 = s.count[i], c1 = s.count[i + 1];
-    u64 m = wave_scan(m0 + m1, lane);
-    u32 c = wave_scan(c0 + c1, lane);
+    u64 m = wave_scan(m0 + m1);
+    u32 c = wave_scan(c0 + c1);
     if (lane == 63) {
       s.part[wave] = m;
       s.part_count[wave] = c;
     }
     if (threadIdx.x == 0) s.place = kNone;
     __syncthreads();
-    for (int w = 0; w < wave; ++w) {
-      m += s.part[w];
-      c += s.part_count[w];
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      m += w < wave ? s.part[w] : 0;
+      c += w < wave ? s.part_count[w] : 0;
     }
     const u64 mb1 = before + m - m1, mb0 = mb1 - m0;
     const u32 cb1 = c - c1, cb0 = cb1 - c0;
@@ -297,11 +310,19 @@ struct Row {
   __device__ __forceinline__ void order(int n) const {
     if (n <= 256) {
       const int i = threadIdx.x;
+      if (i < 8) s.some[n + i] = ~0ull;
+      __syncthreads();
       u64 own = 0;
       int rank = 0;
       if (i < n) {
         own = s.some[i];
-        for (int j = 0; j < n; ++j) rank += s.some[j] < own;
+        for (int j = 0; j < n; j += 8) {
+          u64 other[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) other[k] = s.some[j + k];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) rank += other[k] < own;
+        }
       }
       __syncthreads();
       if (i < n) s.some[rank] = own;
@@ -356,11 +377,12 @@ struct Row {
       w[j] = i + j < n ? weight_bits(point(logit_of(s.some[i + j])).rest, entry) - kWhole : 0;
       own += w[j];
     }
-    u64 run = wave_scan(own, lane);
+    u64 run = wave_scan(own);
     if (lane == 63) s.part[wave] = run;
     __syncthreads();
     run += before - own;
-    for (int a = 0; a < wave; ++a) run += s.part[a];
+#pragma unroll
+    for (int a = 0; a < kWaves; ++a) run += a < wave ? s.part[a] : 0;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       if (i + j < n && (double)run < target) atomicMax(&s.last, s.some[i + j]);
@@ -390,24 +412,32 @@ struct Row {
     return (int)(id / CHUNK) / ((chunks + kBins - 1) / kBins);
   }
 
-  // The first id at which the running sum of f exceeds r, below the total of the
-  // segments. One wave's lanes return it.
-  template <typename F>
-  __device__ __forceinline__ int find(u64 r, F f) const {
+  // The first id at which the running sum of f over the row exceeds `share` of the
+  // segments' sum, which hold the sums of f. All threads call it; the first wave's
+  // get the id.
+  template <typename S, typename F>
+  __device__ __forceinline__ int find(S share, F f) const {
     const int per = (chunks + kBins - 1) / kBins;
-    // the segment, 64 at a time
-    int g = 0;
-    for (int at = 0; at < kBins; at += 64) {
-      const u64 m = wave_scan(s.mass[at + lane], lane);
-      const u64 over = __ballot(m > r);
-      if (over) {
-        const int l = __builtin_ctzll(over);
-        g = at + l;
-        if (l) r -= __shfl(m, l - 1);
-        break;
-      }
-      r -= __shfl(m, 63);
+    const u64 m0 = s.mass[2 * threadIdx.x], m1 = s.mass[2 * threadIdx.x + 1];
+    u64 m = wave_scan(m0 + m1), sum_all = 0;
+    if (lane == 63) s.part[wave] = m;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      m += w < wave ? s.part[w] : 0;
+      sum_all += s.part[w];
     }
+    u64 r = share(sum_all);
+    // the segment in which r lies, and what is left of it there
+    const u64 b1 = m - m1, b0 = b1 - m0;
+    if (b0 <= r && r < m) {
+      s.place = 2 * threadIdx.x + (r >= b1);
+      s.before = r - (r >= b1 ? b1 : b0);
+    }
+    __syncthreads();
+    if (wave != 0) return 0;
+    const int g = (int)s.place;
+    r = s.before;
     for (int c = g * per; c < chunks; ++c) {
       float v[V];
       u64 w[V], sum = 0;
@@ -418,14 +448,14 @@ struct Row {
         w[j] = f(v[j], i + j);
         sum += w[j];
       }
-      const u64 m = wave_scan(sum, lane);
-      const u64 over = __ballot(m > r);
+      const u64 upto = wave_scan(sum);
+      const u64 over = __ballot(upto > r);
       if (!over) {
-        r -= __shfl(m, 63);
+        r -= __shfl(upto, 63);
         continue;
       }
       const int l = __builtin_ctzll(over);
-      u64 run = m - sum;
+      u64 run = upto - sum;
       int id = 0;
       bool done = false;
 #pragma unroll
@@ -517,10 +547,9 @@ struct Row {
         if (keep >= equal) return ((u64)~top_key << 32) | 0xffffffffu;
         const auto equal_ones = [&](float f, int64_t) { return (u64)(key_of(f) == top_key); };
         segments(equal_ones);
-        if (wave == 0) {
-          const int id = find(keep - 1, equal_ones);
-          if (lane == 0) s.place = id;
-        }
+        const int first = find([&](u64) { return (u64)keep - 1; }, equal_ones);
+        __syncthreads();
+        if (threadIdx.x == 0) s.place = first;
         __syncthreads();
         const u32 id = s.place;
         __syncthreads();
@@ -661,9 +690,7 @@ struct Row {
   // The choice among what the segments hold, of the bins before `edge` and of places
   // up to `cut`.
   __device__ __forceinline__ int choose(float u, int edge, u64 cut) const {
-    const u64 sum = total();
-    if (wave != 0) return 0;
-    return find(share(u, sum), [&](float f, int64_t i) -> u64 {
+    return find([&](u64 sum) { return share(u, sum); }, [&](float f, int64_t i) -> u64 {
       const Point a = point(f);
       if (a.bin < edge) return weight(a);
       if (place_of(f, (u32)i) > cut) return 0;
@@ -737,9 +764,7 @@ struct Row {
       if (place <= cut && a.within(reach)) atomicAdd(&s.mass[segment_of((u32)place)], weight(a));
     }
     __syncthreads();
-    const u64 sum = total();
-    if (wave != 0) return 0;
-    return find(share(o.u, sum), [&](float f, int64_t i) -> u64 {
+    return find([&](u64 sum) { return share(o.u, sum); }, [&](float f, int64_t i) -> u64 {
       if (place_of(f, (u32)i) > cut) return 0;
       const Point a = point(f);
       return a.within(reach) ? weight(a) : 0;
@@ -762,8 +787,7 @@ struct Row {
       return place_of(f, (u32)i) <= cut && a.within(reach) ? weight(a) : 0;
     };
     segments(kept);
-    const u64 sum = total();
-    return wave == 0 ? find(share(o.u, sum), kept) : 0;
+    return find([&](u64 sum) { return share(o.u, sum); }, kept);
   }
 };
 
