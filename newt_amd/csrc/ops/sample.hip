@@ -229,6 +229,13 @@ struct Row {
     each(f, [](int) {});
   }
 
+  // The same a number at a time, where there is no hurry.
+  template <typename F>
+  __device__ __forceinline__ void slowly(F f) const {
+#pragma unroll 1
+    for (int i = threadIdx.x; i < vocab; i += kThreads) f(newt::to_f32(x[i]), i);
+  }
+
   __device__ __forceinline__ void clear() const {
     for (int i = threadIdx.x; i < kBins; i += kThreads) {
       s.mass[i] = 0;
@@ -290,22 +297,6 @@ struct Row {
     return sum;
   }
 
-  // The list's first `size`, a power of two, in rising order.
-  __device__ __forceinline__ void sort(int size) const {
-    for (int k = 2; k <= size; k <<= 1)
-      for (int j = k >> 1; j > 0; j >>= 1) {
-        __syncthreads();
-        for (int i = threadIdx.x; i < size / 2; i += kThreads) {
-          const int a = 2 * i - (i & (j - 1)), b = a + j;
-          const u64 u = s.list[a], v = s.list[b];
-          if ((u > v) == ((a & k) == 0)) {
-            s.list[a] = v;
-            s.list[b] = u;
-          }
-        }
-      }
-    __syncthreads();
-  }
   // The first n of `some` in rising order: by counting for few, else bitonic.
   __device__ __forceinline__ void order(int n) const {
     if (n <= 256) {
@@ -332,9 +323,13 @@ struct Row {
     int size = 512;
     while (size < n) size <<= 1;
     for (int i = n + threadIdx.x; i < size; i += kThreads) s.some[i] = ~0ull;
+    // pairs up to 64 apart are a wave's own, in order without a barrier
+    bool wide = true;
     for (int k = 2; k <= size; k <<= 1)
       for (int j = k >> 1; j > 0; j >>= 1) {
-        __syncthreads();
+        if (wide || j > 64) __syncthreads();
+        else __builtin_amdgcn_wave_barrier();
+        wide = j > 64;
         for (int i = threadIdx.x; i < size / 2; i += kThreads) {
           const int a = 2 * i - (i & (j - 1)), b = a + j;
           const u64 u = s.some[a], v = s.some[b];
@@ -392,19 +387,14 @@ struct Row {
     return s.last;
   }
 
-  // The sums of f(number, id), in segments of consecutive chunks that `find`
+  // The sums of f(number, id), slowly, in segments of consecutive chunks that `find`
   // searches; their sum is `total`.
   template <typename F>
   __device__ __forceinline__ void segments(F f) const {
-    const int per = (chunks + kBins - 1) / kBins;
-    for (int g = threadIdx.x; g < kBins; g += kThreads) s.mass[g] = 0;
-    __syncthreads();
-    u64 sum = 0;
-    each([&](float v, int64_t i) { sum += f(v, i); }, [&](int c) {
-      sum = newt::lane_reduce<newt::Sum, 63>(sum);
-      if (per == 1) s.mass[c] = sum;
-      else if (lane == 0) atomicAdd(&s.mass[c / per], sum);
-      sum = 0;
+    clear();
+    slowly([&](float v, int64_t i) {
+      const u64 w = f(v, i);
+      if (w) atomicAdd(&s.mass[segment_of(i)], w);
     });
     __syncthreads();
   }
@@ -476,7 +466,7 @@ struct Row {
   // a search by id. ~0: all stay.
   __device__ __forceinline__ u64 last(bool by_mass, u32 k, double target) const {
     clear();
-    each([&](float f, int64_t) {
+    slowly([&](float f, int64_t) {
       const Point a = point(f);
       if (a.bin < kBins - 1) {
         atomicAdd(&s.count[a.bin], 1u);
@@ -495,7 +485,7 @@ struct Row {
     for (;;) {
       // the smallest and largest key that are there
       u32 least_key = 0xffffffffu, most = 0;
-      each([&](float f, int64_t) {
+      slowly([&](float f, int64_t) {
         const u32 key = key_of(f);
         if (first ? point(f).bin == at : (key >= lo) & (key <= hi)) {
           least_key = key < least_key ? key : least_key;
@@ -519,7 +509,7 @@ struct Row {
       clear();
       const u32 range = hi - lo;
       const int bits = range < kBins ? 0 : 21 - __builtin_clz(range);  // range >> bits < kBins
-      each([&](float f, int64_t) {
+      slowly([&](float f, int64_t) {
         const u32 key = key_of(f);
         if ((key >= lo) & (key <= hi)) {
           const u32 b = (hi - key) >> bits;
