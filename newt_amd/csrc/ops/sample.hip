@@ -245,9 +245,11 @@ struct Row {
   }
 
   // Of the histogram's bins the first where the running count reaches `k` or the
-  // running mass, with `before`, reaches `target`; its place, what lies before
-  // it and what is in it to s. All threads call it; the bins are full.
-  __device__ __forceinline__ void pick(bool by_mass, u64 k, u64 before, double target) const {
+  // running mass, with `before`, reaches `target` (below 0: top_p of all there is);
+  // its place, what lies before it and what is in it to s. All threads call it; the
+  // bins are full. Returns the target.
+  __device__ __forceinline__ double pick(bool by_mass, u64 k, u64 before, double target,
+                                         float top_p = 0.0f) const {
     const int i = threadIdx.x * 2;
     const u64 m0 = s.mass[i], m1 = s.mass[i + 1];
     const u32 c0 = s.count[i], c1 = s.count[i + 1];
@@ -259,11 +261,15 @@ struct Row {
     }
     if (threadIdx.x == 0) s.place = kNone;
     __syncthreads();
+    u64 all = 0;
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) {
+      all += s.part[w];
       m += w < wave ? s.part[w] : 0;
       c += w < wave ? s.part_count[w] : 0;
     }
+    // at least the first token
+    if (target < 0.0) target = __builtin_fmax((double)top_p * (double)all, 0x1p-60);
     const u64 mb1 = before + m - m1, mb0 = mb1 - m0;
     const u32 cb1 = c - c1, cb0 = cb1 - c0;
     const auto reached = [&](u64 mass, u32 count) {
@@ -276,6 +282,7 @@ struct Row {
       found(i + 1, mb1, cb1, m1, c1);
     }
     __syncthreads();
+    return target;
   }
   __device__ __forceinline__ void found(int i, u64 before, u32 before_count, u64 m, u32 c) const {
     s.place = i;
@@ -361,10 +368,9 @@ struct Row {
     return (int)s.picked;
   }
   // The last of `some`, n in order, before which less than the target lies, with
-  // `before` in front of them all: 0 for none. All have the table entry `entry`.
+  // `before`, less than it, in front of them all. All have the table entry `entry`.
   __device__ __forceinline__ u64 last_by_mass(int n, u64 before, double target,
                                               double entry) const {
-    if (threadIdx.x == 0) s.last = 0;
     const int i = 4 * threadIdx.x;
     u64 w[4], own = 0;
 #pragma unroll
@@ -380,8 +386,10 @@ struct Row {
     for (int a = 0; a < kWaves; ++a) run += a < wave ? s.part[a] : 0;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      if (i + j < n && (double)run < target) atomicMax(&s.last, s.some[i + j]);
-      run += w[j];
+      const u64 next = run + w[j];
+      if (i + j < n && (double)run < target && (i + j + 1 == n || !((double)next < target)))
+        s.last = s.some[i + j];
+      run = next;
     }
     __syncthreads();
     return s.last;
@@ -618,10 +626,7 @@ struct Row {
   __device__ __forceinline__ End end(const Settings& o) const {
     End e = {kSums, kBins, kBins, 0, 0, 0.0};
     if (o.by_count | o.by_mass) {
-      // at least the first token
-      if (!o.by_count)
-        e.target = __builtin_fmax((double)o.top_p * (double)total(), 0x1p-60);
-      pick(!o.by_count, o.top_k, 0, e.target);
+      e.target = pick(!o.by_count, o.top_k, 0, -1.0, o.top_p);
       if (s.place != kNone) {
         e.bin = s.place;
         e.before = s.before;
@@ -677,13 +682,13 @@ struct Row {
     __syncthreads();
   }
 
-  // The choice among what the segments hold, of the bins before `edge` and of places
-  // up to `cut`.
+  // The choice among what the segments hold: of the bins before `edge` all, of that
+  // bin places up to `cut` within reach.
   __device__ __forceinline__ int choose(float u, int edge, u64 cut) const {
     return find([&](u64 sum) { return share(u, sum); }, [&](float f, int64_t i) -> u64 {
       const Point a = point(f);
       if (a.bin < edge) return weight(a);
-      if (place_of(f, (u32)i) > cut) return 0;
+      if (a.bin > edge || place_of(f, (u32)i) > cut || !a.within(reach)) return 0;
       return weight_bits(a.rest, s.edge) - kWhole;
     });
   }
@@ -703,17 +708,13 @@ struct Row {
                                                                 : s.some[o.top_k - e.before_count - 1])
                            : last_by_mass(m, e.before, e.target, s.edge);
         }
-        if (threadIdx.x == 0) s.last = 0;
-        __syncthreads();
         for (int i = threadIdx.x; i < m; i += kThreads) {
           const u64 place = s.some[i];
-          if (place > cut) continue;
-          atomicAdd(&s.mass[segment_of((u32)place)],
-                    weight_bits(point(logit_of(place)).rest, s.edge) - kWhole);
-          atomicMax(&s.last, place);
+          if (place <= cut)
+            atomicAdd(&s.mass[segment_of((u32)place)],
+                      weight_bits(point(logit_of(place)).rest, s.edge) - kWhole);
         }
         __syncthreads();
-        cut = s.last;
       }
     }
     return choose(o.u, e.edge, cut);
@@ -734,8 +735,7 @@ struct Row {
         if (place <= cut) atomicAdd(&s.mass[a.bin], weight(a));
       }
       __syncthreads();
-      const double target = __builtin_fmax((double)o.top_p * (double)total(), 0x1p-60);
-      pick(true, 0, 0, target);
+      const double target = pick(true, 0, 0, -1.0, o.top_p);
       const u32 bin = s.place;
       const u64 before = s.before;
       if (bin != kNone) {
@@ -856,12 +856,9 @@ struct Part {
   }
   // Sets the row's largest logit; false where there is nothing to choose.
   __device__ __forceinline__ bool top() {
-    float most = -kInf;
-    bool bad = o.bad;
-    for (int i = 0; i < parts; ++i) {
-      most = __builtin_fmaxf(most, j.top[i]);
-      bad |= j.bad[i] != 0;
-    }
+    const int i = threadIdx.x & 63;  // of at most 64 parts
+    const float most = newt::lane_reduce<newt::Max, 63>(i < parts ? j.top[i] : -kInf);
+    const bool bad = o.bad | (__ballot(i < parts && j.bad[i]) != 0);
     if (bad || !(__builtin_fabsf(most) < kInf)) return false;
     row.set(o, most);
     return true;
@@ -904,8 +901,8 @@ __global__ void __launch_bounds__(kThreads) part_histogram_kernel(newt_sample_pa
   __shared__ Shared s;
   Part<T> a(p, s, blockIdx.x / parts, parts, blockIdx.x % parts, shift);
   a.own();
+  a.row.fill_table();  // while the largest logits are on their way
   if (a.o.greedy || !(a.o.by_count | a.o.by_mass) || !a.top()) return;
-  a.row.fill_table();
   a.row.histogram(a.o);
   for (int i = threadIdx.x; i < kBins; i += kThreads) {
     const u64 v = a.o.by_count ? s.count[i] : s.mass[i];
@@ -920,13 +917,13 @@ __global__ void __launch_bounds__(kThreads) part_sums_kernel(newt_sample_params 
   Part<T> a(p, s, blockIdx.x / parts, parts, blockIdx.x % parts, shift);
   a.own();
   a.preload();
-  if (!a.top()) return;
+  a.row.fill_table();
   if (threadIdx.x == 0) {
     s.listed = 0;
     s.first = 0xffffffffu;
   }
-  a.row.fill_table();
   __syncthreads();
+  if (!a.top()) return;
   if (a.o.greedy) {
     a.row.first();
     if (threadIdx.x == 0) atomicMin(&a.j.first, s.first);
@@ -960,13 +957,13 @@ __global__ void __launch_bounds__(kThreads) part_choose_kernel(newt_sample_param
 #pragma unroll
   for (int i = 0; i < kList / kThreads; ++i)
     s.list[i * kThreads + threadIdx.x] = a.j.list[i * kThreads + threadIdx.x];
+  a.row.fill_table();
+  __syncthreads();
   int id = -1;
   if (a.top()) {
     if (a.o.greedy) {
       id = (int)a.j.first;
     } else {
-      a.row.fill_table();
-      __syncthreads();
       const auto e = a.end();
       if (e.mode == kSlow || n > kList) {
         id = a.row.choose_slowly(a.o);
