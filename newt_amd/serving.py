@@ -693,6 +693,8 @@ def q4_weights(q, scales, zeros=None, gated=False):
     group = K // groups
     if zeros is not None:
         _shape("q4_weights", "zeros", zeros, scales.shape, torch.uint8)
+    if N == 0:
+        raise ValueError("q4_weights: no rows")
     if gated and N % 2:
         raise ValueError(f"q4_weights: {N} rows are not a gate's and what it gates")
     if N >= 2 ** 30 or K >= 2 ** 30:
