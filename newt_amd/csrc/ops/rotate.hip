@@ -6,7 +6,10 @@
 // position, off by 2^-33 of a turn at most; its upper 32 bits give the quadrant
 // and, exactly, the rest of at most pi/4, whose sine and cosine are short sums.
 // HBM bounds it, each number read and written once. A thread keeps the angles of
-// its pairs for a token and turns several heads by them.
+// its pairs for a token and turns several heads by them; what it reads it reads
+// past the caches (non-temporal), which leaves them to the outputs: bf16 4 x (32 + 8)
+// x 4096 x 128 as slices of one product 57.8 us (5.8 TB/s, what a copy reaches) and
+// 67.6 without, 65.7 with the outputs past the caches instead, 63.5 with both.
 #include "common.h"
 
 namespace newt_ops {
@@ -34,8 +37,7 @@ __device__ __forceinline__ void cos_sin(u32 turns, float& c, float& s) {
   if (quadrant & 2) s = -s;
 }
 
-// Whether a launch turns V pairs of a head at a time; the pieces of the rest of
-// a head are 2 V long.
+// A unit is V pairs of a head; what is behind them is copied, V numbers a unit.
 template <typename T, int V, bool INTERLEAVED>
 __global__ void __launch_bounds__(256)
 rotate_kernel(newt_rotate_params p, u32 slots, u32 units, u32 threads) {
@@ -58,16 +60,15 @@ rotate_kernel(newt_rotate_params p, u32 slots, u32 units, u32 threads) {
     return h < (u32)p.heads ? qo + h * p.qo_stride_h : ko + (h - (u32)p.heads) * p.ko_stride_h;
   };
   if ((int)unit >= turned) {
-    const int d = 2 * half + ((int)unit - turned) * 2 * V;
+    const int d = 2 * half + ((int)unit - turned) * V;
+#pragma unroll 4
     for (u32 h = slot; h < heads; h += slots) {
       const T* x = from(h) + d;
       T* y = to(h) + d;
-      if (d + 2 * V <= D) {
-        T v[2 * V];
-        newt::load_vec<T, V>(x, v, newt::any_align());
-        newt::load_vec<T, V>(x + V, v + V, newt::any_align());
+      if (d + V <= D) {
+        T v[V];
+        newt::load_vec_nt<T, V>(x, v, newt::any_align());
         newt::store_vec<T, V>(y, v, newt::any_align());
-        newt::store_vec<T, V>(y + V, v + V, newt::any_align());
       } else {
         for (int j = 0; d + j < D; ++j) y[j] = x[j];
       }
@@ -76,25 +77,31 @@ rotate_kernel(newt_rotate_params p, u32 slots, u32 units, u32 threads) {
   }
   const int position = p.positions[b * p.position_stride_b + (p.each ? t * p.position_stride_t : 0)];
   const u64 at = (u64)((long long)position + (p.each ? 0 : (long long)t));
+  // Two pieces of V numbers, half of what turns apart: neighbouring lanes read
+  // neighbouring pieces. They hold the two sides of V pairs, or V / 2 pairs each (one
+  // pair where V is 1).
+  constexpr bool PAIRS = INTERLEAVED && V > 1;
+  const int d0 = (int)unit * V * (INTERLEAVED && !PAIRS ? 2 : 1);
+  const int d1 = d0 + (INTERLEAVED && !PAIRS ? 1 : half);
   float c[V], s[V];
 #pragma unroll
   for (int j = 0; j < V; ++j) {
-    const u64 turns = at * p.turns[unit * V + j];
+    const int pair = !PAIRS ? (int)unit * V + j : j < V / 2 ? d0 / 2 + j : d1 / 2 + j - V / 2;
+    const u64 turns = at * p.turns[pair];
     cos_sin((u32)((turns + 0x80000000ull) >> 32), c[j], s[j]);
     c[j] *= p.amplitude;
     s[j] *= p.transposed ? -p.amplitude : p.amplitude;
   }
-  const int d0 = (int)unit * V * (INTERLEAVED ? 2 : 1), d1 = d0 + (INTERLEAVED ? V : half);
 #pragma unroll 4
   for (u32 h = slot; h < heads; h += slots) {
     const T* x = from(h);
     T* y = to(h);
     T v[2 * V];
-    newt::load_vec<T, V>(x + d0, v, newt::any_align());
-    newt::load_vec<T, V>(x + d1, v + V, newt::any_align());
+    newt::load_vec_nt<T, V>(x + d0, v, newt::any_align());
+    newt::load_vec_nt<T, V>(x + d1, v + V, newt::any_align());
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      const int ia = INTERLEAVED ? 2 * j : j, ib = INTERLEAVED ? 2 * j + 1 : j + V;
+      const int ia = PAIRS ? 2 * j : j, ib = PAIRS ? 2 * j + 1 : j + V;
       const float a = newt::to_f32(v[ia]), e = newt::to_f32(v[ib]);
       v[ia] = (T)(a * c[j] - e * s[j]);
       v[ib] = (T)(e * c[j] + a * s[j]);
@@ -106,9 +113,10 @@ rotate_kernel(newt_rotate_params p, u32 slots, u32 units, u32 threads) {
 
 template <typename T, int V>
 int launch(const newt_rotate_params& p, hipStream_t stream) {
-  const int64_t units = p.rot_dim / 2 / V + (p.head_dim - p.rot_dim + 2 * V - 1) / (2 * V);
+  const int64_t units = p.rot_dim / 2 / V + (p.head_dim - p.rot_dim + V - 1) / V;
   const int64_t heads = p.heads + p.kv_heads, tokens = p.batch * p.tokens;
-  // a thread turns up to 8 heads, fewer where the threads would not fill the chip
+  // a thread turns up to 8 heads (of 4, 8 and 16 the large case above takes 66, 68 and
+  // 73 us without the hint), fewer where the threads would not fill the chip
   int64_t each = units * tokens * heads / (256 * 1024);
   each = each < 1 ? 1 : each > 8 ? 8 : each;
   const int64_t slots = (heads + each - 1) / each, threads = units * tokens * slots;
