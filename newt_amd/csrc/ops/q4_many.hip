@@ -107,23 +107,17 @@ q4_many_kernel(newt_q4_params p, int m_blocks, int n_blocks, int per) {
         w[f][i] = *(const u32x4*)(q + (int64_t)b * 1024 + q_at[f] + 512 * i);
   };
 
-  // The sums of 16 rows of a block, in three parts.
-  const auto add_up = [&](const T* x_lds, bf16x4* to_sums) {
-    f32x4 all = (f32x4)(0.0f);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const TX x = __builtin_bit_cast(TX, newt::lds_frag_k<T, kBlock, 16>(x_lds, 16 * wave, 32 * j, lane));
-      all = newt::mfma_16x16x32(ones, x, all);
-      if ((j + 1) % (GROUP / 32) == 0) {
-        const bf16 hi = (bf16)all[0];
-        const float rest = all[0] - (float)hi;
-        const bf16 mid = (bf16)rest;
-        if (lane < 16)
-          to_sums[j / (GROUP / 32) * kRows + 16 * wave + lane] =
-              bf16x4{hi, mid, (bf16)(rest - (float)mid), (bf16)0.0f};
-        all = (f32x4)(0.0f);
-      }
-    }
+  // The sums of 16 rows over 32 columns, and a group's in three parts.
+  const auto add_32 = [&](const T* x_lds, int k, f32x4 all) {
+    const TX x = __builtin_bit_cast(TX, newt::lds_frag_k<T, kBlock, 16>(x_lds, 16 * wave, k, lane));
+    return newt::mfma_16x16x32(ones, x, all);
+  };
+  const auto keep = [&](const f32x4& all, bf16x4* to_sums) {
+    const bf16 hi = (bf16)all[0];
+    const float rest = all[0] - (float)hi;
+    const bf16 mid = (bf16)rest;
+    if (lane < 16)
+      to_sums[16 * wave + lane] = bf16x4{hi, mid, (bf16)(rest - (float)mid), (bf16)0.0f};
   };
 
   // One block, while the one after the next is on its way: the next one is there,
@@ -135,7 +129,6 @@ q4_many_kernel(newt_q4_params p, int m_blocks, int n_blocks, int per) {
     __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
     newt::barrier_nofence();
     load(b + 2, w, next, next_levels);
-    add_up(after, next_sums);
     // not unrolled: groups side by side would not fit the registers
 #pragma unroll 1
     for (int g = 0; g < PER; ++g) {
@@ -155,9 +148,11 @@ q4_many_kernel(newt_q4_params p, int m_blocks, int n_blocks, int per) {
         for (int f = 0; f < 2; ++f) a[i & 1][f] = widen(v[f][i & 1][i / 2]);
       };
       operands(0);
+      f32x4 all = (f32x4)(0.0f);
 #pragma unroll
       for (int i = 0; i < STEPS; ++i) {
         if (i + 1 < STEPS) operands(i + 1);
+        if (i & 1) all = add_32(after, 16 * (g * STEPS + i - 1), all);
 #pragma unroll
         for (int f = 0; f < 2; ++f)
 #pragma unroll
@@ -170,6 +165,7 @@ q4_many_kernel(newt_q4_params p, int m_blocks, int n_blocks, int per) {
           __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);  // vector instructions
         }
       }
+      keep(all, next_sums + g * kRows);
       bf16x8 less_x[2];
 #pragma unroll
       for (int m = 0; m < 2; ++m) {
@@ -221,7 +217,13 @@ q4_many_kernel(newt_q4_params p, int m_blocks, int n_blocks, int per) {
   load(from + 1, w1, x1, levels1);
   newt::wait_vmcnt<0>();
   __syncthreads();
-  add_up(x0, sums[0]);
+#pragma unroll 1
+  for (int g = 0; g < PER; ++g) {
+    f32x4 all = (f32x4)(0.0f);
+#pragma unroll
+    for (int k = 0; k < GROUP; k += 32) all = add_32(x0, g * GROUP + k, all);
+    keep(all, sums[0] + g * kRows);
+  }
   for (int b = from; b < to; b += 6) {
 #define NEWT_STEP(i, X, AFTER, NEXT, S)                                                        \
   if (b + i < to)                                                                              \
