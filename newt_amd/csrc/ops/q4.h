@@ -15,15 +15,17 @@ template <> struct frag<f16> { typedef f16x8 type; };
 // the compiler, which would rather use two instructions with constants in them.
 template <typename T>
 struct Widen {
-  u32 mask, one;
+  u32 mask;
+  u32x4 ones;  // 1 in both halves: an operand of ones, too
   __device__ __forceinline__ Widen() {
     constexpr bool B = __is_same(T, bf16);  // the upper 4 of 7 bits, or of 10
     mask = B ? 0x00780078u : 0x03c003c0u;
-    one = B ? 0x3f803f80u : 0x3c003c00u;
+    ones = (u32x4)(B ? 0x3f803f80u : 0x3c003c00u);
     asm("" : "+s"(mask));
-    asm("" : "+v"(one));
+    asm("" : "+v"(ones));
   }
   __device__ __forceinline__ typename frag<T>::type operator()(u32 w) const {
+    const u32 one = ones[0];
     u32x4 r;
     if constexpr (__is_same(T, bf16)) {
       r[0] = (w & mask) | one;

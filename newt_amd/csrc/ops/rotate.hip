@@ -6,10 +6,11 @@
 // position, off by 2^-33 of a turn at most; its upper 32 bits give the quadrant
 // and, exactly, the rest of at most pi/4, whose sine and cosine are short sums.
 // HBM bounds it, each number read and written once. A thread keeps the angles of
-// its pairs for a token and turns several heads by them; what it reads it reads
-// past the caches (non-temporal), which leaves them to the outputs: bf16 4 x (32 + 8)
-// x 4096 x 128 as slices of one product 57.8 us (5.8 TB/s, what a copy reaches) and
-// 67.6 without, 65.7 with the outputs past the caches instead, 63.5 with both.
+// its pairs for a token and turns two heads by them. What it reads it reads past the
+// caches (non-temporal), which leaves them to the outputs: bf16 4 x (32 + 8) x 4096 x
+// 128 as slices of one product, outputs in the same memory every time, 56 us (6.0 TB/s)
+// and 67 without; in other memory every time 65 (5.2 TB/s) and 70. Outputs past the
+// caches too take 63 either way, but the next operator would find them in HBM.
 #include "common.h"
 
 namespace newt_ops {
@@ -115,10 +116,11 @@ template <typename T, int V>
 int launch(const newt_rotate_params& p, hipStream_t stream) {
   const int64_t units = p.rot_dim / 2 / V + (p.head_dim - p.rot_dim + V - 1) / V;
   const int64_t heads = p.heads + p.kv_heads, tokens = p.batch * p.tokens;
-  // a thread turns up to 8 heads (of 4, 8 and 16 the large case above takes 66, 68 and
-  // 73 us without the hint), fewer where the threads would not fill the chip
+  // two heads a thread, or one where the threads would not fill the chip: us of 1, 2, 4
+  // and 8 in the large case above, outputs in other memory every time, 71 / 65 / 67 /
+  // 68, interleaved 64 / 63 / 65 / 66, of 2 x 40 x 4096 x 128 in fp32 60 / 63 / 65 / 69
   int64_t each = units * tokens * heads / (256 * 1024);
-  each = each < 1 ? 1 : each > 8 ? 8 : each;
+  each = each < 1 ? 1 : each > 2 ? 2 : each;
   const int64_t slots = (heads + each - 1) / each, threads = units * tokens * slots;
   if (threads > 0xffffffffll - 256 || units > 0x7fffffff)
     return fail(NEWT_ERR_INVALID, "newt_rotate: too many tokens");

@@ -411,6 +411,16 @@ def test_sample_narrow_and_wide_rows(dtype, T, V):
                 assert got[r] == orc.sample(y[r], uniform(T, 3)[r].item(), **row), (r, scale, row)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_sample_longest_vocabularies(dtype):
+    """Segments of several chunks, weights of fewer bits."""
+    V = 1300003
+    x = rnd(2, V, dtype=dtype, seed=11, scale=2.0)
+    x[1] = 0.25
+    for settings in ({}, {"top_p": 0.9}, {"top_k": 1000, "top_p": 0.5}, {"min_p": 0.01}):
+        check_sample(x, uniform(2, 5), **settings)
+
+
 def test_sample_strides():
     base = rnd(5, 2000, dtype=F16, seed=5, scale=3.0)
     x = base[1::2, 3:1500]
