@@ -5,10 +5,10 @@
 // The weights' bytes bound it: each is read once, 16 bytes a lane in the order in
 // which the matrix unit takes it, and no number of it goes through LDS. A weight
 // becomes a 16-bit number without a conversion: its 4 bits are put below the point of
-// a number in [1, 2), (16 + q) / 16, exactly. The products' sums then hold (16 + z) /
-// 16 times the sum of x too much, which comes from one more product, of x and ones,
-// for all rows of weights that a wave has:
-//   sum_k x (q - z) = 16 (sum_k x (16 + q) / 16 - (16 + z) / 16 sum_k x)
+// a number in [1, 2), (16 + q) / 16, exactly. The products begin with minus the sum of
+// x, which comes from one more product, of x and -1, for all rows of weights that a
+// wave has; zeros take a sixteenth of it each:
+//   sum_k x (q - z) = 16 ((sum_k x (16 + q) / 16 - sum_k x) - z / 16 sum_k x)
 // Everything up to the output's rounding is fp32; the factor 16 comes last, so that
 // nothing overflows that the result does not. Where x holds an infinity its sum does,
 // and the difference is no number.
@@ -52,74 +52,80 @@ q4_kernel(newt_q4_params p, int n_blocks) {
     x[m] = (const T*)p.x + (row < p.rows ? row : p.rows - 1) * p.x_stride + 8 * part;
   }
   const Widen<T> widen;
-  const TX ones = __builtin_bit_cast(TX, widen.ones);
+  TX minus_one;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) minus_one[i] = (T)-1.0f;
   f32x4 acc[NT][MT];
 #pragma unroll
   for (int n = 0; n < NT; ++n)
 #pragma unroll
     for (int m = 0; m < MT; ++m) acc[n][m] = (f32x4)(0.0f);
 
-  for (int b = wave; b < blocks; b += WAVES) {
-    u32x4 w[NT];
-    u32x2 s[PER][NT];
-    u32 z[PER][NT];
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      w[n] = q[n][(int64_t)b * 64];
-#pragma unroll
-      for (int g = 0; g < PER; ++g) {
-        const int64_t i = at[n] + (int64_t)(b * PER + g) * 16;
-        s[g][n] = *(const u32x2*)((const unsigned short*)p.scales + i);
-        z[g][n] = p.zeros ? *(const u32*)((const unsigned char*)p.zeros + i) : 0x08080808u;
-      }
-    }
-    TX v[MT][4];
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int k = b * 128 + 32 * j < (int)p.cols ? b * 128 + 32 * j : 0;
-        T t[8];
-        newt::load_vec<T, 8>(x[m] + k, t, newt::any_align());
-        v[m][j] = __builtin_bit_cast(TX, newt::pack8(t[0], t[1], t[2], t[3], t[4], t[5], t[6], t[7]));
-      }
-#pragma unroll
-    for (int g = 0; g < PER; ++g) {
-      f32x4 all[MT];
-#pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        all[m] = (f32x4)(0.0f);
-#pragma unroll
-        for (int j = 0; j < STEPS; ++j)
-          all[m] = newt::mfma_16x16x32(ones, v[m][g * STEPS + j], all[m]);
-      }
+  const auto all_blocks = [&](auto scale_type) {
+    typedef decltype(scale_type) S;
+    for (int b = wave; b < blocks; b += WAVES) {
+      u32x4 w[NT];
+      S s[PER][NT][4];
+      u32 z[PER][NT];
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        f32x4 part_sum[MT];
+        w[n] = q[n][(int64_t)b * 64];
 #pragma unroll
-        for (int m = 0; m < MT; ++m) part_sum[m] = (f32x4)(0.0f);
+        for (int g = 0; g < PER; ++g) {
+          const int64_t i = at[n] + (int64_t)(b * PER + g) * 16;
+          newt::load_vec<S, 4>((const S*)p.scales + i, s[g][n]);
+          z[g][n] = p.zeros ? *(const u32*)((const unsigned char*)p.zeros + i) : 0x08080808u;
+        }
+      }
+      TX v[MT][4];
 #pragma unroll
-        for (int j = 0; j < STEPS; ++j) {
-          const TX a = widen(w[n][g * STEPS + j]);
+      for (int m = 0; m < MT; ++m)
 #pragma unroll
-          for (int m = 0; m < MT; ++m)
-            part_sum[m] = newt::mfma_16x16x32(a, v[m][g * STEPS + j], part_sum[m]);
+        for (int j = 0; j < 4; ++j) {
+          const int k = b * 128 + 32 * j < (int)p.cols ? b * 128 + 32 * j : 0;
+          T t[8];
+          newt::load_vec<T, 8>(x[m] + k, t, newt::any_align());
+          v[m][j] = __builtin_bit_cast(TX, newt::pack8(t[0], t[1], t[2], t[3], t[4], t[5], t[6], t[7]));
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const u32 bits = s[g][n][i / 2] >> (16 * (i & 1));
-          const float scale = p.scale_dtype == NEWT_F16
-                                  ? newt::to_f32(__builtin_bit_cast(f16, (unsigned short)bits))
-                                  : newt::bits_f32(bits << 16);
-          const float zero = -1.0f - 0.0625f * (float)((z[g][n] >> (8 * i)) & 255);
+      for (int g = 0; g < PER; ++g) {
+        // minus the sum of x, the same in all rows, and a sixteenth of it
+        f32x4 less[MT];
+        float part_of[MT];
 #pragma unroll
-          for (int m = 0; m < MT; ++m)
-            acc[n][m][i] = __builtin_fmaf(__builtin_fmaf(all[m][i], zero, part_sum[m][i]), scale,
-                                          acc[n][m][i]);
+        for (int m = 0; m < MT; ++m) {
+          less[m] = (f32x4)(0.0f);
+#pragma unroll
+          for (int j = 0; j < STEPS; ++j)
+            less[m] = newt::mfma_16x16x32(minus_one, v[m][g * STEPS + j], less[m]);
+          part_of[m] = less[m][0] * 0.0625f;
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          f32x4 sum[MT];  // of x q / 16
+#pragma unroll
+          for (int m = 0; m < MT; ++m) sum[m] = less[m];
+#pragma unroll
+          for (int j = 0; j < STEPS; ++j) {
+            const TX a = widen(w[n][g * STEPS + j]);
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+              sum[m] = newt::mfma_16x16x32(a, v[m][g * STEPS + j], sum[m]);
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float scale = newt::to_f32(s[g][n][i]), zero = (float)((z[g][n] >> (8 * i)) & 255);
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+              acc[n][m][i] = __builtin_fmaf(__builtin_fmaf(part_of[m], zero, sum[m][i]), scale,
+                                            acc[n][m][i]);
+          }
         }
       }
     }
-  }
+  };
+  if (p.scale_dtype == NEWT_F16) all_blocks(f16());
+  else all_blocks(bf16());
 #pragma unroll
   for (int n = 0; n < NT; ++n)
 #pragma unroll
