@@ -3,7 +3,7 @@
 // for the pairs of a head, f the pair's frequency, p the token's position.
 // Angles are fractions of a turn: with f / 2 pi held as a 64-bit fraction the
 // product with p modulo 2^64 is the fraction of a turn that is left, whatever the
-// position, off by 2^-33 of a turn at most; its upper 32 bits give the quadrant
+// position, off by 2^-34 of a turn at most; its upper 32 bits, rounded, give the quadrant
 // and, exactly, the rest of at most pi/4, whose sine and cosine are short sums.
 // HBM bounds it, each number read and written once. A thread keeps the angles of
 // its pairs for a token and turns two heads by them. What it reads it reads past the

@@ -532,6 +532,7 @@ struct Row {
       });
       __syncthreads();
       pick(by_mass, k - before_count, before, target);
+      if (s.place == kNone) return ~0ull;  // never: the bin holds the end
       before = s.before;
       before_count += s.before_count;
       const u32 top_key = hi - (s.place << bits);

@@ -594,7 +594,7 @@ def rotate(q, k, rotary, positions, transposed=False, q_out=None, k_out=None):
     fp16 or bf16 (any strides but along head_dim), turned as `rotary` says by
     their tokens' positions; k may be None. positions are int32, [B, S], or [B]: the
     first token's, the others follow it. They may be any, negative ones too: the
-    angle is right to 2^-30 of a radian everywhere.
+    angle is right to 2^-29 of a radian everywhere.
 
     (a, b) -> amplitude (a cos - b sin, b cos + a sin) in fp32, rounded once;
     dimensions from the rotary's on are copied. Transposed, the angle's sign is
