@@ -68,6 +68,25 @@ __device__ __forceinline__ V wave_scan(V v) {
   return v;
 }
 
+__device__ __forceinline__ u64 of_lane(u64 v, int lane) {
+  return ((u64)(u32)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32) |
+         (u32)__builtin_amdgcn_readlane((int)(u32)v, lane);
+}
+__device__ __forceinline__ u32 of_lane(u32 v, int lane) {
+  return (u32)__builtin_amdgcn_readlane((int)v, lane);
+}
+
+// What the waves' parts, one each, are in all and before this wave's.
+template <typename V>
+struct Offset {
+  V all, before;
+  __device__ __forceinline__ Offset(const V* part, int lane, int wave) {
+    const V v = wave_scan(lane < kWaves ? part[lane] : (V)0);
+    all = of_lane(v, kWaves - 1);
+    before = wave ? of_lane(v, wave - 1) : (V)0;
+  }
+};
+
 struct Shared {
   double table[kBins];  // 2^shift e^(-i / 64)
   u64 mass[kBins];      // a histogram's masses, a search's segments
@@ -266,13 +285,10 @@ struct Row {
     }
     if (threadIdx.x == 0) s.place = kNone;
     __syncthreads();
-    u64 all = 0;
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
-      all += s.part[w];
-      m += w < wave ? s.part[w] : 0;
-      c += w < wave ? s.part_count[w] : 0;
-    }
+    const Offset<u64> masses(s.part, lane, wave);
+    const u64 all = masses.all;
+    m += masses.before;
+    c += Offset<u32>(s.part_count, lane, wave).before;
     // at least the first token
     if (target < 0.0) target = __builtin_fmax((double)top_p * (double)all, 0x1p-60);
     const u64 mb1 = before + m - m1, mb0 = mb1 - m0;
@@ -302,9 +318,7 @@ struct Row {
     const u64 m = newt::lane_reduce<newt::Sum, 63>(s.mass[2 * threadIdx.x] + s.mass[2 * threadIdx.x + 1]);
     if (lane == 0) s.part[wave] = m;
     __syncthreads();
-    u64 sum = 0;
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) sum += s.part[w];
+    const u64 sum = Offset<u64>(s.part, lane, wave).all;
     __syncthreads();
     return sum;
   }
@@ -386,9 +400,7 @@ struct Row {
     u64 run = wave_scan(own);
     if (lane == 63) s.part[wave] = run;
     __syncthreads();
-    run += before - own;
-#pragma unroll
-    for (int a = 0; a < kWaves; ++a) run += a < wave ? s.part[a] : 0;
+    run += before - own + Offset<u64>(s.part, lane, wave).before;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const u64 next = run + w[j];
@@ -422,15 +434,12 @@ struct Row {
   __device__ __forceinline__ int find(S share, F f) const {
     const int per = (chunks + kBins - 1) / kBins;
     const u64 m0 = s.mass[2 * threadIdx.x], m1 = s.mass[2 * threadIdx.x + 1];
-    u64 m = wave_scan(m0 + m1), sum_all = 0;
+    u64 m = wave_scan(m0 + m1);
     if (lane == 63) s.part[wave] = m;
     __syncthreads();
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
-      m += w < wave ? s.part[w] : 0;
-      sum_all += s.part[w];
-    }
-    u64 r = share(sum_all);
+    const Offset<u64> sums_of(s.part, lane, wave);
+    m += sums_of.before;
+    u64 r = share(sums_of.all);
     // the segment in which r lies, and what is left of it there
     const u64 b1 = m - m1, b0 = b1 - m0;
     if (b0 <= r && r < m) {
@@ -594,13 +603,8 @@ struct Row {
       s.first = 0xffffffffu;
     }
     __syncthreads();
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
-      most = __builtin_fmaxf(most, s.top[w]);
-      nan |= s.bad[w] != 0;
-    }
-    bad = nan;
-    return most;
+    bad = __ballot(lane < kWaves && s.bad[lane]) != 0;
+    return newt::lane_reduce<newt::Max, 63>(lane < kWaves ? s.top[lane] : -kInf);
   }
 
   // Bins' counts, for top_k, or masses, for top_p alone.
