@@ -250,6 +250,22 @@ def test_q4_matmul_strides():
     assert W().q4_matmul(x[:0], on_gpu(*raw)).shape == (0, 50)
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_q4_matmul_many_rows_of_any_stride(dtype, group):
+    """Rows that are not aligned to 16 bytes, the same row again and again, and the
+    numbers of rows on either side of the tiles'."""
+    raw = weights(300, 896, group, seed=group, dtype=F16)
+    base = rnd(131, 1001, dtype=dtype, seed=8)
+    laid_out = on_gpu(*raw)
+    check_q4(base[1::2, 5:901], raw, laid_out=laid_out)
+    check_q4(base[7:8, :896].expand(70, 896), raw, laid_out=laid_out)
+    check_q4(base[7:8, :896].expand(9, 896), raw, laid_out=laid_out)
+    aligned = base[:, :896].contiguous()
+    for M in (48, 49, 64, 65, 128):
+        check_q4(aligned[:M], raw, laid_out=laid_out, bias=rnd(300, dtype=dtype, seed=M))
+
+
 def test_q4_matmul_common_offset():
     """Rows far from zero: what the products have too much is taken off again."""
     raw = weights(64, 2048, 128, seed=9)
@@ -409,6 +425,12 @@ def test_sample_narrow_and_wide_rows(dtype, T, V):
                 row = {k: v if k == "top_k" else torch.tensor(v, dtype=F32).item()
                        for k, v in {"temperature": temperature, **settings}.items()}
                 assert got[r] == orc.sample(y[r], uniform(T, 3)[r].item(), **row), (r, scale, row)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_sample_many_rows(dtype):
+    x = rnd(3000, 70, dtype=dtype, seed=12, scale=3.0)
+    check_sample(x, uniform(3000, 13), top_k=20, top_p=0.8)
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
