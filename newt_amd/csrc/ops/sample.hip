@@ -139,6 +139,7 @@ struct Row {
   Shared& s;
   float top;     // the largest logit
   double by;     // 64 / T
+  double most;   // of max - x: the last bin
   double reach;  // 64 ln(1 / min_p): of (max - x) 64 / T
 
   __device__ __forceinline__ Row(const newt_sample_params& p, Shared& s_, int64_t r, int shift_)
@@ -148,6 +149,7 @@ struct Row {
   __device__ __forceinline__ void set(const Settings& o, float top_) {
     top = top_;
     by = 64.0 / (double)o.temperature;
+    most = (kBins - 1) / by;
     // 2^-46 less of a weight, as little as it is rounded by, still reaches min_p
     reach = o.min_p > 0.0f ? 0x1p-40 - 64.0 * log((double)__builtin_fminf(o.min_p, 1.0f)) : 1e300;
   }
@@ -197,9 +199,10 @@ struct Row {
     __device__ __forceinline__ bool within(double reach) const { return rest + bin <= reach; }
   };
   __device__ __forceinline__ Point point(float f) const {
-    const double t = __builtin_fmin(((double)top - (double)f) * by, (double)(kBins - 1));
-    const double whole = t + 6755399441055744.0;  // 1.5 2^52: the low bits are the bin
-    return {t - (whole - 6755399441055744.0), (int)__builtin_bit_cast(u64, whole)};
+    const double d = __builtin_fmin((double)top - (double)f, most);
+    // 1.5 2^52 more: the low bits are the bin
+    const double whole = __builtin_fma(d, by, 6755399441055744.0);
+    return {__builtin_fma(d, by, 6755399441055744.0 - whole), (int)__builtin_bit_cast(u64, whole)};
   }
   // e^(-rest / 64), off by 2^-45 of it, times the table's entry, rounded to a whole
   // number by 2^52 more: its low 52 bits.
