@@ -49,7 +49,8 @@ __device__ __forceinline__ float activate(float v, int act) {
 
 // 4 neighbouring outputs of a row from `first` on.
 template <typename T>
-__device__ __forceinline__ void store4(const newt_q4_params& p, int64_t row, int64_t first, f32x4 y) {
+__device__ __forceinline__ void store4(const newt_q4_params& p, int64_t row, int64_t first,
+                                       f32x4 y) {
   const int count = p.outputs - first < 4 ? (int)(p.outputs - first) : 4;
   if (p.bias) {
 #pragma unroll

@@ -14,9 +14,9 @@
 // and the difference is no number.
 // A wave takes NT tiles of 16 weight rows, MT tiles of 16 rows of x and every
 // WAVES-th block of 128 columns; the waves' sums are joined in LDS in their order.
-// bf16, groups of 128, three sets of weights in turn: 1 x 4096 x 6144 6.1 us, of which
-// the kernel is 6 (2.2 TB/s); gated 1 x 4096 x 2 x 12288 11.3 us (4.7 TB/s); 4 x 4096 x
-// 128000 to fp32 53.5 us (5.1 TB/s; the same weights again 46).
+// bf16, groups of 128, three sets of weights in turn: 1 x 4096 x 6144 5.8 us (2.3 TB/s);
+// gated 1 x 4096 x 2 x 12288 11.7 us (4.5 TB/s); 4 x 4096 x 128000 to fp32 53.4 us
+// (5.1 TB/s; the same weights again 46).
 #include "q4.h"
 
 namespace newt_ops {
@@ -85,7 +85,8 @@ q4_kernel(newt_q4_params p, int n_blocks) {
           const int k = b * 128 + 32 * j < (int)p.cols ? b * 128 + 32 * j : 0;
           T t[8];
           newt::load_vec<T, 8>(x[m] + k, t, newt::any_align());
-          v[m][j] = __builtin_bit_cast(TX, newt::pack8(t[0], t[1], t[2], t[3], t[4], t[5], t[6], t[7]));
+          v[m][j] = __builtin_bit_cast(
+              TX, newt::pack8(t[0], t[1], t[2], t[3], t[4], t[5], t[6], t[7]));
         }
 #pragma unroll
       for (int g = 0; g < PER; ++g) {
@@ -114,7 +115,8 @@ q4_kernel(newt_q4_params p, int n_blocks) {
           }
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const float scale = newt::to_f32(s[g][n][i]), zero = (float)((z[g][n] >> (8 * i)) & 255);
+            const float scale = newt::to_f32(s[g][n][i]);
+            const float zero = (float)((z[g][n] >> (8 * i)) & 255);
 #pragma unroll
             for (int m = 0; m < MT; ++m)
               acc[n][m][i] = __builtin_fmaf(__builtin_fmaf(part_of[m], zero, sum[m][i]), scale,
@@ -137,7 +139,8 @@ q4_kernel(newt_q4_params p, int n_blocks) {
   const auto joined = [&](int n, int m, int l) {
     f32x4 t = (f32x4)(0.0f);
 #pragma unroll
-    for (int i = 0; i < WAVES; ++i) t += *(const f32x4*)(sums + i * SIZE + ((n * MT + m) * 64 + l) * 4);
+    for (int i = 0; i < WAVES; ++i)
+      t += *(const f32x4*)(sums + i * SIZE + ((n * MT + m) * 64 + l) * 4);
     return t * 16.0f;
   };
   for (int e = threadIdx.x; e < OUT * MT * 64; e += 64 * WAVES) {
@@ -161,7 +164,8 @@ template <typename T, int GROUP, bool GATED>
 int launch(const newt_q4_params& p, hipStream_t stream) {
   const int64_t tiles = (p.outputs + 15) / 16 * (GATED ? 2 : 1);
   const auto go = [&](auto nt, auto mt, auto waves) {
-    constexpr int NT = decltype(nt)::value, MT = decltype(mt)::value, WAVES = decltype(waves)::value;
+    constexpr int NT = decltype(nt)::value, MT = decltype(mt)::value;
+    constexpr int WAVES = decltype(waves)::value;
     const int64_t n_blocks = (tiles + NT - 1) / NT, m_blocks = (p.rows + 16 * MT - 1) / (16 * MT);
     if (n_blocks * m_blocks > 0x7fffffff)
       return fail(NEWT_ERR_INVALID, "newt_q4_matmul: too many rows");
@@ -214,8 +218,10 @@ constexpr int64_t kFewRows = 48;
 
 const char* wrong(const newt_q4_params& p) {
   if (p.rows < 0 || p.outputs < 0 || p.cols <= 0) return "bad size";
-  if (p.rows >= 1 << 30 || p.outputs >= 1 << 30 || p.cols >= 1 << 30) return "sizes stay below 2^30";
-  if (p.group != 32 && p.group != 64 && p.group != 128) return "groups are of 32, 64 or 128 columns";
+  if (p.rows >= 1 << 30 || p.outputs >= 1 << 30 || p.cols >= 1 << 30)
+    return "sizes stay below 2^30";
+  if (p.group != 32 && p.group != 64 && p.group != 128)
+    return "groups are of 32, 64 or 128 columns";
   if (p.cols % p.group) return "columns have to be whole groups";
   if (p.act != NEWT_ACT_NONE && p.act != NEWT_ACT_SILU && p.act != NEWT_ACT_GELU)
     return "unknown activation";

@@ -12,13 +12,14 @@
 // ahead, between its products.
 // A group's sums then take their scales on the way into the accumulators, in fp32.
 // Few programs split the columns; a second kernel adds the parts in their order.
-// bf16 512 x 4096 x 2 x 12288, gated, groups of 128: 119 us, 867 TFLOP/s; groups of 64
-// 154, of 32 216 us. The products alone, with nothing loaded, widened or scaled, took
-// 83 us of 121 (an eighth of them is what is taken off): under them the chip's power
-// lets the clock fall to 1.5 GHz or so. Beside that, one at a time, the scales cost 8%,
-// loading x 6%, its sums 5% (before they went between the products), widening and the
-// operands' reads 7%, the weights' loads 1%. fp16 333 x 8192 x 2003 in groups of 32:
-// 42 us (258 TFLOP/s), of 128 29 us.
+// bf16 512 x 4096 x 2 x 12288, gated, groups of 128: 123 us, 838 TFLOP/s (119 on
+// another card); groups of 64 155, of 32 216 us. The products alone, with nothing
+// loaded, widened or scaled, took 83 us of 121 (an eighth of them is what is taken
+// off): under them the chip's power lets the clock fall to 1.5 GHz or so. Beside
+// that, one at a time, the scales cost 8%, loading x 6%, its sums 5% (before they
+// went between the products), widening and the operands' reads 7%, the weights'
+// loads 1%. fp16 333 x 8192 x 2003 in groups of 32: 42 us (261 TFLOP/s), of 128 30
+// us.
 #include "q4.h"
 
 namespace newt_ops {
@@ -89,7 +90,8 @@ q4_many_kernel(newt_q4_params p, int m_blocks, int n_blocks, int per) {
                                to_lds + (c * 256 + 64 * wave) * 8);
       } else {
         T t[8] = {};
-        if (in) newt::load_vec<T, 8>(base + (row0 + 16 * c) * p.x_stride + k0, t, newt::any_align());
+        if (in)
+          newt::load_vec<T, 8>(base + (row0 + 16 * c) * p.x_stride + k0, t, newt::any_align());
         newt::store_vec<T, 8>(to_lds + (c * 256 + threadIdx.x) * 8, t);
       }
     }
@@ -192,8 +194,9 @@ q4_many_kernel(newt_q4_params p, int m_blocks, int n_blocks, int per) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           S t[4];
-          newt::load_vec<S, 4>(
-              (const S*)(levels + 2048 * wave) + ((own + i / 2) * PER + g) * 16 + 8 * (i & 1) + 4 * half, t);
+          newt::load_vec<S, 4>((const S*)(levels + 2048 * wave) + ((own + i / 2) * PER + g) * 16 +
+                                   8 * (i & 1) + 4 * half,
+                               t);
 #pragma unroll
           for (int j = 0; j < 4; ++j) scale[4 * i + j] = newt::to_f32(t[j]);
         }

@@ -9,7 +9,7 @@
 // its pairs for a token and turns two heads by them. What it reads it reads past the
 // caches (non-temporal), which leaves them to the outputs: bf16 4 x (32 + 8) x 4096 x
 // 128 as slices of one product, outputs in the same memory every time, 56 us (6.0 TB/s)
-// and 67 without; in other memory every time 65 (5.2 TB/s) and 70. Outputs past the
+// and 67 without; in other memory every time 64 (5.3 TB/s) and 70. Outputs past the
 // caches too take 63 either way, but the next operator would find them in HBM.
 #include "common.h"
 
@@ -125,8 +125,8 @@ int launch(const newt_rotate_params& p, hipStream_t stream) {
   if (threads > 0xffffffffll - 256 || units > 0x7fffffff)
     return fail(NEWT_ERR_INVALID, "newt_rotate: too many tokens");
   const auto kernel = p.interleaved ? rotate_kernel<T, V, true> : rotate_kernel<T, V, false>;
-  return run("newt_rotate", kernel, (threads + 255) / 256, 256, 0, stream, p, (u32)slots, (u32)units,
-             (u32)threads);
+  return run("newt_rotate", kernel, (threads + 255) / 256, 256, 0, stream, p, (u32)slots,
+             (u32)units, (u32)threads);
 }
 
 template <typename T>

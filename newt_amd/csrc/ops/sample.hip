@@ -10,9 +10,9 @@
 // read again.
 // The vector unit bounds long rows: an exponential in 64 bits takes a dozen fp64
 // instructions (by a table of 2048 and a polynomial of degree 4), and top_p needs two
-// of them a logit. bf16 256 x 100003 by top_p: 55 us, without a filter 30; 64 x 32000
-// fp32 with settings of each row's own 23.6; 1 x 128000 with all three filters 28, in
-// four kernels of 4 + 5 + 8 + 12 us, each a chain of short steps.
+// of them a logit. bf16 256 x 100003 by top_p: 53 us, without a filter 30; 64 x 32000
+// fp32 with settings of each row's own 22; 1 x 128000 with all three filters 27, in
+// four kernels of 3 + 5 + 9 + 12 us, each a chain of short steps.
 // Weights are whole numbers of 2^-45 (less for more than 2^17 ids), from
 // exponentials in 64 bits: their sums are exact, whatever the order in which
 // atomics add them, so the same row gives the same id in every call, and a border is
@@ -318,7 +318,8 @@ struct Row {
 
   // The mass of all bins.
   __device__ __forceinline__ u64 total() const {
-    const u64 m = newt::lane_reduce<newt::Sum, 63>(s.mass[2 * threadIdx.x] + s.mass[2 * threadIdx.x + 1]);
+    const u64 m =
+        newt::lane_reduce<newt::Sum, 63>(s.mass[2 * threadIdx.x] + s.mass[2 * threadIdx.x + 1]);
     if (lane == 0) s.part[wave] = m;
     __syncthreads();
     const u64 sum = Offset<u64>(s.part, lane, wave).all;
@@ -717,9 +718,10 @@ struct Row {
         cut = ~0ull;
         if (e.bin == e.edge) {
           order(m);
-          cut = o.by_count ? ((u64)m < o.top_k - e.before_count ? ~0ull
-                                                                : s.some[o.top_k - e.before_count - 1])
-                           : last_by_mass(m, e.before, e.target, s.edge);
+          const u64 left = o.top_k - e.before_count;
+          cut = !o.by_count ? last_by_mass(m, e.before, e.target, s.edge)
+                : m < left  ? ~0ull
+                            : s.some[left - 1];
         }
         for (int i = threadIdx.x; i < m; i += kThreads) {
           const u64 place = s.some[i];
@@ -1035,7 +1037,8 @@ int launch(const newt_sample_params& p, int shift, hipStream_t stream) {
   const bool none = !p.top_k && !p.top_p && !(p.top_k_all > 0 && p.top_k_all < p.vocab) &&
                     p.top_p_all >= 1.0f;
   if (status == NEWT_OK && !none)
-    status = run(what, part_histogram_kernel<T>, p.rows * parts, kThreads, 0, stream, p, parts, shift);
+    status = run(what, part_histogram_kernel<T>, p.rows * parts, kThreads, 0, stream, p, parts,
+                 shift);
   if (status == NEWT_OK)
     status = run(what, part_sums_kernel<T>, p.rows * parts, kThreads, 0, stream, p, parts, shift);
   if (status == NEWT_OK)

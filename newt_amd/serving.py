@@ -4,9 +4,9 @@ They stand beside the kernels of `newt_amd.workloads`, which re-exports them:
 `rmsnorm` beside `layernorm`, `window_attention` and `cached_attention` beside
 `attention`, `token_logprobs` and `sample` beside `softmax`, `q4_matmul` and
 `q4_gated` beside `matmul`, `rotate` in front of `kv_append`. All are forward
-only, as the others are (`rotate` transposed is its own gradient). The kernels are in csrc/ops, behind the C ABI of
-include/newt_ops.h; they are compiled ahead of time, so a first call costs no
-compilation.
+only, as the others are (`rotate` transposed is its own gradient). The kernels
+are in csrc/ops, behind the C ABI of include/newt_ops.h; they are compiled ahead
+of time, so a first call costs no compilation.
 
 As everywhere in newt, tensors have to be on the current GPU, a call launches
 on torch's current stream, synchronizes nothing and can be captured into a
