@@ -598,3 +598,29 @@ def test_offsets_past_32_bits():
     w.rotate(q, None, rot, ints([0, 9]), q_out=far)
     at = ints([0, 9])[:, None] + torch.arange(32, device="cuda")
     check_rotated(far, q, orc.frequencies(128), at)
+
+
+# ---------------------------------------------------------------------------
+# what lies at the borders of the products with 4-bit weights
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("M", [1, 20, 48, 49, 130])
+@pytest.mark.parametrize("N,K,group", [(40, 96, 32), (40, 32, 32), (2100, 160, 32), (40, 192, 64),
+                                       (8200, 320, 64)])
+def test_q4_what_lies_behind_weighs_nothing(dtype, M, N, K, group):
+    """Weights, zeros and scales behind the last column and row are any finite numbers."""
+    raw = weights(N, K, group, seed=M + K)
+    w = on_gpu(*raw)
+    g = torch.Generator().manual_seed(K)
+    words = w.q.clone()
+    scales, zeros = w.scales.clone(), w.zeros.clone()
+    for i in range(K % 128 // 32, 4):  # 32 columns each: a word of all lanes
+        words[:, -1, :, i] = torch.randint(-2 ** 31, 2 ** 31, words.shape[:1] + (64,), generator=g).cuda()
+    first = K // group
+    scales[:, first:] = torch.randn(scales[:, first:].shape, generator=g).to(scales) * 100
+    zeros[:, first:] = torch.randint(0, 256, zeros[:, first:].shape, generator=g).to(zeros)
+    rows = N % 16  # of the last tile
+    scales[-1, :, rows:], zeros[-1, :, rows:] = -1000.0, 200
+    words[-1].view(-1, 4, 16, 4)[:, :, rows:] = 0x7abcdef0
+    x = rnd(M, K, dtype=dtype, seed=M + 1)
+    check_q4(x, raw, laid_out=w._replace(q=words, scales=scales, zeros=zeros))
