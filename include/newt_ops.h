@@ -184,7 +184,7 @@ typedef struct {
   const void* x;            /* [rows, cols] of dtype, F16 or BF16 */
   const void* q;            /* weights, aligned to 16 bytes */
   const void* scales;       /* of scale_dtype, F16 or BF16, aligned to 16 bytes */
-  const void* zeros;        /* bytes 0..15, aligned to 16 bytes, or NULL: 8 */
+  const void* zeros;        /* bytes, aligned to 16 bytes, or NULL: 8 */
   const void* bias;         /* [outputs] of dtype, or NULL */
   void* out;                /* [rows, outputs] of out_dtype: dtype or F32 */
   void* workspace;          /* newt_q4_matmul_workspace() bytes, or NULL if that is 0 */

@@ -6,9 +6,9 @@
 // so that a word of weights is widened once for 64 rows and a piece of x is read
 // from LDS twice for 128 rows of weights. As for few rows the sums hold (16 + z) /
 // 16 times the sum of x too much. That is taken off within the matrix unit: one
-// more step multiplies -(16 + z) / 16, which bf16 holds exactly, by the sum of x
-// in three bf16 parts, exactly what fp32 holds; on the vector unit it would take
-// as long as widening the weights. Each wave sums 16 rows of x for all, a block
+// more step multiplies -1 and -z / 16, which bf16 holds exactly for any byte z, by
+// the sum of x in three bf16 parts, exactly what fp32 holds; on the vector unit it
+// would take as long as widening the weights. Each wave sums 16 rows of x for all, a block
 // ahead, between its products.
 // A group's sums then take their scales on the way into the accumulators, in fp32.
 // Few programs split the columns; a second kernel adds the parts in their order.
@@ -180,7 +180,7 @@ q4_many_kernel(newt_q4_params p, int m_blocks, int n_blocks, int per) {
       for (int m = 0; m < 2; ++m) {
         const bf16x4 t = own_sums[g * kRows + 32 * m + (lane & 31)];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) less_x[m][i] = i < 3 && half == 0 ? t[i] : (bf16)0.0f;
+        for (int i = 0; i < 8; ++i) less_x[m][i] = half == 0 ? t[i & 3] : (bf16)0.0f;
       }
 #pragma unroll
       for (int f = 0; f < 2; ++f) {
@@ -200,10 +200,10 @@ q4_many_kernel(newt_q4_params p, int m_blocks, int n_blocks, int per) {
 #pragma unroll
           for (int j = 0; j < 4; ++j) scale[4 * i + j] = newt::to_f32(t[j]);
         }
-        const bf16 less = (bf16)(-1.0f - 0.0625f * (float)zero);
-        bf16x8 less_a;
+        const bf16 part_of = (bf16)(-0.0625f * (float)zero);
+        bf16x8 less_a;  // by the three parts and 0, twice
 #pragma unroll
-        for (int i = 0; i < 8; ++i) less_a[i] = i < 3 ? less : (bf16)0.0f;
+        for (int i = 0; i < 8; ++i) less_a[i] = i < 4 ? (bf16)-1.0f : part_of;
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
           part[f][m] = newt::mfma_32x32x16(less_a, less_x[m], part[f][m]);

@@ -670,8 +670,8 @@ def q4_weights(q, scales, zeros=None, gated=False):
     """Weights [N, K] of 4 bits, laid out once for q4_matmul or, gated, for q4_gated:
     (number - zero) * scale. q [N, K / 2] uint8 holds two neighbouring columns'
     numbers a byte, the first one's in the lower half. scales [N, K / group] fp16
-    or bf16 and zeros, uint8 as scales (8 without), are for groups of 32, 64 or 128
-    columns. Of gated weights the first N / 2 rows are the gate's."""
+    or bf16 and zeros, any uint8 as scales (8 without), are for groups of 32, 64 or
+    128 columns. Of gated weights the first N / 2 rows are the gate's."""
     for name, t in (("q", q), ("scales", scales)) + ((("zeros", zeros),) if zeros is not None else ()):
         if not isinstance(t, torch.Tensor):
             raise TypeError(f"q4_weights: {name} must be a tensor")

@@ -624,3 +624,14 @@ def test_q4_what_lies_behind_weighs_nothing(dtype, M, N, K, group):
     words[-1].view(-1, 4, 16, 4)[:, :, rows:] = 0x7abcdef0
     x = rnd(M, K, dtype=dtype, seed=M + 1)
     check_q4(x, raw, laid_out=w._replace(q=words, scales=scales, zeros=zeros))
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("M", [3, 33, 48, 49, 130])
+def test_q4_matmul_zeros_of_any_byte(M, group):
+    q, s, z = weights(100, 384, group, seed=M)
+    z = torch.randint(0, 256, z.shape, generator=torch.Generator().manual_seed(M)).to(torch.uint8)
+    z[:40] |= 0xf1  # odd ones from 241 on
+    x = rnd(M, 384, dtype=BF16, seed=M)
+    check_q4(x, (q, s, z), out_dtype=F32)
+    check_q4(x.half(), (q, s, z))
