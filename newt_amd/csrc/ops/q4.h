@@ -9,18 +9,28 @@ template <typename T> struct frag;
 template <> struct frag<bf16> { typedef bf16x8 type; };
 template <> struct frag<f16> { typedef f16x8 type; };
 
-// 8 weights to (16 + q) / 16: the 4 bits go below the point of a number in [1, 2),
-// by one shift and one v_and_or_b32 for two of them. That instruction takes one
-// constant from a scalar register and none from the code, so both are kept from
-// the compiler, which would rather use two instructions with constants in them.
+// What weights are multiplied by as operands, a power of two: sums hold this times
+// x (16 + q) / 16 for the columns of a group. Where x is bf16 they would leave fp32's
+// range long before the result does; of 128 columns and zeros of any byte none comes
+// to 2^128 this way (16 x 2^7 x 2^128 / 2^12). Sums below 2^-110 pay: they
+// lose up to 2^-133 an addition.
+template <typename T> constexpr float kUnit = __is_same(T, bf16) ? 0x1p-12f : 1.0f;
+// A group's sum (q - z) x from what is summed.
+template <typename T> constexpr float kWhole = 16.0f / kUnit<T>;
+
+// 8 weights to kUnit (16 + q) / 16: the 4 bits go below the point of a number in
+// [kUnit, 2 kUnit), by one shift and one v_and_or_b32 for two of them. That
+// instruction takes one constant from a scalar register and none from the code, so
+// both are kept from the compiler, which would rather use two instructions with
+// constants in them.
 template <typename T>
 struct Widen {
   u32 mask;
-  u32x4 ones;  // 1 in both halves: an operand of ones, too
+  u32x4 ones;  // kUnit in both halves: an operand of these, too
   __device__ __forceinline__ Widen() {
     constexpr bool B = __is_same(T, bf16);  // the upper 4 of 7 bits, or of 10
     mask = B ? 0x00780078u : 0x03c003c0u;
-    ones = (u32x4)(B ? 0x3f803f80u : 0x3c003c00u);
+    ones = (u32x4)(B ? 0x39803980u : 0x3c003c00u);
     asm("" : "+s"(mask));
     asm("" : "+v"(ones));
   }

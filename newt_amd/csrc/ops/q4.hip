@@ -9,9 +9,10 @@
 // x, which comes from one more product, of x and -1, for all rows of weights that a
 // wave has; zeros take a sixteenth of it each:
 //   sum_k x (q - z) = 16 ((sum_k x (16 + q) / 16 - sum_k x) - z / 16 sum_k x)
-// Everything up to the output's rounding is fp32; the factor 16 comes last, so that
-// nothing overflows that the result does not. Where x holds an infinity its sum does,
-// and the difference is no number.
+// Everything up to the output's rounding is fp32; the factor 16 comes last, and for
+// bf16 all of it is held 2^-12 times as large (kUnit), so that no group's sums overflow
+// for any finite x and nothing does that the result does not. Where x holds an
+// infinity its sum does, and the difference is no number.
 // A wave takes NT tiles of 16 weight rows, MT tiles of 16 rows of x and every
 // WAVES-th block of 128 columns; the waves' sums are joined in LDS in their order.
 // bf16, groups of 128, three sets of weights in turn: 1 x 4096 x 6144 5.8 us (2.3 TB/s);
@@ -52,9 +53,9 @@ q4_kernel(newt_q4_params p, int n_blocks) {
     x[m] = (const T*)p.x + (row < p.rows ? row : p.rows - 1) * p.x_stride + 8 * part;
   }
   const Widen<T> widen;
-  TX minus_one;
+  TX minus;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) minus_one[i] = (T)-1.0f;
+  for (int i = 0; i < 8; ++i) minus[i] = (T)-kUnit<T>;
   f32x4 acc[NT][MT];
 #pragma unroll
   for (int n = 0; n < NT; ++n)
@@ -102,7 +103,7 @@ q4_kernel(newt_q4_params p, int n_blocks) {
           less[m] = (f32x4)(0.0f);
 #pragma unroll
           for (int j = 0; j < STEPS; ++j)
-            less[m] = newt::mfma_16x16x32(minus_one, v[m][g * STEPS + j], less[m]);
+            less[m] = newt::mfma_16x16x32(minus, v[m][g * STEPS + j], less[m]);
           part_of[m] = less[m][0] * 0.0625f;
         }
 #pragma unroll
@@ -145,7 +146,7 @@ q4_kernel(newt_q4_params p, int n_blocks) {
 #pragma unroll
     for (int i = 0; i < WAVES; ++i)
       t += *(const f32x4*)(sums + i * SIZE + ((n * MT + m) * 64 + l) * 4);
-    return t * 16.0f;
+    return t * kWhole<T>;
   };
   for (int e = threadIdx.x; e < OUT * MT * 64; e += 64 * WAVES) {
     const int l = e & 63, m = e / 64 % MT, n = e / 64 / MT;

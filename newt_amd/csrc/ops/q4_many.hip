@@ -8,9 +8,10 @@
 // 16 times the sum of x too much. That is taken off within the matrix unit: one
 // more step multiplies -1 and -z / 16, which bf16 holds exactly for any byte z, by
 // the sum of x in three bf16 parts, exactly what fp32 holds; on the vector unit it
-// would take as long as widening the weights. Each wave sums 16 rows of x for all, a block
-// ahead, between its products.
-// A group's sums then take their scales on the way into the accumulators, in fp32.
+// would take as long as widening the weights. Each wave sums 16 rows of x for all, a
+// block ahead, between its products. A group's sums then take their scales on the
+// way into the accumulators, in fp32; up to the output all is held kUnit / 16 times
+// as large.
 // Few programs split the columns; a second kernel adds the parts in their order.
 // bf16 512 x 4096 x 2 x 12288, gated, groups of 128: 123 us, 838 TFLOP/s (119 on
 // another card); groups of 64 155, of 32 216 us. The products alone, with nothing
@@ -116,7 +117,7 @@ q4_many_kernel(newt_q4_params p, int m_blocks, int n_blocks, int per) {
         w[f][i] = *(const u32x4*)(q + (int64_t)b * 1024 + q_at[f] + 512 * i);
   };
 
-  // The sums of 16 rows over 32 columns, and a group's in three parts.
+  // The sums of 16 rows over 32 columns, times kUnit, and a group's in three parts.
   const auto add_32 = [&](const T* x_lds, int k, f32x4 all) {
     const TX x = __builtin_bit_cast(TX, newt::lds_frag_k<T, kBlock, 16>(x_lds, 16 * wave, k, lane));
     return newt::mfma_16x16x32(ones, x, all);
@@ -259,20 +260,20 @@ q4_many_kernel(newt_q4_params p, int m_blocks, int n_blocks, int per) {
       for (int i = 0; i < 4; ++i) {
         const int t = tile + 2 * f + i / 2, in_tile = 8 * (i & 1) + 4 * half;
         if (t >= tiles) continue;
-        const auto quad = [&](int j) {
+        const auto part_of = [&](int j) {
           return f32x4{acc[f][m][4 * j], acc[f][m][4 * j + 1], acc[f][m][4 * j + 2],
-                       acc[f][m][4 * j + 3]} * 16.0f;
+                       acc[f][m][4 * j + 3]};
         };
         if (!whole) {
           float* to_part = (float*)p.workspace + ((int64_t)split * p.rows + m0 + row) * tiles * 16;
-          *(f32x4*)(to_part + t * 16 + in_tile) = quad(i);
+          *(f32x4*)(to_part + t * 16 + in_tile) = part_of(i);
         } else if (!gated) {
           const int64_t first = (int64_t)t * 16 + in_tile;
-          if (first < p.outputs) store4<T>(p, m0 + row, first, quad(i));
+          if (first < p.outputs) store4<T>(p, m0 + row, first, part_of(i) * kWhole<T>);
         } else if (i < 2) {
           const int64_t first = (int64_t)(t / 2) * 16 + in_tile;
-          f32x4 y = quad(i + 2);
-          const f32x4 gate = quad(i);
+          f32x4 y = part_of(i + 2) * kWhole<T>;
+          const f32x4 gate = part_of(i) * kWhole<T>;
 #pragma unroll
           for (int c = 0; c < 4; ++c) y[c] *= activate(gate[c], p.act);
           if (first < p.outputs) store4<T>(p, m0 + row, first, y);
@@ -294,7 +295,7 @@ __global__ void __launch_bounds__(256) q4_join_kernel(newt_q4_params p, int spli
     const float* from = (const float*)p.workspace + row * width + at;
     f32x4 y = *(const f32x4*)from;
     for (int s = 1; s < splits; ++s) y += *(const f32x4*)(from + s * p.rows * width);
-    return y;
+    return y * kWhole<T>;
   };
   if (!gated) {
     store4<T>(p, row, first, joined(first));

@@ -635,3 +635,44 @@ def test_q4_matmul_zeros_of_any_byte(M, group):
     x = rnd(M, 384, dtype=BF16, seed=M)
     check_q4(x, (q, s, z), out_dtype=F32)
     check_q4(x.half(), (q, s, z))
+
+
+def check_q4_bound(x, raw, laid_out=None, out_dtype=F32):
+    """Each number within the roundings of its sums, whatever the sums' cancellation."""
+    got = W().q4_matmul(x, on_gpu(*raw) if laid_out is None else laid_out, out_dtype=out_dtype)
+    want, bound = q4_bound(x.cpu(), *raw)
+    step = half_step(out_dtype)
+    assert bool(((got.double().cpu() - want).abs() <= bound * (1 + step) + want.abs() * step).all())
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("M", [3, 33, 60, 200])
+def test_q4_matmul_of_the_largest_numbers(M, group):
+    """Rows of one sign near the largest bf16, with finite results: their sums are far
+    beyond fp32, and so are those of x times a number."""
+    q, s, z = weights(70, 512, group, seed=M)
+    s = s * 2.0 ** -13
+    z[::3] = 255
+    g = torch.Generator().manual_seed(M)
+    x = ((torch.rand(M, 512, generator=g) + 1.0) * 2.0 ** 126 * 1.98).to(BF16)
+    x[::2] *= -1
+    x[1::4] *= torch.randint(0, 2, x[1::4].shape, generator=g) * 2 - 1
+    x = x.cuda()
+    assert bool(x.isfinite().all())
+    check_q4_bound(x, (q, s, z))
+    check_q4_bound(x, (q, s, None))
+
+
+@pytest.mark.parametrize("M", [3, 60])
+def test_q4_matmul_of_the_smallest_numbers(M):
+    """Sums are held 2^16 times smaller than the results: 160 roundings of at most
+    2^-149 each, times the scale."""
+    q, s, z = weights(70, 256, 64, seed=M)
+    g = torch.Generator().manual_seed(M)
+    x = (torch.randn(M, 256, generator=g) * 2.0 ** torch.randint(-126, -90, (M, 256), generator=g))
+    x = x.to(BF16).cuda()
+    s = (s * 64).contiguous()
+    got = W().q4_matmul(x, on_gpu(q, s, z), out_dtype=F32)
+    want, bound = q4_bound(x.cpu(), q, s, z)
+    bound = bound + (160 * 4 * 2.0 ** -133 * s.double().abs().amax(1) + 2.0 ** -149)[None]
+    assert bool(((got.double().cpu() - want).abs() <= bound * (1 + EPS)).all())
