@@ -54,7 +54,9 @@ struct Widen {
 
 __device__ __forceinline__ float activate(float v, int act) {
   if (act == NEWT_ACT_SILU) return v / (1.0f + __builtin_expf(-v));
-  return 0.5f * v * (1.0f + erff(v * 0.70710678f));
+  // 1 + erf cancels below 0: 4% off at -5. 512 x 4096 x 2 x 12288 takes 129 us with erfc, 125
+  // with erf, one row 12 with either.
+  return 0.5f * v * erfcf(v * -0.70710678f);
 }
 
 // 4 neighbouring outputs of a row from `first` on.

@@ -676,3 +676,18 @@ def test_q4_matmul_of_the_smallest_numbers(M):
     want, bound = q4_bound(x.cpu(), q, s, z)
     bound = bound + (160 * 4 * 2.0 ** -133 * s.double().abs().amax(1) + 2.0 ** -149)[None]
     assert bool(((got.double().cpu() - want).abs() <= bound * (1 + EPS)).all())
+
+
+@pytest.mark.parametrize("M", [1, 20, 60])
+def test_q4_gated_gelu_of_negative_gates(M):
+    """v (1 + erf(v / sqrt 2)) / 2 cancels below 0 unless it is v erfc(-v / sqrt 2) / 2. The
+    argument is off by 1.3 roundings of fp32, of which erfc's relative slope there, 2 v^2 / 2
+    + 1, makes 190 at v = -12; erfc itself by 32 at most, three products by 3."""
+    q = torch.full((32, 64), 0x99, dtype=torch.uint8)  # weights of 1 everywhere
+    laid_out = on_gpu(q, torch.ones(32, 1, dtype=BF16), None, gated=True)
+    for v in torch.linspace(-12.0, -0.25, 48).to(BF16).tolist():
+        x = torch.zeros(M, 128, dtype=BF16, device="cuda")
+        x[:, 0] = v
+        got = W().q4_gated(x, laid_out, act="gelu").double().cpu()
+        want = 0.5 * v * math.erfc(-v / math.sqrt(2.0)) * v
+        assert bool(((got - want).abs() <= abs(want) * (2.0 ** -16 + half_step(BF16))).all()), v
