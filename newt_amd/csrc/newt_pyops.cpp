@@ -397,7 +397,8 @@ PyObject* rotate(PyObject* const* a, int64_t device, void* stream) {
 // x and laid out weights; the outputs' sizes are left to the caller
 bool q4(PyObject* x_, PyObject* w, int64_t device, bool gated, newt_q4_params* p, Arg* x) {
   *x = Arg(x_, device);
-  if (!x->ok || !PyTuple_Check(w) || PyTuple_GET_SIZE(w) != 7) return false;
+  // Q4Weights, a subclass of tuple, and no tuple of the same seven
+  if (!x->ok || !PyTuple_Check(w) || PyTuple_CheckExact(w) || PyTuple_GET_SIZE(w) != 7) return false;
   const Arg q(PyTuple_GET_ITEM(w, 0), device), scales(PyTuple_GET_ITEM(w, 1), device),
       zeros(PyTuple_GET_ITEM(w, 2), device, true);
   int64_t outputs, cols, group;

@@ -691,3 +691,12 @@ def test_q4_gated_gelu_of_negative_gates(M):
         got = W().q4_gated(x, laid_out, act="gelu").double().cpu()
         want = 0.5 * v * math.erfc(-v / math.sqrt(2.0)) * v
         assert bool(((got - want).abs() <= abs(want) * (2.0 ** -16 + half_step(BF16))).all()), v
+
+
+def test_weights_are_what_q4_weights_gives():
+    """A plain tuple of the same seven is not taken, in C++ or Python."""
+    raw = weights(40, 256, 128)
+    w, x = on_gpu(*raw), rnd(3, 256, dtype=BF16)
+    for bad in (tuple(w), list(w)):
+        with pytest.raises(TypeError, match="Q4Weights"):
+            W().q4_matmul(x, bad)
