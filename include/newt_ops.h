@@ -187,7 +187,8 @@ typedef struct {
   const void* zeros;        /* bytes, aligned to 16 bytes, or NULL: 8 */
   const void* bias;         /* [outputs] of dtype, or NULL */
   void* out;                /* [rows, outputs] of out_dtype: dtype or F32 */
-  void* workspace;          /* newt_q4_matmul_workspace() bytes, or NULL if that is 0 */
+  void* workspace;          /* newt_q4_matmul_workspace() bytes, aligned to 16, or NULL if that
+                             * is 0 */
   int64_t rows, cols, outputs;
   int64_t x_stride, out_stride;
   int32_t group;            /* 32, 64 or 128; divides cols */

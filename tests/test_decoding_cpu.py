@@ -242,6 +242,18 @@ def test_c_entries_refuse():
         call(L.newt_sample, serving._SAMPLE.pack(*bad), message)
 
 
+def test_q4_workspace_has_to_be_aligned():
+    """Splits' sums are written 16 bytes at a time."""
+    L = serving.lib()
+    P = 4096
+    many = [P, P, P, P, 0, P, 0, 100, 1 << 20, 40, 1 << 20, 40, 64, 2, 1, 2, 0, 0]
+    assert L.newt_q4_matmul_workspace(serving._Q4.pack(*many)) > 0
+    for workspace in (0, P + 4, P + 8):
+        many[6] = workspace
+        assert L.newt_q4_matmul(serving._Q4.pack(*many), None) == 10002
+        assert b"workspace" in L.newt_ops_last_error()
+
+
 def test_empty_calls_launch_nothing():
     L = serving.lib()
     P = 4096
