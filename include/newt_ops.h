@@ -186,7 +186,7 @@ typedef struct {
   const void* scales;       /* of scale_dtype, F16 or BF16, aligned to 16 bytes */
   const void* zeros;        /* bytes, aligned to 16 bytes, or NULL: 8 */
   const void* bias;         /* [outputs] of dtype, or NULL */
-  void* out;                /* [rows, outputs] of out_dtype: dtype or F32 */
+  void* out;                /* [rows, outputs] of out_dtype: dtype or F32; not over x or bias */
   void* workspace;          /* newt_q4_matmul_workspace() bytes, aligned to 16, or NULL if that
                              * is 0 */
   int64_t rows, cols, outputs;

@@ -1,6 +1,7 @@
 // What the products with 4-bit weights share: from a word of weights to an operand
 // of the matrix unit, and from sums to outputs.
 #pragma once
+#include "byte_rows.h"
 #include "common.h"
 
 namespace newt_ops {
@@ -80,6 +81,14 @@ __device__ __forceinline__ void store4(const newt_q4_params& p, int64_t row, int
     if (count == 4) newt::store_vec<T, 4>(out, t, newt::any_align());
     else for (int i = 0; i < count; ++i) out[i] = t[i];
   }
+}
+
+// Whether out lies over x or bias, which programs read while others write.
+inline bool out_meets(const newt_q4_params& p) {
+  const int64_t size = p.out_dtype == NEWT_F32 ? 4 : 2;
+  const ByteRows out(p.out, p.rows, p.out_stride * size, p.outputs * size);
+  return rows_meet(out, ByteRows(p.x, p.rows, p.x_stride * 2, p.cols * 2)) ||
+         rows_meet(out, ByteRows(p.bias, p.bias ? 1 : 0, 0, p.outputs * 2));
 }
 
 // q4_many.hip: products with many rows of x.

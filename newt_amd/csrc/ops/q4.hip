@@ -74,7 +74,7 @@ q4_kernel(newt_q4_params p, int n_blocks) {
 #pragma unroll
         for (int g = 0; g < PER; ++g) {
           const int64_t i = at[n] + (int64_t)(b * PER + g) * 16;
-          // 0 for a group behind the last column, which a block's first one never is: 0 to 4%
+          // 0 for a group behind the last column, which a block's first one never is: 0 to 5%
           // of a call; a branch around such groups takes up to a third, zeros for x 12%
           u32x2 bits = *(const u32x2*)((const S*)p.scales + i);
           if (g > 0) bits &= b * 128 + g * GROUP < (int)p.cols ? ~0u : 0u;
@@ -259,5 +259,6 @@ extern "C" int newt_q4_matmul(const newt_q4_params* params, void* stream) {
     return fail(NEWT_ERR_INVALID, "newt_q4_matmul: weights are not aligned");
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (p.rows > kFewRows) return q4_many(p, s);
+  if (out_meets(p)) return fail(NEWT_ERR_INVALID, "newt_q4_matmul: out overlaps x or bias");
   return p.dtype == NEWT_F16 ? by_act<f16>(p, s) : by_act<bf16>(p, s);
 }

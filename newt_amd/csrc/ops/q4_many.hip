@@ -347,6 +347,7 @@ int launch(const newt_q4_params& p, hipStream_t stream) {
   if (grid > 0x7fffffff) return fail(NEWT_ERR_INVALID, "newt_q4_matmul: too many rows");
   if (r.splits > 1 && (!p.workspace || ((uintptr_t)p.workspace & 15)))
     return fail(NEWT_ERR_INVALID, "newt_q4_matmul: null or unaligned workspace");
+  if (out_meets(p)) return fail(NEWT_ERR_INVALID, "newt_q4_matmul: out overlaps x or bias");
   // whole pieces of 16 bytes, within 2^31 bytes of a program's first
   const bool direct = p.x_stride % 8 == 0 && ((uintptr_t)p.x & 15) == 0 && p.x_stride >= 0 &&
                       p.x_stride < 1 << 23;

@@ -783,7 +783,8 @@ def q4_matmul(x, w, bias=None, out_dtype=None, out=None):
     [N] is of x's dtype. Products are summed in fp32 and multiplied there by their
     group's scale; the result is rounded once. For few rows the weights are read
     once; for many, matmul over weights of 16 bits is faster. A row of x that holds
-    an infinity or NaN gives no numbers."""
+    an infinity or NaN gives no numbers. An `out` given shares no memory with x or
+    bias."""
     r = _fast("q4_matmul", x, w, bias, -1 if out_dtype is None else _DTYPE.get(out_dtype, -2), out)
     if r is not None:
         return r
@@ -810,8 +811,8 @@ def q4_gated(x, w, act="silu", out=None):
     """act(x Wg) * (x Wu) [M, F] in x's dtype, the first half of a gated feed-forward
     block: x [M, K] fp16 or bf16, w of q4_weights(..., gated=True) with the 2 F rows
     of Wg and Wu transposed. act is silu, v / (1 + e^-v), or gelu, v (1 + erf(v / sqrt
-    2)) / 2. Both products stay in fp32 until the result is rounded; x as in
-    q4_matmul."""
+    2)) / 2. Both products stay in fp32 until the result is rounded; x and `out`
+    as in q4_matmul."""
     r = _fast("q4_gated", x, w, act, out)
     if r is not None:
         return r

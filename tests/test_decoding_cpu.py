@@ -242,6 +242,66 @@ def test_c_entries_refuse():
         call(L.newt_sample, serving._SAMPLE.pack(*bad), message)
 
 
+def test_q4_refuses_an_out_over_its_inputs():
+    L = serving.lib()
+    P = 1 << 40
+
+    def refused(rows, out, bias=0, out_dtype=2, workspace=1 << 20):
+        assert L.newt_q4_matmul(serving._Q4.pack(
+            P, 1 << 20, 1 << 20, 0, bias, out, workspace, rows, 256, 40, 256, 40, 64, 2, 1, out_dtype,
+            0, 0), None) == 10002
+        assert b"out overlaps x or bias" in L.newt_ops_last_error()
+
+    for rows in (1, 3, 48, 49, 500):
+        for out in (P, P + 2, P - 78, P + 512 * rows - 2):
+            refused(rows, out)
+        refused(rows, P - 158, out_dtype=0)
+        for bias in (1 << 30, (1 << 30) + 80 * rows - 2, (1 << 30) - 78):
+            refused(rows, 1 << 30, bias)
+
+
+def test_rows_that_meet(tmp_path):
+    """The check of outputs over inputs against every pair of rows."""
+    src = tmp_path / "meet.cpp"
+    src.write_text('''
+#include <cstdio>
+#include <cstdlib>
+#include "byte_rows.h"
+using namespace newt_ops;
+int main() {
+  srand(1);
+  int seen[2] = {0, 0};
+  for (int n = 0; n < 400000; ++n) {
+    int64_t v[8];
+    for (int i = 0; i < 2; ++i) {
+      v[4 * i] = 1000 + rand() % 200;
+      v[4 * i + 1] = rand() % 6;
+      v[4 * i + 2] = rand() % 81 - 20;
+      v[4 * i + 3] = 1 + rand() % 30;
+    }
+    if (n % 2) v[6] = v[2];
+    bool meet = false;
+    for (int64_t i = 0; i < v[1]; ++i)
+      for (int64_t j = 0; j < v[5]; ++j) {
+        const int64_t a = v[0] + i * v[2], b = v[4] + j * v[6];
+        meet |= a < b + v[7] && b < a + v[3];
+      }
+    const ByteRows a((void*)v[0], v[1], v[2], v[3]), b((void*)v[4], v[5], v[6], v[7]);
+    if (rows_meet(a, b) != meet || rows_meet(b, a) != meet) {
+      for (int64_t x : v) printf("%ld ", (long)x);
+      return 1;
+    }
+    ++seen[meet];
+  }
+  return seen[0] < 100000 || seen[1] < 100000;
+}
+''')
+    subprocess.run(["g++", "-std=c++17", "-I" + os.path.join(ROOT, "newt_amd/csrc/ops"), str(src), "-o",
+                    str(tmp_path / "meet")], check=True)
+    out = subprocess.run([str(tmp_path / "meet")], capture_output=True, text=True)
+    assert out.returncode == 0, out.stdout
+
+
 def test_q4_workspace_has_to_be_aligned():
     """Splits' sums are written 16 bytes at a time."""
     L = serving.lib()

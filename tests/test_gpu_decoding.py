@@ -700,3 +700,29 @@ def test_weights_are_what_q4_weights_gives():
     for bad in (tuple(w), list(w)):
         with pytest.raises(TypeError, match="Q4Weights"):
             W().q4_matmul(x, bad)
+
+
+@pytest.mark.parametrize("M", [5, 48, 100])
+def test_q4_outputs_beside_their_inputs(M):
+    """Columns of the same rows, rows between x's rows; over x or bias they are refused."""
+    raw = weights(64, 256, 64, seed=13)
+    laid_out, x = on_gpu(*raw), rnd(M, 256, dtype=BF16, seed=14)
+    base = torch.zeros(2 * M + 1, 400, dtype=BF16, device="cuda")
+    base[:M, 64:320], base[M:2 * M, 300:364] = x, 7.0
+    a = base[:M, 64:320]
+    for out in (base[:M, :64], base[:M, 320:384]):
+        check_q4(a, raw, laid_out=laid_out, out=out)
+    base[1:2 * M:2, :256] = x
+    b = base[1:2 * M:2, :256]
+    check_q4(b, raw, laid_out=laid_out, out=base[:2 * M:2, 100:164])
+    check_q4(b, raw, laid_out=laid_out, out=base[2:2 * M + 1:2, :64])
+    kept = base.clone()
+    for out in (base[1:2 * M:2, :64], base[1:2 * M:2, 250:314], base[:M, 100:164]):
+        with pytest.raises(ValueError, match="overlaps"):
+            W().q4_matmul(b, laid_out, out=out)
+    with pytest.raises(ValueError, match="overlaps"):
+        W().q4_matmul(x, laid_out, bias=base[M + 1, 300:364], out=base[:M + 2, 300:364][2:])
+    gated = on_gpu(*raw, gated=True)
+    with pytest.raises(ValueError, match="overlaps"):
+        W().q4_gated(b, gated, out=base[1:2 * M:2, 224:256])
+    assert torch.equal(base, kept)
