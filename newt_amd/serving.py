@@ -536,13 +536,14 @@ class Rotary(NamedTuple):
 
 
 _PI = decimal.Decimal("3.14159265358979323846264338327950288419716939937510")
+_MOST_TURNS = 10 ** 30  # of which 50 digits of pi give 2^-64
 
 
 def rotary(dim, base=10000.0, factor=1.0, ramp=None, amplitude=1.0, interleaved=False,
            frequencies=None, device=None):
     """The Rotary of heads whose first `dim` dimensions turn: pair i by base^(-2 i /
-    dim) radians a position, or by frequencies[i]. Pairs are (i, i + dim / 2), or
-    (2 i, 2 i + 1) where interleaved.
+    dim) radians a position, or by frequencies[i], 1e30 turns at most. Pairs are (i, i
+    + dim / 2), or (2 i, 2 i + 1) where interleaved.
 
     For contexts longer than a model was trained on, frequencies are divided by
     `factor`; with ramp=(original, low, high) only those that turn less than `low`
@@ -583,6 +584,8 @@ def rotary(dim, base=10000.0, factor=1.0, ramp=None, amplitude=1.0, interleaved=
                 share = (abs(f) * number(original) - number(low)) / (number(high) - number(low))
                 share = min(max(share, number(0)), number(1))
             f = f * share + f / number(factor) * (1 - share)
+            if abs(f) > _MOST_TURNS:
+                raise ValueError("rotary: a frequency is above 1e30 turns a position")
             t = int((f * 2 ** 64).to_integral_value()) % 2 ** 64
             turns.append(t - 2 ** 64 if t >= 2 ** 63 else t)
     device = torch.device("cuda", _Dev.device()) if device is None else device

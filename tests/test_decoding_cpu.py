@@ -375,6 +375,20 @@ def test_rotary_turns():
     assert abs(abs(int(turns[1])) / 2 ** 64 - 0.5) < 1e-14
 
 
+def test_rotary_of_high_frequencies():
+    """Whole turns in any number that 50 digits of pi leave a fraction of; more are refused."""
+    with decimal.localcontext(decimal.Context(prec=80)):
+        pi2 = 2 * decimal.Decimal("3.1415926535897932384626433832795028841971693993751058209749445923")
+        for f in (1e6, 1e15, -1e20, 1e29, 6e30):
+            t = int(workloads.rotary(2, frequencies=[f], device="cpu").turns[0])
+            off = int((decimal.Decimal(f) / pi2 * 2 ** 64).to_integral_value()) - t
+            assert min(off % 2 ** 64, -off % 2 ** 64) <= 1, f
+    for kw in ({"frequencies": [1.0, -1e31]}, {"frequencies": [1e300, 0.0]}, {"factor": 1e-31},
+               {"base": 1e-64}, {"frequencies": [1e20, 1.0], "factor": 1e-12},
+               {"factor": 1e-31, "ramp": (4096, 1000.0, 2000.0)}):
+        refused(ValueError, "1e30 turns", workloads.rotary, 4, device="cpu", **kw)
+
+
 def test_rotate_definition():
     """Turning by p and q is turning by p + q, and back again by -(p + q)."""
     x = torch.randn(1, 2, 3, 8, generator=torch.Generator().manual_seed(0))
