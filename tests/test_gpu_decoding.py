@@ -726,3 +726,148 @@ def test_q4_outputs_beside_their_inputs(M):
     with pytest.raises(ValueError, match="overlaps"):
         W().q4_gated(b, gated, out=base[1:2 * M:2, 224:256])
     assert torch.equal(base, kept)
+
+
+# ---------------------------------------------------------------------------
+# the instances and loops that large sizes take
+# ---------------------------------------------------------------------------
+def tiles_of(outputs, gated=False):
+    return -(-outputs // 16) * (2 if gated else 1)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("M,N", [(1, 2100), (16, 2100), (4, 33000), (5, 16500), (20, 8200), (40, 8200)])
+def test_q4_matmul_of_many_outputs(dtype, group, M, N):
+    """More than 128 tiles of weights (two a wave), 1024 and 2048 (four a wave, few
+    waves), and for 17 rows and more 512 (four a wave); of nine blocks of columns the
+    first waves have two."""
+    assert tiles_of(N) in (132, 513, 1032, 2063)
+    raw = weights(N, 1152, group, zeros=M % 2 > 0, dtype=dtype, seed=M)
+    check_q4(rnd(M, 1152, dtype=dtype, seed=M + 1), raw)
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("M,F,act", [(1, 1100, "silu"), (1, 16400, "gelu"), (9, 8200, "silu"),
+                                     (20, 4100, "gelu"), (48, 4100, "silu")])
+def test_q4_gated_of_many_outputs(group, M, F, act):
+    raw = weights(2 * F, 1152, group, dtype=BF16, seed=M + F)
+    x = rnd(M, 1152, dtype=BF16, seed=3, scale=0.25)
+    check_gated(x, raw, act)
+
+
+def check_gated(x, raw, act):
+    got = W().q4_gated(x, on_gpu(*raw, gated=True), act=act).double().cpu()
+    y, bound = q4_bound(x.cpu(), *raw)
+    F = y.shape[1] // 2
+    gate, up = y[:, :F], y[:, F:]
+    a = orc.activate(gate, act)
+    want = a * up
+    # slopes below 1.13, 8 roundings of fp32 in the activation, as in test_q4_gated
+    fp32 = (1.13 * bound[:, :F] + 8 * EPS * gate.abs()) * (up.abs() + bound[:, F:]) \
+        + a.abs() * bound[:, F:]
+    tiny = 2.0 ** -25 if x.dtype == F16 else 0.0
+    assert bool(((got - want).abs() <= fp32 + (want.abs() + fp32) * half_step(x.dtype) + tiny).all())
+
+
+def parts(M, N, K, group, act=0):
+    """How many parts q4_many splits the columns into, from what it asks for."""
+    from newt_amd import serving
+    need = serving.lib().newt_q4_matmul_workspace(serving._Q4.pack(
+        *[4096] * 4, 0, 4096, 0, M, K, N, K, N, group, 2, 2, 2, act, 0))
+    return need // (4 * M * tiles_of(N, act > 0) * 16) or 1
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("group,K", [(32, 2080), (64, 2112), (128, 2176)])
+def test_q4_matmul_many_rows_long_programs(dtype, group, K):
+    """17 blocks of columns in a program, the last one ragged: each stage of LDS and
+    each set of sums is used again and again."""
+    M, N = 500, 8190
+    assert parts(M, N, K, group) == 1 and -(-K // 128) == 17
+    raw = weights(N, K, group, zeros=dtype == F16, dtype=dtype, seed=K)
+    check_q4(rnd(M, K, dtype=dtype, seed=1), raw)
+
+
+@pytest.mark.parametrize("group,N,K", [(32, 4003, 9312), (64, 2003, 8000), (128, 2003, 16384)])
+def test_q4_matmul_many_rows_long_parts(group, N, K):
+    """Parts of seven blocks and more, the last one shorter."""
+    M = 130
+    n = parts(M, N, K, group)
+    assert n > 1 and -(-K // 128) // n >= 7, n
+    raw = weights(N, K, group, seed=K)
+    check_q4(rnd(M, K, dtype=BF16, seed=1), raw)
+    odd = rnd(M, K + 3, dtype=BF16, seed=2)[:, 3:]  # not aligned to 16 bytes
+    check_q4(odd, raw)
+
+
+@pytest.mark.parametrize("group,K", [(32, 1056), (64, 1728), (128, 1664)])
+def test_q4_gated_many_rows_long_programs(group, K):
+    M, F = 500, 4090
+    assert parts(M, F, K, group, 1) == 1
+    check_gated(rnd(M, K, dtype=BF16, seed=1, scale=0.25), weights(2 * F, K, group, seed=K), "silu")
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("D,dim,S", [(128, 128, 2100), (128, 64, 2100), (80, 40, 3500)])
+def test_rotate_two_heads_a_thread(dtype, interleaved, D, dim, S):
+    """As many tokens as give a thread two heads, an odd number of heads in all."""
+    w = W()
+    H, KV = 32, 1
+    wide = 16 // dtype.itemsize
+    V = wide if dim % (2 * wide) == 0 else 4
+    units = dim // 2 // V + -(-(D - dim) // V)
+    assert units * S * (H + KV) >= 2 * 256 * 1024
+    rot = w.rotary(dim, interleaved=interleaved)
+    q, k = rnd(1, H, S, D, dtype=dtype, seed=1), rnd(1, KV, S, D, dtype=dtype, seed=2)
+    at = ints([5])[:, None] + torch.arange(S, device="cuda")
+    for o, x in zip(w.rotate(q, k, rot, ints([5])), (q, k)):
+        check_rotated(o, x, orc.frequencies(dim), at, interleaved=interleaved)
+    # the same in place, and heads of more than one tensor in a thread
+    want = w.rotate(q, k, rot, ints([5]))
+    w.rotate(q, k, rot, ints([5]), q_out=q, k_out=k)
+    assert torch.equal(q, want[0]) and torch.equal(k, want[1])
+
+
+# ---------------------------------------------------------------------------
+# rows of logits with little to choose
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("T,V", [(3, 3000), (3, 90000), (150, 20001)])
+def test_sample_of_few_tokens_with_weight(dtype, T, V):
+    """Fewer tokens than top_k that are not masked, or that have any weight at a low
+    temperature."""
+    x = rnd(T, V, dtype=dtype, seed=V, scale=2.5)
+    u = uniform(T, 3)
+    few = torch.full_like(x, -INF)
+    for r in range(T):
+        n = 5 + 7 * r % 26
+        at = torch.randperm(V, generator=torch.Generator().manual_seed(r))[:n].cuda()
+        few[r, at] = x[r, at]
+    rows = slice(None, None, 1 + T // 40)
+    for settings in ({"top_k": 50, "top_p": 0.9}, {"top_k": 50}, {"top_k": 5, "top_p": 0.99},
+                     {"top_k": 30, "top_p": 0.5, "min_p": 0.02}, {"top_p": 0.9}):
+        check_rows(few, u, rows, settings)
+    low = torch.finfo(dtype).min
+    check_rows(few.clamp(min=low), u, rows, {"top_k": 50, "top_p": 0.9})
+    for temperature in (0.02, 0.05, 0.1, 0.2):
+        check_rows(x, u, rows, {"temperature": temperature, "top_k": 50, "top_p": 0.9})
+        check_rows(x, u, rows, {"temperature": temperature, "top_k": 2000, "top_p": 0.999,
+                                "min_p": 0.001})
+
+
+def check_rows(logits, u, rows, settings):
+    got = W().sample(logits, u, **settings)[rows].tolist()
+    row = {k: v if k == "top_k" else torch.tensor(v, dtype=F32).item() for k, v in settings.items()}
+    for g, x, v in zip(got, logits[rows], u[rows].tolist()):
+        assert g == orc.sample(x, v, **row), settings
+
+
+def test_sample_top_k_beyond_the_list():
+    """A bin that fits a list, behind more tokens than fit one."""
+    x = rnd(4, 40000, seed=21)
+    for V in (40000, 20000):
+        for top_k in (4095, 4097, 9000, 15000):
+            for settings in ({}, {"top_p": 0.9}, {"top_p": 0.3, "min_p": 0.1}):
+                check_rows(x[:, :V], uniform(4, 1), slice(None), {"top_k": top_k, **settings})
