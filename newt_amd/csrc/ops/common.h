@@ -22,10 +22,13 @@ int hip_fail(hipError_t e, const char* what);
 template <typename T> struct same { typedef T type; };
 
 // Launches a kernel and gives this launch's own status: what other code's
-// calls have left behind is not looked at.
+// calls have left behind is not looked at. Of 2^32 work-items and more the runtime
+// leaves some out without an error.
 template <typename... P>
 int run(const char* what, void (*kernel)(P...), int64_t grid, int block, unsigned lds,
         hipStream_t stream, typename same<P>::type... args) {
+  if (grid * block > 0xffffffffll)
+    return fail(NEWT_ERR_INVALID, "%s: more than a launch takes", what);
   void* list[] = {static_cast<void*>(&args)...};
   const hipError_t e = hipLaunchKernel(reinterpret_cast<const void*>(kernel),
                                        dim3((unsigned)grid), dim3((unsigned)block), list, lds,

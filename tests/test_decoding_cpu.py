@@ -329,6 +329,20 @@ def test_empty_calls_launch_nothing():
     assert L.newt_sample_workspace(0, 100000, 2) == 0
 
 
+def test_launches_of_too_many_programs_are_refused():
+    """2^32 work-items and more, of which the runtime would leave some out: rows that
+    no memory holds, but for a stride of 0. Nothing is launched."""
+    L = serving.lib()
+    P = 4096
+    rows = (1 << 31) - 1
+    sizes = serving._RMSNORM.pack(P, 0, P, P, 0, 0, rows, 64, 0, 0, 64, 0, 1e-6, 2, 2, 2, 0, 0)
+    q4 = serving._Q4.pack(P, P, P, 0, 0, 1 << 40, 0, 40, 64, (1 << 30) - 1, 0, 1 << 30, 64, 2, 2, 2, 0,
+                          0)
+    for entry, params in ((L.newt_rmsnorm, sizes), (L.newt_q4_matmul, q4)):
+        assert entry(params, None) == 10002
+        assert b"more than a launch takes" in L.newt_ops_last_error(), L.newt_ops_last_error()
+
+
 # ---------------------------------------------------------------------------
 # layouts and definitions
 # ---------------------------------------------------------------------------
