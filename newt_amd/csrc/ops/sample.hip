@@ -1029,7 +1029,23 @@ template <typename T>
 int launch(const newt_sample_params& p, int shift, hipStream_t stream) {
   const char* const what = "newt_sample";
   const int parts = parts_of(p.rows, p.vocab, p.dtype);
-  if (parts == 1) return run(what, sample_kernel<T>, p.rows, kThreads, 0, stream, p, shift);
+  if (parts == 1) {
+    int status = NEWT_OK;
+    constexpr int64_t kMost = 1 << 21;  // programs of a launch: 2^31 work-items
+    for (int64_t r = 0; r < p.rows && status == NEWT_OK; r += kMost) {
+      newt_sample_params some = p;
+      some.rows = p.rows - r < kMost ? p.rows - r : kMost;
+      some.logits = (const T*)p.logits + r * p.stride;
+      some.u += r;
+      some.ids += r;
+      if (p.temperature) some.temperature += r;
+      if (p.top_k) some.top_k += r;
+      if (p.top_p) some.top_p += r;
+      if (p.min_p) some.min_p += r;
+      status = run(what, sample_kernel<T>, some.rows, kThreads, 0, stream, some, shift);
+    }
+    return status;
+  }
   if (!p.workspace || ((uintptr_t)p.workspace & 7))
     return fail(NEWT_ERR_INVALID, "newt_sample: null or unaligned workspace");
   int status = run(what, part_top_kernel<T>, p.rows * parts, kThreads, 0, stream, p, parts, shift);

@@ -871,3 +871,19 @@ def test_sample_top_k_beyond_the_list():
         for top_k in (4095, 4097, 9000, 15000):
             for settings in ({}, {"top_p": 0.9}, {"top_p": 0.3, "min_p": 0.1}):
                 check_rows(x[:, :V], uniform(4, 1), slice(None), {"top_k": top_k, **settings})
+
+
+def test_sample_more_rows_than_a_launch_takes():
+    """2^22 programs of 1024 threads are 2^32 work-items."""
+    T = (1 << 22) + 70
+    x = rnd(97, 5, seed=22, scale=2.0).repeat(T // 97 + 1, 1)[:T]
+    u = uniform(97, 23).repeat(T // 97 + 1)[:T]
+    t = torch.tensor([0.0, 0.7, 1.5], device="cuda").repeat(T // 3 + 1)[:T]
+    k = torch.tensor([0, 2, 3, 5], dtype=torch.int32, device="cuda").repeat(T // 4 + 1)[:T]
+    for settings in ({"top_p": 0.8}, {"temperature": t, "top_k": k}):
+        ids = W().sample(x, u, **settings)
+        n = 97 * 12  # rows until everything comes again
+        few = {name: v[:n] if isinstance(v, torch.Tensor) else v for name, v in settings.items()}
+        again = W().sample(x[:n], u[:n], **few)
+        assert torch.equal(ids, again.repeat(T // n + 1)[:T])
+    check_rows(x, u, slice(T - 40, T), {"top_p": 0.8})
