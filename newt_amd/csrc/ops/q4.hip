@@ -16,8 +16,8 @@
 // A wave takes NT tiles of 16 weight rows, MT tiles of 16 rows of x and every
 // WAVES-th block of 128 columns; the waves' sums are joined in LDS in their order.
 // bf16, groups of 128, three sets of weights in turn: 1 x 4096 x 6144 5.8 us (2.3 TB/s);
-// gated 1 x 4096 x 2 x 12288 11.7 us (4.5 TB/s); 4 x 4096 x 128000 to fp32 53.4 us
-// (5.1 TB/s; the same weights again 46).
+// gated 1 x 4096 x 2 x 12288 11.6 us (4.6 TB/s); 4 x 4096 x 128000 to fp32 53.8 us
+// (5.1 TB/s; the same weights again 45).
 #include "q4.h"
 
 namespace newt_ops {
@@ -218,7 +218,9 @@ int by_act(const newt_q4_params& p, hipStream_t stream) {
 
 // more take the tiles of q4_many.hip: us for 64 rows, gated, 4096 x 2 x 12288 bf16 44
 // here, 32 there; 2048 x 2 x 5504 fp16, groups of 64, 17 and 22; 48 rows of the first
-// 31 and 31, of the second 11.6 and 19.7
+// 31 and 31, of the second 11.6 and 19.7. One border for all sizes is a compromise: 48
+// rows here and 49 there take 34 and 33 for the first, 11.5 and 20 for the second, 16 and
+// 20 for 4096 x 6144, 143 and 93 for 4096 x 128000.
 constexpr int64_t kFewRows = 48;
 
 const char* wrong(const newt_q4_params& p) {

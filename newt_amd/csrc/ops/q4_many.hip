@@ -14,7 +14,7 @@
 // as large.
 // Few programs split the columns; a second kernel adds the parts in their order.
 // bf16 512 x 4096 x 2 x 12288, gated, groups of 128: 123 us, 838 TFLOP/s (119 on
-// another card); groups of 64 155, of 32 216 us. The products alone, with nothing
+// another card); groups of 64 154, of 32 213 us. The products alone, with nothing
 // loaded, widened or scaled, took 83 us of 121 (an eighth of them is what is taken
 // off): under them the chip's power lets the clock fall to 1.5 GHz or so. Beside
 // that, one at a time, the scales cost 8%, loading x 6%, its sums 5% (before they

@@ -4,15 +4,26 @@
 // What is kept is the beginning of the logits in falling order, of which only the
 // part around its end is ever put in order: a histogram over (max - x) / T finds
 // the bin in which the last kept one lies, and the few logits of that bin are
-// sorted in LDS (or, with top_k, all up to it, where LDS holds them). Where a bin
-// holds too many, finer histograms over the bits of its logits take its place. A
-// token chosen by its running weight is found by sums of segments, of which one is
-// read again.
-// The vector unit bounds long rows: an exponential in 64 bits takes a dozen fp64
-// instructions (by a table of 2048 and a polynomial of degree 4), and top_p needs two
-// of them a logit. bf16 256 x 100003 by top_p: 53 us, without a filter 30; 64 x 32000
-// fp32 with settings of each row's own 22; 1 x 128000 with all three filters 27, in
-// four kernels of 3 + 5 + 9 + 12 us, each a chain of short steps.
+// sorted in LDS (or, with top_k, all up to it, where LDS holds them). A token chosen
+// by its running weight is found by sums of segments, of which one is read again.
+// Three kinds of rows go another way (kSlow), over finer and finer histograms of the
+// bits of the logits, in one program and without haste:
+//   - the bin of the end holds more than a list (all equal, or a huge temperature);
+//   - top_k together with top_p, and more than a list up to top_k's end;
+//   - top_k together with top_p, and fewer than top_k tokens within 32 temperatures
+//     of the largest logit: masked rows, or low temperatures.
+// The third is the commonest: by top_k 50 and top_p 0.9 at temperatures of 0.75 / 0.2 /
+// 0.05 1 x 128000 bf16 takes 26 / 71 / 160 us, 64 x 32000 fp32 18 / 52 / 53, 256 x 100003
+// bf16 38 / 155 / 247. At 0.75 with a top_k of 5000 it is 269, 103 and 389, at 50 by top_p
+// alone 405, 58 and 457.
+// Long rows are bound by the vector unit, which issues in 64% of the cycles, and by
+// LDS: an exponential in 64 bits takes a dozen fp64 instructions (by a table of 2048
+// and a polynomial of degree 4), and top_p needs two of them a logit; the histogram's
+// 64-bit atomics make two thirds of the LDS' active cycles bank conflicts. bf16 256 x
+// 100003 by top_p: 54 us, without a filter 31, greedy, which reads a row twice, 20; 64 x
+// 32000 fp32 with settings of each row's own 22, greedy 6; 1 x 128000 with all three
+// filters 27, in four kernels of 3 + 5 + 8 + 12 us, each a chain of short steps, greedy
+// 11.
 // Weights are whole numbers of 2^-45 (less for more than 2^17 ids), from
 // exponentials in 64 bits: their sums are exact, whatever the order in which
 // atomics add them, so the same row gives the same id in every call, and a border is
@@ -1009,6 +1020,9 @@ __global__ void __launch_bounds__(kThreads) part_choose_kernel(newt_sample_param
 //   1 x 128000 bf16: no filter 28 / 17, top_p 56 / 37, all three 35 / 34;
 //   16 x 128000, settings of each row's own: 74 / 53; 64 x 128000, top_p 69 / 55;
 //   64 x 32000 fp32, settings of each row's own: 28 / 37; 16 x 32000 bf16 28 / 36.
+// Between the two lengths nothing decided where the border lies: one row by all three
+// filters takes 22 us of 50000, 24 of 65535 and 28, in several, of 65536. From 129 rows
+// on a row has one program, 129 to 255 of 100003 logits by top_p 50 to 54 us.
 int parts_of(int64_t rows, int64_t vocab, int dtype) {
   const int64_t chunk = dtype == NEWT_F32 ? 256 : 512;
   int64_t n = rows && vocab >= 65536 ? 256 / rows : 1;

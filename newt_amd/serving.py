@@ -17,10 +17,11 @@ range) before anything is launched.
 One step of a decoder layer over the 8-bit cache:
 
     x, _, hidden = rmsnorm(x, w_norm, residual=hidden)
-    q, k, v = ...                      # slices of q4_matmul(x, w_qkv)
-    q, k = rotate(q, k, positions_of, lens - k.shape[2])
-    kv_append(cache, k, v, block_table, lens - k.shape[2])
+    q, k, v = ...                      # slices of q4_matmul(x, w_qkv), [B, heads, S, D]
+    q, k = rotate(q, k, turns, lens - S)             # turns = rotary(D), once
+    kv_append(cache, k, v, block_table, lens - S)
     o = cached_attention(q, cache, block_table, lens)
+    o = o.transpose(1, 2).reshape(B * S, -1)         # a row a token again
     x, _, hidden = rmsnorm(q4_matmul(o, w_out), w_norm2, residual=hidden)
     x = q4_matmul(q4_gated(x, w_gate_up), w_down)
 
@@ -784,10 +785,12 @@ def q4_matmul(x, w, bias=None, out_dtype=None, out=None):
     """x [M, K] fp16 or bf16, rows of any stride, times the transposed 4-bit
     weights (q4_weights): [M, N] of x's dtype or, with out_dtype=float32, fp32. bias
     [N] is of x's dtype. Products are summed in fp32 and multiplied there by their
-    group's scale; the result is rounded once. For few rows the weights are read
-    once; for many, matmul over weights of 16 bits is faster. A row of x that holds
-    an infinity or NaN gives no numbers. An `out` given shares no memory with x or
-    bias."""
+    group's scale; the result is rounded once. The sums hold x (16 + number) and x
+    (16 + zero), so their roundings count against the sum of |x| (32 + number + zero)
+    |scale|, not against the result: a large x whose weights are all 0 still costs the
+    others precision. For few rows the weights are read once; for hundreds, matmul is
+    faster where a program has the weights in 16 bits too. A row of x that holds an
+    infinity or NaN gives no numbers. An `out` given shares no memory with x or bias."""
     r = _fast("q4_matmul", x, w, bias, -1 if out_dtype is None else _DTYPE.get(out_dtype, -2), out)
     if r is not None:
         return r
